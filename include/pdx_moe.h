@@ -310,6 +310,106 @@ int pdx_moe_layer(const void *x, const void *gate, int64_t T, int64_t H, int64_t
                   pdx_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (MXFP4).  No counterpart in the reference,
+ * whose experts are BF16.  A block is 32 consecutive values of a row: one E8M0
+ * scale byte b (2^(b - 127)) and 32 E2M1 codes, two per byte, the even element
+ * in the low nibble.  b = max(floor(log2 max|x|) - 2 + 127, 0), codes round to
+ * nearest even and saturate at 6; a block that holds an infinity or NaN gets
+ * b = 255 and reads back as NaN.
+ * rows x cols values with row stride ld (elements, >= cols; unit stride within
+ * a row); cols a multiple of 32.  codes: dense [rows, cols/2], 4-byte aligned,
+ * scales: dense [rows, cols/32].  rows = 0 does nothing. */
+#define PDX_DTYPE_BF16 0
+#define PDX_DTYPE_FP16 1
+#define PDX_DTYPE_FP32 2
+int pdx_mxfp4_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, void *codes,
+                       void *scales, pdx_stream_t stream);
+int pdx_mxfp4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t cols, int64_t ld,
+                         int32_t dtype, void *out, pdx_stream_t stream);
+
+/* MXFP4 experts, the 4-bit form of pdx_expert_weights.  With Hp, Ip = H, I
+ * rounded up to 128, slot s holds
+ *   codes  + s*code_stride:  gate [Ip, Hp/2] | up [Ip, Hp/2] | down [Hp, Ip/2]
+ *   scales + s*scale_stride: the scales of gate | up | down, 3*Ip*Hp/32 bytes
+ * (strides in bytes, padding rows and columns zero).  A projection's scales
+ * are stored as tiles of 128 rows x 128 columns, 512 bytes each, row tiles
+ * outermost: byte (r % 32)*16 + (r / 32)*4 + c / 32 of a tile belongs to row r
+ * and columns c .. c + 31.  codes 128-byte, scales 16-byte aligned;
+ * code_stride a multiple of Hp/2 and of Ip/2, scale_stride of 16. */
+typedef struct pdx_mxfp4_weights {
+    const void *codes;
+    const void *scales;
+    int64_t code_stride;
+    int64_t scale_stride;
+    int64_t num_slots;
+    const int32_t *slot_of_expert; /* device int32[E] or NULL */
+} pdx_mxfp4_weights;
+
+/* pdx_moe_ffn_grouped on MXFP4 experts:
+ *   y[p] = bf16( Wd (silu(Wg x) * (Wu x)) ),  x = x[tokens[p]] (BF16)
+ * with exactly dequantised weights, FP32 sums and one rounding at the end.
+ * H, I multiples of 32; rows of no active expert are left as they are. */
+size_t pdx_mxfp4_ffn_workspace_bytes(int64_t rows, int64_t E, int64_t H, int64_t I);
+int pdx_mxfp4_ffn_grouped(const void *x, int64_t T, const int32_t *tokens, const int32_t *offsets,
+                          const int32_t *active, int64_t E, int64_t rows, const pdx_mxfp4_weights *weights,
+                          int64_t H, int64_t I, void *y_out, void *workspace, size_t workspace_bytes,
+                          pdx_stream_t stream);
+
+/* pdx_moe_layer on MXFP4 experts; flags: 0 or PDX_LAYER_OUT_NORM. */
+size_t pdx_mxfp4_layer_workspace_bytes(int64_t T, int64_t H, int64_t E, int32_t top_k, int64_t I);
+int pdx_mxfp4_moe_layer(const void *x, const void *gate, int64_t T, int64_t H, int64_t E, int32_t top_k,
+                        int32_t normalize, const pdx_mxfp4_weights *weights, int64_t I, const void *residual,
+                        void *out, void *logits_out, int64_t *selected_out, void *weights_out, int32_t *counts_out,
+                        int32_t flags, void *workspace, size_t workspace_bytes, pdx_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * The norms before and after a block, its gate and the residual scale in one
+ * pass (the decoder-layer steps around the MoE path that the reference leaves
+ * to its host model).  Per row, in FP32, each output rounded once:
+ *   z = post(y) * post_weight
+ *   s = residual_scale * residual + block_scale * act(gate) * z  -> stream_out
+ *   n = pre(s) * pre_weight                                      -> normed_out
+ * post, pre: PDX_NORM_NONE, _RMS (v / sqrt(mean(v^2) + eps)) or _LAYER
+ * ((v - mean) / sqrt(var + eps), population variance); weights BF16 [H] or
+ * NULL (ones).  gate: BF16 with element strides gate_row, gate_col (0 =
+ * broadcast), or NULL; gate_sigmoid applies the logistic function to it.
+ * y BF16 [T, H], or NULL: s = residual_scale * residual.  residual and
+ * stream_out are FP32 if residual_fp32, else BF16; normed_out is BF16; either
+ * output may be NULL and may alias y or residual of the same type.
+ * 1 <= H <= 8192. */
+#define PDX_NORM_NONE 0
+#define PDX_NORM_RMS 1
+#define PDX_NORM_LAYER 2
+typedef struct pdx_block_norm_args {
+    int32_t post, pre;
+    const void *post_weight, *pre_weight;
+    const void *gate;
+    int64_t gate_row, gate_col;
+    int32_t gate_sigmoid, residual_fp32;
+    float residual_scale, block_scale, eps;
+} pdx_block_norm_args;
+int pdx_block_norm(const void *y, const void *residual, int64_t T, int64_t H, const pdx_block_norm_args *args,
+                   void *stream_out, void *normed_out, pdx_stream_t stream);
+
+/* The same with y[t] = sum_s weights[t,s] * rows[inverse[t*k+s]] formed in
+ * FP32 (the combine of the expert rows).  Entries of inverse outside
+ * [0, y_rows) raise PDX_DEVERR_BAD_EXPERT and count as zero rows.  Outputs must
+ * not alias rows. */
+int pdx_combine_block_norm(const void *rows, int64_t y_rows, const void *weights, const int32_t *inverse, int64_t T,
+                           int32_t top_k, int64_t H, const void *residual, const pdx_block_norm_args *args,
+                           void *stream_out, void *normed_out, pdx_stream_t stream);
+
+/* A whole MoE block of a stack: route -> pack -> grouped FFN on x (the normed
+ * activation), then pdx_combine_block_norm on the residual stream.  Exactly one
+ * of weights and mxfp4 is given; mode as pdx_moe_ffn_grouped (0 with mxfp4).
+ * Workspace: pdx_layer_workspace_bytes or pdx_mxfp4_layer_workspace_bytes. */
+int pdx_moe_block(const void *x, const void *gate, int64_t T, int64_t H, int64_t E, int32_t top_k, int32_t normalize,
+                  const pdx_expert_weights *weights, const pdx_mxfp4_weights *mxfp4, int64_t I, const void *residual,
+                  const pdx_block_norm_args *args, void *stream_out, void *normed_out, void *logits_out,
+                  int64_t *selected_out, void *weights_out, int32_t *counts_out, int32_t mode, void *workspace,
+                  size_t workspace_bytes, pdx_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Expert parallelism.  No counterpart in the reference (single-GPU); these
  * lay the same layer out over `ranks` GPUs with expert e on rank e / EL,
  * EL = E / ranks; the exchange itself is NCCL all-to-all (see

@@ -7,11 +7,16 @@ rebuild it); the first use of any runtime name loads it and raises if it is
 missing -- there is no fallback.
 """
 _RUNTIME_NAMES = ("PDScopeCudaRuntime", "PdxGpuBackend", "ExpertSlab", "ResidentMoELayer", "Routing", "combine",
-                  "compact_expert_groups", "expert_forward", "expert_groups", "pack", "route", "topk_from_logits")
+                  "compact_expert_groups", "expert_forward", "expert_groups", "pack", "route", "topk_from_logits",
+                  "BlockNorm", "block_norm", "combine_block_norm")
+_MXFP4_NAMES = ("Mxfp4", "Mxfp4ExpertSlab", "dequantize_mxfp4", "moe_ffn_mxfp4", "quantize_mxfp4")
 
 
 def __getattr__(name):
     if name in _RUNTIME_NAMES:
         from . import runtime
         return getattr(runtime, name)
+    if name in _MXFP4_NAMES:
+        from . import mxfp4
+        return getattr(mxfp4, name)
     raise AttributeError(name)

@@ -27,6 +27,9 @@ PDX_DEVERR_BAD_SLOT = 3
 FFN_AUTO, FFN_GEMV, FFN_GEMM, FFN_SIMT, FFN_GEMM_1CTA, FFN_GEMM_PAIR, FFN_GEMV_STAGED = 0, 1, 2, 3, 4, 5, 6
 LAYER_OUT_NORM = 0x100   # OR into pdx_moe_layer's mode: out = layer_norm(MoE(x) + residual)
 
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
 ABI_VERSION = 1
 
 c_i64 = ctypes.c_int64
@@ -40,6 +43,19 @@ class ExpertWeights(ctypes.Structure):
     _fields_ = [("gate", c_vp), ("up", c_vp), ("down", c_vp),
                 ("gate_stride", c_i64), ("up_stride", c_i64), ("down_stride", c_i64),
                 ("num_slots", c_i64), ("slot_of_expert", c_vp)]
+
+
+class Mxfp4Weights(ctypes.Structure):
+    """pdx_mxfp4_weights."""
+    _fields_ = [("codes", c_vp), ("scales", c_vp), ("code_stride", c_i64), ("scale_stride", c_i64),
+                ("num_slots", c_i64), ("slot_of_expert", c_vp)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """pdx_block_norm_args."""
+    _fields_ = [("post", c_i32), ("pre", c_i32), ("post_weight", c_vp), ("pre_weight", c_vp), ("gate", c_vp),
+                ("gate_row", c_i64), ("gate_col", c_i64), ("gate_sigmoid", c_i32), ("residual_fp32", c_i32),
+                ("residual_scale", ctypes.c_float), ("block_scale", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
 class OffloadConfig(ctypes.Structure):
@@ -103,6 +119,21 @@ SIGNATURES = {
     "pdx_moe_layer": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32,
                                      ctypes.POINTER(ExpertWeights), c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                      c_i32, c_vp, c_sz, c_vp]),
+    "pdx_mxfp4_quantize": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "pdx_mxfp4_dequantize": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_vp]),
+    "pdx_mxfp4_ffn_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64]),
+    "pdx_mxfp4_ffn_grouped": (ctypes.c_int, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64,
+                                             ctypes.POINTER(Mxfp4Weights), c_i64, c_i64, c_vp, c_vp, c_sz, c_vp]),
+    "pdx_mxfp4_layer_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i32, c_i64]),
+    "pdx_mxfp4_moe_layer": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32,
+                                           ctypes.POINTER(Mxfp4Weights), c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                           c_i32, c_vp, c_sz, c_vp]),
+    "pdx_block_norm": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, ctypes.POINTER(BlockNormArgs), c_vp, c_vp, c_vp]),
+    "pdx_combine_block_norm": (ctypes.c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i64, c_vp,
+                                              ctypes.POINTER(BlockNormArgs), c_vp, c_vp, c_vp]),
+    "pdx_moe_block": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, ctypes.POINTER(ExpertWeights),
+                                     ctypes.POINTER(Mxfp4Weights), c_i64, c_vp, ctypes.POINTER(BlockNormArgs), c_vp,
+                                     c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_sz, c_vp]),
     "pdx_ep_dispatch": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i64, c_i64, c_i32, c_i64, c_vp, c_vp,
                                        c_vp]),
     "pdx_ep_layout": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp]),

@@ -15,10 +15,11 @@
 #include <type_traits>
 #include <utility>
 
+#include "block_norm.cu"
 #include "combine.cu"
 #include "ffn_decode.cu"
 #include "ffn_gemm.cu"
-#include "ffn_gemv.cu"
+#include "ffn_mx4.cu"
 #include "ffn_stream.cu"
 #include "pack.cu"
 #include "ep.cu"
@@ -875,17 +876,240 @@ PackBufs carve_pack(Carver& c, int64_t T, int32_t k, int64_t E, int32_t* counts_
     return p;
 }
 
-}  // namespace
-}  // namespace pdx
-
-using namespace pdx;
-
 int check_norm_shape(int64_t H) {
     if (H < 8 || H % 8 || H > 8 * kLnThreads * (kLnMaxPerThread / 8))
         return fail(PDX_ERR_UNSUPPORTED, "layer norm needs H a multiple of 8 and <= %d",
                     8 * kLnThreads * (kLnMaxPerThread / 8));
     return PDX_OK;
 }
+
+// ---- MXFP4 ---------------------------------------------------------------------------
+int64_t round128(int64_t v) { return (v + 127) / 128 * 128; }
+
+int check_mx4_matrix(int64_t rows, int64_t cols, int64_t ld, int32_t dtype) {
+    if (dtype != PDX_DTYPE_BF16 && dtype != PDX_DTYPE_FP16 && dtype != PDX_DTYPE_FP32)
+        return fail(PDX_ERR_INVALID, "unknown dtype %d", dtype);
+    if (rows < 0 || cols < 1 || cols % kMxBlock)
+        return fail(PDX_ERR_INVALID, "MXFP4 needs rows of a positive multiple of 32 values (got %lld)",
+                    static_cast<long long>(cols));
+    if (ld < cols) return fail(PDX_ERR_INVALID, "row stride %lld shorter than a row", static_cast<long long>(ld));
+    if (rows > (int64_t(1) << 40) / cols) return fail(PDX_ERR_UNSUPPORTED, "matrix too large");
+    return PDX_OK;
+}
+
+bool mx4_aligned(const void* p, int64_t ld, int32_t dtype) {
+    const int64_t size = dtype == PDX_DTYPE_FP32 ? 4 : 2;
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld * size % 16 == 0;
+}
+
+template <typename F>
+cudaError_t with_mx4_type(int32_t dtype, bool aligned, F f) {
+    auto with_type = [&](auto type) { return aligned ? f(type, std::true_type{}) : f(type, std::false_type{}); };
+    if (dtype == PDX_DTYPE_BF16) return with_type(bf16{});
+    if (dtype == PDX_DTYPE_FP16) return with_type(__half{});
+    return with_type(float{});
+}
+
+dim3 mx4_grid(int64_t chunks) {
+    return dim3(static_cast<unsigned>(std::min<int64_t>((chunks + kMxThreads - 1) / kMxThreads, 16 * kPlanSMs)));
+}
+
+int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool gathered,
+                  const pdx_mxfp4_weights* w) {
+    if (T < 1 || rows < 1 || E < 1) return fail(PDX_ERR_INVALID, "empty FFN batch");
+    if (H < 32 || I < 32 || H % 32 || I % 32)
+        return fail(PDX_ERR_UNSUPPORTED, "H=%lld, I=%lld must be positive multiples of 32", static_cast<long long>(H),
+                    static_cast<long long>(I));
+    if (H > 65536 || I > 65536 || rows >= (int64_t(1) << 31) || T >= (int64_t(1) << 31) || E > (int64_t(1) << 20))
+        return fail(PDX_ERR_UNSUPPORTED, "FFN batch too large");
+    if (!gathered && T < rows) return fail(PDX_ERR_INVALID, "x has fewer rows than the packed order");
+    if (!w || !w->codes || !w->scales) return fail(PDX_ERR_INVALID, "expert weights missing");
+    if (w->num_slots < 1) return fail(PDX_ERR_INVALID, "num_slots must be >= 1");
+    const int64_t Hp = round128(H), Ip = round128(I);
+    if ((reinterpret_cast<uintptr_t>(w->codes) & 127u) || (reinterpret_cast<uintptr_t>(w->scales) & 15u))
+        return fail(PDX_ERR_INVALID, "codes must be 128-byte and scales 16-byte aligned");
+    if (w->num_slots > 1 && (w->code_stride < 3 * Hp * Ip / 2 || w->scale_stride < 3 * Hp * Ip / 32 ||
+                             w->code_stride % (Hp / 2) || w->code_stride % (Ip / 2) || w->scale_stride % 16))
+        return fail(PDX_ERR_INVALID, "slot strides must cover one expert and be whole rows");
+    return PDX_OK;
+}
+
+size_t mx4_ffn_ws_bytes(int64_t rows, int64_t E, int64_t H, int64_t I) {
+    return align_up(static_cast<size_t>(rows) * I * 4);
+}
+
+int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_t* offsets, const int32_t* active,
+                   int64_t E, int64_t rows, const pdx_mxfp4_weights* w, int64_t H, int64_t I, void* y, Carver& ws,
+                   cudaStream_t stream) {
+    float* h = static_cast<float*>(ws.take(static_cast<size_t>(rows) * I * 4));
+    if (ws.overflow) return fail(PDX_ERR_WORKSPACE, "FFN workspace too small (%zu > %zu bytes)", ws.used, ws.cap);
+    const Mx4Slab slab{static_cast<const uint8_t*>(w->codes), static_cast<const uint8_t*>(w->scales), w->code_stride,
+                       w->scale_stride, w->num_slots, w->slot_of_expert};
+    const int Hi = static_cast<int>(H), Ii = static_cast<int>(I), n = static_cast<int>(rows);
+    const int Hp = static_cast<int>(round128(H)), Ip = static_cast<int>(round128(I));
+    const unsigned split = rows < 1024 ? 16 : 1;
+    PDX_PDL_TRY(launch_pdl(k_mx4_gateup, dim3(n, split), dim3(256), 0, stream, static_cast<const uint16_t*>(x), tokens,
+                           static_cast<int>(T), offsets, active, slab, n, Hi, Ii, Hp, Ip, h));
+    PDX_PDL_TRY(launch_pdl(k_mx4_down, dim3(n, split), dim3(256), 0, stream, static_cast<const float*>(h), offsets,
+                           active, slab, n, Hi, Ii, Hp, Ip, static_cast<uint16_t*>(y)));
+    return PDX_OK;
+}
+
+// ---- block norms ---------------------------------------------------------------------
+int check_block_norm(const pdx_block_norm_args* a, const void* residual, int64_t T, int64_t H, const void* stream_out,
+                     const void* normed_out) {
+    if (!a || !residual) return fail(PDX_ERR_INVALID, "null block-norm argument");
+    if (!stream_out && !normed_out) return fail(PDX_ERR_INVALID, "block norm without an output");
+    if (T < 1 || T >= (int64_t(1) << 31)) return fail(PDX_ERR_INVALID, "empty block-norm batch");
+    if (H < 1 || H > kBnMaxH) return fail(PDX_ERR_UNSUPPORTED, "block norm needs 1 <= H <= %d", kBnMaxH);
+    if (a->post < PDX_NORM_NONE || a->post > PDX_NORM_LAYER || a->pre < PDX_NORM_NONE || a->pre > PDX_NORM_LAYER)
+        return fail(PDX_ERR_INVALID, "unknown norm");
+    if (!(a->eps > 0.f)) return fail(PDX_ERR_INVALID, "eps must be positive");
+    if (a->gate && (a->gate_row < 0 || a->gate_col < 0)) return fail(PDX_ERR_INVALID, "negative gate stride");
+    return PDX_OK;
+}
+
+BlockNormArgs to_block_norm(const pdx_block_norm_args* p, const void* residual, int64_t H, void* stream_out,
+                            void* normed_out) {
+    BlockNormArgs a{};
+    a.residual = residual;
+    a.post_weight = static_cast<const uint16_t*>(p->post_weight);
+    a.pre_weight = static_cast<const uint16_t*>(p->pre_weight);
+    a.gate = static_cast<const uint16_t*>(p->gate);
+    a.gate_row = p->gate_row;
+    a.gate_col = p->gate_col;
+    a.gate_sigmoid = p->gate_sigmoid;
+    a.post = p->post;
+    a.pre = p->pre;
+    a.residual_scale = p->residual_scale;
+    a.block_scale = p->block_scale;
+    a.eps = p->eps;
+    a.H = static_cast<int>(H);
+    a.stream = stream_out;
+    a.normed = static_cast<uint16_t*>(normed_out);
+    return a;
+}
+
+template <typename RES, bool COMBINE>
+cudaError_t launch_block_norm_typed(const BlockNormArgs& a, int64_t T, bool vec, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(T)), block(kBnThreads);
+    if (vec) {
+        if (a.H <= 8 * kBnThreads) return launch_pdl(k_block_norm<RES, COMBINE, 8, 1>, grid, block, 0, stream, a);
+        if (a.H <= 16 * kBnThreads) return launch_pdl(k_block_norm<RES, COMBINE, 8, 2>, grid, block, 0, stream, a);
+        return launch_pdl(k_block_norm<RES, COMBINE, 8, 4>, grid, block, 0, stream, a);
+    }
+    if (a.H <= 4 * kBnThreads) return launch_pdl(k_block_norm<RES, COMBINE, 1, 4>, grid, block, 0, stream, a);
+    return launch_pdl(k_block_norm<RES, COMBINE, 1, kBnMaxH / kBnThreads>, grid, block, 0, stream, a);
+}
+
+template <bool COMBINE>
+int launch_block_norm(const BlockNormArgs& a, int64_t T, bool fp32, cudaStream_t stream) {
+    // 16-byte accesses: whole vectors per row and every row pointer aligned
+    uintptr_t bits = reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual) |
+                     reinterpret_cast<uintptr_t>(a.post_weight) | reinterpret_cast<uintptr_t>(a.pre_weight) |
+                     reinterpret_cast<uintptr_t>(a.stream) | reinterpret_cast<uintptr_t>(a.normed);
+    if (a.gate && a.gate_col == 1) bits |= reinterpret_cast<uintptr_t>(a.gate) | static_cast<uintptr_t>(a.gate_row * 2);
+    const bool vec = a.H % 8 == 0 && (bits & 15u) == 0;
+    PDX_PDL_TRY((fp32 ? launch_block_norm_typed<float, COMBINE>(a, T, vec, stream)
+                      : launch_block_norm_typed<uint16_t, COMBINE>(a, T, vec, stream)));
+    return PDX_OK;
+}
+
+// ---- the layer up to its combine ------------------------------------------------------
+struct LayerRows {
+    uint16_t* y;
+    const uint16_t* weights;
+    const int32_t* inverse;
+};
+
+// workspace of routing, packing and the expert rows of one layer
+size_t layer_common_bytes(int64_t T, int64_t H, int64_t E, int32_t top_k) {
+    const int64_t N = T * top_k;
+    Carver c{nullptr, SIZE_MAX};
+    c.take(T * E * 2);           // logits
+    c.take(route_partial_bytes(T, E));
+    c.take(N * 8);               // selected
+    c.take(N * 2);               // weights
+    carve_pack(c, T, top_k, E, nullptr);
+    c.take(N * H * 2);           // y
+    return c.used;
+}
+
+int check_out_norm(bool out_norm, const void* residual, int64_t H) {
+    if (!out_norm) return PDX_OK;
+    if (!residual) return fail(PDX_ERR_INVALID, "PDX_LAYER_OUT_NORM needs a residual");
+    return check_norm_shape(H);
+}
+
+// route -> pack -> grouped FFN on the BF16 (weights) or MXFP4 (w4) experts.
+int layer_rows(const void* x, const void* gate, int64_t T, int64_t H, int64_t E, int32_t top_k, int32_t normalize,
+               const pdx_expert_weights* weights, const pdx_mxfp4_weights* w4, int64_t I, void* logits_out,
+               int64_t* selected_out, void* weights_out, int32_t* counts_out, int32_t mode, void* workspace,
+               size_t workspace_bytes, LayerRows& out, cudaStream_t stream) {
+    int st = check_route_shape(T, H, E, top_k);
+    if (st) return st;
+    if (!x || !gate) return fail(PDX_ERR_INVALID, "null layer argument");
+    const int64_t N = T * top_k;
+    const int m = w4 ? PDX_FFN_AUTO : resolve_mode(mode, N, E, H, I);
+    if (w4) {
+        if ((st = check_mx4_ffn(T, N, E, H, I, true, w4))) return st;
+    } else {
+        if ((st = check_ffn_shape(H, I, m))) return st;
+        if ((st = check_weights(weights, H, I))) return st;
+    }
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1)))
+        return fail(PDX_ERR_WORKSPACE, "workspace must be non-null and 256-byte aligned");
+    Carver c{static_cast<char*>(workspace), workspace_bytes};
+    RouteBufs rb;
+    rb.logits = logits_out ? static_cast<uint16_t*>(logits_out) : static_cast<uint16_t*>(c.take(T * E * 2));
+    rb.partials = static_cast<double*>(c.take(route_partial_bytes(T, E)));
+    rb.selected = selected_out ? selected_out : static_cast<int64_t*>(c.take(N * 8));
+    rb.weights = weights_out ? static_cast<uint16_t*>(weights_out) : static_cast<uint16_t*>(c.take(N * 2));
+    PackBufs pb = carve_pack(c, T, top_k, E, counts_out);
+    uint16_t* y = static_cast<uint16_t*>(c.take(N * H * 2));
+    // decode batches: both projections in one launch straight from x
+    const bool one_launch = !w4 && m == PDX_FFN_GEMV && decode_direct_ok(T, N, E, H, I, pb.o.tokens);
+    DecodeBufs db{};
+    if (one_launch) db = carve_decode(c, T, N, E, H, I, true);
+    if (c.overflow) return fail(PDX_ERR_WORKSPACE, "layer workspace too small (%zu > %zu bytes)", c.used, c.cap);
+    // the routing kernel also packs when the pack's shared memory fits the default 48 KiB
+    // (and then clears the single-launch FFN's tickets and counters)
+    const bool fused = T <= kTailMaxTokens && topk_pack_smem_bytes(E, N) <= 48 * 1024;
+    const bool zeroed = fused && one_launch;
+    if ((st = launch_route(x, gate, T, H, E, top_k, normalize, rb, fused ? &pb.o : nullptr, stream,
+                           zeroed ? db.counters : nullptr, zeroed ? db.plan.zero_words : 0)))
+        return st;
+    if (!fused && (st = launch_pack(rb.selected, rb.weights, T, top_k, E, pb.o, pb.chunk_hist, stream))) return st;
+    if (w4)
+        st = launch_mx4_ffn(x, T, pb.o.tokens, pb.o.offsets, pb.o.active, E, N, w4, H, I, y, c, stream);
+    else if (one_launch)
+        st = launch_decode_ffn(x, T, pb.o.tokens, pb.o.offsets, pb.o.active, N, weights, H, I, y, db, zeroed, stream);
+    else
+        st = launch_ffn(x, T, pb.o.tokens, pb.o.offsets, pb.o.active, E, N, weights, H, I, y, m, c, stream);
+    if (st) return st;
+    out = LayerRows{y, rb.weights, pb.o.inverse};
+    return PDX_OK;
+}
+
+int finish_layer(const LayerRows& r, int64_t T, int32_t top_k, int64_t H, const void* residual, bool out_norm,
+                 void* out, cudaStream_t stream) {
+    const int Ti = static_cast<int>(T), Hi = static_cast<int>(H), N = static_cast<int>(T * top_k);
+    const uint16_t* res = static_cast<const uint16_t*>(residual);
+    const dim3 grid(static_cast<unsigned>(T)), block(kCombineThreads);
+    if (out_norm)
+        PDX_PDL_TRY(launch_combine_norm(H, grid, block, 0, stream, static_cast<const uint16_t*>(r.y), r.weights,
+                                        r.inverse, Ti, static_cast<int>(top_k), Hi, N, res, PDX_LAYER_NORM_EPS,
+                                        static_cast<uint16_t*>(out)));
+    else
+        PDX_PDL_TRY(launch_pdl(k_combine, grid, block, 0, stream, static_cast<const uint16_t*>(r.y), r.weights,
+                               r.inverse, Ti, static_cast<int>(top_k), Hi, N, res, static_cast<uint16_t*>(out)));
+    return ok();
+}
+
+}  // namespace
+}  // namespace pdx
+
+using namespace pdx;
 
 extern "C" {
 
@@ -1087,15 +1311,8 @@ size_t pdx_layer_workspace_bytes(int64_t T, int64_t H, int64_t E, int32_t top_k,
     E = std::max<int64_t>(E, 1);
     top_k = std::max<int32_t>(top_k, 1);
     const int64_t N = T * top_k;
-    Carver c{nullptr, SIZE_MAX};
-    c.take(T * E * 2);           // logits
-    c.take(route_partial_bytes(T, E));
-    c.take(N * 8);               // selected
-    c.take(N * 2);               // weights
-    carve_pack(c, T, top_k, E, nullptr);
-    c.take(N * H * 2);           // y
     const int m = resolve_mode(mode, T * top_k, E, H, I);
-    return c.used + ffn_ws_bytes(N, E, H, I, m) + kAlign;
+    return layer_common_bytes(T, H, E, top_k) + ffn_ws_bytes(N, E, H, I, m) + kAlign;
 }
 
 int pdx_moe_layer(const void* x, const void* gate, int64_t T, int64_t H, int64_t E, int32_t top_k, int32_t normalize,
@@ -1104,59 +1321,141 @@ int pdx_moe_layer(const void* x, const void* gate, int64_t T, int64_t H, int64_t
                   size_t workspace_bytes, pdx_stream_t stream) {
     int st = check_route_shape(T, H, E, top_k);
     if (st) return st;
-    if (!x || !gate || !out) return fail(PDX_ERR_INVALID, "null layer argument");
+    if (!out) return fail(PDX_ERR_INVALID, "null layer argument");
     const bool out_norm = (mode & PDX_LAYER_OUT_NORM) != 0;
-    mode &= ~PDX_LAYER_OUT_NORM;
-    if (out_norm) {
-        if (!residual) return fail(PDX_ERR_INVALID, "PDX_LAYER_OUT_NORM needs a residual");
-        if ((st = check_norm_shape(H))) return st;
-    }
-    const int m = resolve_mode(mode, T * top_k, E, H, I);
-    if ((st = check_ffn_shape(H, I, m))) return st;
-    if ((st = check_weights(weights, H, I))) return st;
+    if ((st = check_out_norm(out_norm, residual, H))) return st;
+    LayerRows r;
+    if ((st = layer_rows(x, gate, T, H, E, top_k, normalize, weights, nullptr, I, logits_out, selected_out, weights_out,
+                         counts_out, mode & ~PDX_LAYER_OUT_NORM, workspace, workspace_bytes, r, stream)))
+        return st;
+    return finish_layer(r, T, top_k, H, residual, out_norm, out, stream);
+}
+
+size_t pdx_mxfp4_layer_workspace_bytes(int64_t T, int64_t H, int64_t E, int32_t top_k, int64_t I) {
+    T = std::max<int64_t>(T, 1);
+    E = std::max<int64_t>(E, 1);
+    top_k = std::max<int32_t>(top_k, 1);
+    const int64_t N = T * top_k;
+    return layer_common_bytes(T, H, E, top_k) + mx4_ffn_ws_bytes(N, E, H, I) + kAlign;
+}
+
+int pdx_mxfp4_moe_layer(const void* x, const void* gate, int64_t T, int64_t H, int64_t E, int32_t top_k,
+                        int32_t normalize, const pdx_mxfp4_weights* weights, int64_t I, const void* residual,
+                        void* out, void* logits_out, int64_t* selected_out, void* weights_out, int32_t* counts_out,
+                        int32_t flags, void* workspace, size_t workspace_bytes, pdx_stream_t stream) {
+    int st = check_route_shape(T, H, E, top_k);
+    if (st) return st;
+    if (!out || !weights) return fail(PDX_ERR_INVALID, "null layer argument");
+    if (flags & ~PDX_LAYER_OUT_NORM) return fail(PDX_ERR_INVALID, "unknown layer flags 0x%x", flags);
+    if ((st = check_out_norm(flags != 0, residual, H))) return st;
+    LayerRows r;
+    if ((st = layer_rows(x, gate, T, H, E, top_k, normalize, nullptr, weights, I, logits_out, selected_out, weights_out,
+                         counts_out, PDX_FFN_AUTO, workspace, workspace_bytes, r, stream)))
+        return st;
+    return finish_layer(r, T, top_k, H, residual, flags != 0, out, stream);
+}
+
+int pdx_moe_block(const void* x, const void* gate, int64_t T, int64_t H, int64_t E, int32_t top_k, int32_t normalize,
+                  const pdx_expert_weights* weights, const pdx_mxfp4_weights* mxfp4, int64_t I, const void* residual,
+                  const pdx_block_norm_args* args, void* stream_out, void* normed_out, void* logits_out,
+                  int64_t* selected_out, void* weights_out, int32_t* counts_out, int32_t mode, void* workspace,
+                  size_t workspace_bytes, pdx_stream_t stream) {
+    if ((weights == nullptr) == (mxfp4 == nullptr))
+        return fail(PDX_ERR_INVALID, "exactly one of the BF16 and the MXFP4 weights is required");
+    if (mxfp4 && mode != PDX_FFN_AUTO) return fail(PDX_ERR_INVALID, "MXFP4 experts have no FFN mode %d", mode);
+    int st = check_block_norm(args, residual, T, H, stream_out, normed_out);
+    if (st) return st;
+    LayerRows r;
+    if ((st = layer_rows(x, gate, T, H, E, top_k, normalize, weights, mxfp4, I, logits_out, selected_out, weights_out,
+                         counts_out, mode, workspace, workspace_bytes, r, stream)))
+        return st;
+    BlockNormArgs a = to_block_norm(args, residual, H, stream_out, normed_out);
+    a.y = r.y;
+    a.weights = r.weights;
+    a.inverse = r.inverse;
+    a.k = top_k;
+    a.y_rows = static_cast<int>(T * top_k);
+    st = launch_block_norm<true>(a, T, args->residual_fp32 != 0, stream);
+    return st ? st : ok();
+}
+
+int pdx_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, void* codes,
+                       void* scales, pdx_stream_t stream) {
+    int st = check_mx4_matrix(rows, cols, ld, dtype);
+    if (st) return st;
+    if (rows == 0) return ok();
+    if (!x || !codes || !scales) return fail(PDX_ERR_INVALID, "null quantisation argument");
+    if (reinterpret_cast<uintptr_t>(codes) & 3u) return fail(PDX_ERR_INVALID, "codes must be 4-byte aligned");
+    PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(x, ld, dtype), [&](auto type, auto aligned) {
+        using T = decltype(type);
+        return launch_pdl(k_mx4_quantize<T, decltype(aligned)::value>, mx4_grid(rows * cols / 8), dim3(kMxThreads), 0,
+                          stream, static_cast<const T*>(x), rows, cols, ld, static_cast<uint32_t*>(codes),
+                          static_cast<uint8_t*>(scales));
+    }));
+    return ok();
+}
+
+int pdx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, int64_t ld,
+                         int32_t dtype, void* out, pdx_stream_t stream) {
+    int st = check_mx4_matrix(rows, cols, ld, dtype);
+    if (st) return st;
+    if (rows == 0) return ok();
+    if (!out || !codes || !scales) return fail(PDX_ERR_INVALID, "null quantisation argument");
+    if (reinterpret_cast<uintptr_t>(codes) & 3u) return fail(PDX_ERR_INVALID, "codes must be 4-byte aligned");
+    PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(out, ld, dtype), [&](auto type, auto aligned) {
+        using T = decltype(type);
+        return launch_pdl(k_mx4_dequantize<T, decltype(aligned)::value>, mx4_grid(rows * cols / 8), dim3(kMxThreads),
+                          0, stream, static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(scales), rows,
+                          cols, ld, static_cast<T*>(out));
+    }));
+    return ok();
+}
+
+size_t pdx_mxfp4_ffn_workspace_bytes(int64_t rows, int64_t E, int64_t H, int64_t I) {
+    return mx4_ffn_ws_bytes(std::max<int64_t>(rows, 1), std::max<int64_t>(E, 1), H, I) + kAlign;
+}
+
+int pdx_mxfp4_ffn_grouped(const void* x, int64_t T, const int32_t* tokens, const int32_t* offsets,
+                          const int32_t* active, int64_t E, int64_t rows, const pdx_mxfp4_weights* weights,
+                          int64_t H, int64_t I, void* y_out, void* workspace, size_t workspace_bytes,
+                          pdx_stream_t stream) {
+    if (!x || !offsets || !active || !y_out) return fail(PDX_ERR_INVALID, "null FFN argument");
+    int st = check_mx4_ffn(T, rows, E, H, I, tokens != nullptr, weights);
+    if (st) return st;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1)))
         return fail(PDX_ERR_WORKSPACE, "workspace must be non-null and 256-byte aligned");
-    const int64_t N = T * top_k;
     Carver c{static_cast<char*>(workspace), workspace_bytes};
-    RouteBufs rb;
-    rb.logits = logits_out ? static_cast<uint16_t*>(logits_out) : static_cast<uint16_t*>(c.take(T * E * 2));
-    rb.partials = static_cast<double*>(c.take(route_partial_bytes(T, E)));
-    rb.selected = selected_out ? selected_out : static_cast<int64_t*>(c.take(N * 8));
-    rb.weights = weights_out ? static_cast<uint16_t*>(weights_out) : static_cast<uint16_t*>(c.take(N * 2));
-    PackBufs pb = carve_pack(c, T, top_k, E, counts_out);
-    uint16_t* y = static_cast<uint16_t*>(c.take(N * H * 2));
-    // decode batches: both projections in one launch straight from x
-    const bool one_launch = m == PDX_FFN_GEMV && decode_direct_ok(T, N, E, H, I, pb.o.tokens);
-    DecodeBufs db{};
-    if (one_launch) db = carve_decode(c, T, N, E, H, I, true);
-    if (c.overflow) return fail(PDX_ERR_WORKSPACE, "layer workspace too small (%zu > %zu bytes)", c.used, c.cap);
-    // the routing kernel also packs when the pack's shared memory fits the default 48 KiB
-    // (and then clears the single-launch FFN's tickets and counters)
-    const bool fused = T <= kTailMaxTokens && topk_pack_smem_bytes(E, N) <= 48 * 1024;
-    const bool zeroed = fused && one_launch;
-    if ((st = launch_route(x, gate, T, H, E, top_k, normalize, rb, fused ? &pb.o : nullptr, stream,
-                           zeroed ? db.counters : nullptr, zeroed ? db.plan.zero_words : 0)))
-        return st;
-    if (!fused && (st = launch_pack(rb.selected, rb.weights, T, top_k, E, pb.o, pb.chunk_hist, stream))) return st;
-    if (one_launch)
-        st = launch_decode_ffn(x, T, pb.o.tokens, pb.o.offsets, pb.o.active, N, weights, H, I, y, db, zeroed, stream);
-    else
-        st = launch_ffn(x, T, pb.o.tokens, pb.o.offsets, pb.o.active, E, N, weights, H, I, y, m, c, stream);
+    st = launch_mx4_ffn(x, T, tokens, offsets, active, E, rows, weights, H, I, y_out, c, stream);
+    return st ? st : ok();
+}
+
+int pdx_block_norm(const void* y, const void* residual, int64_t T, int64_t H, const pdx_block_norm_args* args,
+                   void* stream_out, void* normed_out, pdx_stream_t stream) {
+    int st = check_block_norm(args, residual, T, H, stream_out, normed_out);
     if (st) return st;
-    if (out_norm)
-        PDX_PDL_TRY(launch_combine_norm(H, dim3(static_cast<unsigned>(T)), dim3(kCombineThreads), 0, stream,
-                               static_cast<const uint16_t*>(y), static_cast<const uint16_t*>(rb.weights),
-                               static_cast<const int32_t*>(pb.o.inverse), static_cast<int>(T),
-                               static_cast<int>(top_k), static_cast<int>(H), static_cast<int>(N),
-                               static_cast<const uint16_t*>(residual), PDX_LAYER_NORM_EPS,
-                               static_cast<uint16_t*>(out)));
-    else
-        PDX_PDL_TRY(launch_pdl(k_combine, dim3(static_cast<unsigned>(T)), dim3(kCombineThreads), 0, stream,
-                               static_cast<const uint16_t*>(y), static_cast<const uint16_t*>(rb.weights),
-                               static_cast<const int32_t*>(pb.o.inverse), static_cast<int>(T),
-                               static_cast<int>(top_k), static_cast<int>(H), static_cast<int>(N),
-                               static_cast<const uint16_t*>(residual), static_cast<uint16_t*>(out)));
-    return ok();
+    BlockNormArgs a = to_block_norm(args, residual, H, stream_out, normed_out);
+    a.y = static_cast<const uint16_t*>(y);
+    st = launch_block_norm<false>(a, T, args->residual_fp32 != 0, stream);
+    return st ? st : ok();
+}
+
+int pdx_combine_block_norm(const void* rows, int64_t y_rows, const void* weights, const int32_t* inverse, int64_t T,
+                           int32_t top_k, int64_t H, const void* residual, const pdx_block_norm_args* args,
+                           void* stream_out, void* normed_out, pdx_stream_t stream) {
+    int st = check_block_norm(args, residual, T, H, stream_out, normed_out);
+    if (st) return st;
+    if (!rows || !weights || !inverse) return fail(PDX_ERR_INVALID, "null combine argument");
+    if (top_k < 1 || y_rows < 1) return fail(PDX_ERR_INVALID, "empty combine");
+    if (top_k > kMaxTopK) return fail(PDX_ERR_UNSUPPORTED, "top_k > %d", kMaxTopK);
+    if (y_rows >= (int64_t(1) << 31)) return fail(PDX_ERR_UNSUPPORTED, "y_rows too large");
+    BlockNormArgs a = to_block_norm(args, residual, H, stream_out, normed_out);
+    a.y = static_cast<const uint16_t*>(rows);
+    a.weights = static_cast<const uint16_t*>(weights);
+    a.inverse = inverse;
+    a.k = top_k;
+    a.y_rows = static_cast<int>(y_rows);
+    st = launch_block_norm<true>(a, T, args->residual_fp32 != 0, stream);
+    return st ? st : ok();
 }
 
 int pdx_ep_dispatch(const void* x, const int32_t* tokens, const int32_t* positions, const int32_t* offsets, int64_t T,

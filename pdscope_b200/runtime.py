@@ -305,6 +305,145 @@ def residual_layernorm(y, residual, eps=LN_EPS, out=None):
     return out
 
 
+_NORMS = dict(none=_lib.NORM_NONE, rms=_lib.NORM_RMS, layer=_lib.NORM_LAYER)
+RMS_EPS = 1e-6
+
+
+@dataclass
+class BlockNorm:
+    """The norms around one block, its gate and the residual scale:
+
+        z = post(y) * post_weight
+        s = residual_scale * residual + block_scale * act(gate) * z
+        n = pre(s) * pre_weight
+
+    in FP32, each output rounded once.  ``post`` and ``pre`` are "none",
+    "rms" (``v / sqrt(mean(v^2) + eps)``) or "layer" (population variance);
+    their weights are BF16 [H] or None.  ``gate`` is None or a BF16 tensor that
+    broadcasts against [T, H]: [T, 1], [H], [1, H] or [T, H] (any strides);
+    ``gate_act`` "sigmoid" applies the logistic function to it first."""
+    post: str = "none"
+    post_weight: object = None
+    gate: object = None
+    gate_act: str = "none"
+    residual_scale: float = 1.0
+    block_scale: float = 1.0
+    pre: str = "rms"
+    pre_weight: object = None
+    eps: float = RMS_EPS
+
+    def args(self, t_count, hidden, residual_dtype, device):
+        """Check against a [t_count, hidden] batch and form pdx_block_norm_args."""
+        if self.post not in _NORMS or self.pre not in _NORMS:
+            raise ValueError("post and pre must be 'none', 'rms' or 'layer'")
+        if self.gate_act not in ("none", "sigmoid"):
+            raise ValueError("gate_act must be 'none' or 'sigmoid'")
+        for name, norm in (("post", self.post), ("pre", self.pre)):
+            w = getattr(self, name + "_weight")
+            if w is not None:
+                _require_cuda_bf16(name + "_weight", w, 1)
+                if norm == "none":
+                    raise ValueError(f"{name}_weight without a {name} norm")
+                if w.shape[0] != hidden or w.device != device:
+                    raise ValueError(f"{name}_weight must be [H] on the device of residual")
+        a = _lib.BlockNormArgs(post=_NORMS[self.post], pre=_NORMS[self.pre],
+                               post_weight=self.post_weight.data_ptr() if self.post_weight is not None else None,
+                               pre_weight=self.pre_weight.data_ptr() if self.pre_weight is not None else None,
+                               gate_sigmoid=int(self.gate_act == "sigmoid"),
+                               residual_fp32=int(residual_dtype == torch.float32),
+                               residual_scale=self.residual_scale, block_scale=self.block_scale, eps=self.eps)
+        g = self.gate
+        if g is not None:
+            if not isinstance(g, torch.Tensor) or g.device != device or g.dtype != torch.bfloat16:
+                raise ValueError("gate must be a BF16 tensor on the device of residual")
+            if g.ndim > 2 or any(n not in (1, full) for n, full in zip(g.shape[::-1], (hidden, t_count))):
+                raise ValueError("gate does not broadcast against [T, H]")
+            g = g.expand(t_count, hidden)
+            a.gate, a.gate_row, a.gate_col = g.data_ptr(), g.stride(0), g.stride(1)
+        return a
+
+
+def _overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size()
+            and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
+def _block_norm_outputs(norm, residual, stream_out, out):
+    if not isinstance(residual, torch.Tensor) or residual.device.type != "cuda" or residual.ndim != 2 \
+            or residual.dtype not in (torch.bfloat16, torch.float32) or not residual.is_contiguous():
+        raise ValueError("residual must be a contiguous [T, H] BF16 or FP32 CUDA tensor")
+    if stream_out is None:
+        stream_out = torch.empty_like(residual)
+    elif (stream_out.shape != residual.shape or stream_out.dtype != residual.dtype
+          or stream_out.device != residual.device or not stream_out.is_contiguous()):
+        raise ValueError("stream_out must be contiguous and like residual")
+    if out is None:
+        out = torch.empty(residual.shape, dtype=torch.bfloat16, device=residual.device)
+    else:
+        _require_cuda_bf16("out", out, 2)
+        if out.shape != residual.shape or out.device != residual.device:
+            raise ValueError("out must have residual's shape and device")
+    if _overlap(stream_out, out):
+        raise ValueError("stream_out and out must not overlap")
+    args = norm.args(*residual.shape, residual.dtype, residual.device)
+    return args, stream_out, out
+
+
+def block_norm(y, residual, *, norm=None, stream_out=None, out=None, **options):
+    """The norm after a block, its gate and residual scale, and the norm before
+    the next block in one pass; returns ``(stream, normed)``.
+
+    ``y`` [T, H] BF16 is the block's output (None: ``s = residual_scale *
+    residual``, the norm before a first block), ``residual`` [T, H] BF16 or
+    FP32.  The options are ``BlockNorm``'s fields, or ``norm=BlockNorm(...)``.
+    ``stream`` has residual's type, ``normed`` is BF16; ``stream_out`` and
+    ``out`` may be ``y`` or ``residual``."""
+    norm = _block_norm_of(norm, options)
+    args, stream_out, out = _block_norm_outputs(norm, residual, stream_out, out)
+    if y is not None:
+        _require_cuda_bf16("y", y, 2)
+        if y.shape != residual.shape or y.device != residual.device:
+            raise ValueError("y and residual shapes differ")
+    t_count, hidden = residual.shape
+    with torch.cuda.device(residual.device):
+        check(lib.pdx_block_norm(_ptr(y), _ptr(residual), t_count, hidden, ctypes.byref(args), _ptr(stream_out),
+                                 _ptr(out), _stream()))
+    return stream_out, out
+
+
+def combine_block_norm(rows, weights, inverse, residual, *, norm=None, stream_out=None, out=None, **options):
+    """``block_norm`` of the weighted combine of the expert rows,
+    ``y[t] = sum_s weights[t, s] * rows[inverse[t*k + s]]`` in FP32 (``combine``
+    without its roundings in between); the arguments of both."""
+    norm = _block_norm_of(norm, options)
+    _require_cuda_bf16("rows", rows, 2)
+    _require_cuda_bf16("weights", weights, 2)
+    t_count, k = weights.shape
+    if not isinstance(inverse, torch.Tensor) or inverse.dtype != torch.int32 or inverse.device != rows.device \
+            or inverse.numel() != t_count * k or not inverse.is_contiguous():
+        raise ValueError("inverse must be a contiguous int32 tensor of T*k entries on the device of rows")
+    args, stream_out, out = _block_norm_outputs(norm, residual, stream_out, out)
+    if residual.shape != (t_count, rows.shape[1]) or residual.device != rows.device \
+            or weights.device != rows.device:
+        raise ValueError("residual must be [T, H] on the device of rows")
+    if _overlap(stream_out, rows) or _overlap(out, rows):
+        raise ValueError("the outputs must not alias rows")
+    with torch.cuda.device(rows.device):
+        check(lib.pdx_combine_block_norm(_ptr(rows), rows.shape[0], _ptr(weights), _ptr(inverse), t_count, k,
+                                         rows.shape[1], _ptr(residual), ctypes.byref(args), _ptr(stream_out),
+                                         _ptr(out), _stream()))
+    return stream_out, out
+
+
+def _block_norm_of(norm, options):
+    if norm is None:
+        return BlockNorm(**options)
+    if options or not isinstance(norm, BlockNorm):
+        raise ValueError("pass either norm=BlockNorm(...) or its fields")
+    return norm
+
+
 # ---------------------------------------------------------------------------
 # Weight placement
 # ---------------------------------------------------------------------------
@@ -371,6 +510,46 @@ class ExpertSlab:
 # ---------------------------------------------------------------------------
 
 
+def is_mxfp4(slab):
+    """Whether a slab's experts are MXFP4 (pdx_mxfp4_weights) rather than BF16."""
+    return isinstance(slab.struct, _lib.Mxfp4Weights)
+
+
+def layer_workspace_bytes(slab, t_count, experts, top_k, mode=_lib.FFN_AUTO):
+    """Workspace of one layer call on ``slab`` (BF16 or MXFP4 experts)."""
+    if is_mxfp4(slab):
+        return lib.pdx_mxfp4_layer_workspace_bytes(t_count, slab.hidden, experts, top_k, slab.inter)
+    return lib.pdx_layer_workspace_bytes(t_count, slab.hidden, experts, top_k, slab.inter, mode)
+
+
+def ffn_workspace_bytes(slab, rows, experts, mode=_lib.FFN_AUTO):
+    """Workspace of one grouped-FFN call on ``slab``."""
+    if is_mxfp4(slab):
+        return lib.pdx_mxfp4_ffn_workspace_bytes(rows, experts, slab.hidden, slab.inter)
+    return lib.pdx_ffn_workspace_bytes(rows, experts, slab.hidden, slab.inter, mode)
+
+
+def _scratch(slab, device, nbytes, tag):
+    """Workspace of one call: MXFP4 calls take theirs from the stream-ordered
+    allocator, so calls on two streams or in two graphs share no scratch."""
+    if is_mxfp4(slab):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _WS.get(device, nbytes, tag)
+
+
+def grouped_ffn(x, t_count, tokens, offsets, active, experts, rows, slab, y, workspace, mode=_lib.FFN_AUTO):
+    """One grouped-FFN call on ``slab`` into ``y``, on the current stream."""
+    head = (_ptr(x), t_count, _ptr(tokens), _ptr(offsets), _ptr(active), experts, rows, ctypes.byref(slab.struct),
+            slab.hidden, slab.inter, _ptr(y))
+    tail = (_ptr(workspace), workspace.numel(), _stream())
+    if is_mxfp4(slab):
+        if mode != _lib.FFN_AUTO:
+            raise ValueError("MXFP4 experts have no FFN modes")
+        check(lib.pdx_mxfp4_ffn_grouped(*head, *tail))
+    else:
+        check(lib.pdx_moe_ffn_grouped(*head, mode, *tail))
+
+
 @dataclass
 class LayerOutputs:
     out: torch.Tensor
@@ -384,7 +563,8 @@ class ResidentMoELayer:
     """One MoE layer whose experts are all resident in HBM.
 
     ``forward`` runs route -> pack -> grouped FFN -> combine in one C-ABI call
-    with no host synchronisation.
+    with no host synchronisation.  ``slab`` is an ``ExpertSlab`` or an
+    ``Mxfp4ExpertSlab`` (which has no FFN modes).
     """
 
     def __init__(self, gate, slab, top_k=8, normalize=True):
@@ -397,7 +577,7 @@ class ResidentMoELayer:
         self.top_k, self.normalize = top_k, normalize
 
     def workspace_bytes(self, t_count, mode=_lib.FFN_AUTO):
-        return lib.pdx_layer_workspace_bytes(t_count, self.hidden, self.experts, self.top_k, self.inter, mode)
+        return layer_workspace_bytes(self.slab, t_count, self.experts, self.top_k, mode)
 
     def forward(self, x, residual=None, *, mode=_lib.FFN_AUTO, outputs=None, workspace=None):
         _require_cuda_bf16("x", x, 2)
@@ -411,12 +591,13 @@ class ResidentMoELayer:
                 weights=torch.empty((t_count, self.top_k), dtype=torch.bfloat16, device=dev),
                 counts=torch.empty(self.experts, dtype=torch.int32, device=dev))
         if workspace is None:
-            workspace = _WS.get(dev, self.workspace_bytes(t_count, mode), "layer")
-        check(lib.pdx_moe_layer(_ptr(x), _ptr(self.gate), t_count, self.hidden, self.experts, self.top_k,
-                                int(self.normalize), ctypes.byref(self.slab.struct), self.inter, _ptr(residual),
-                                _ptr(outputs.out), _ptr(outputs.logits), _ptr(outputs.selected),
-                                _ptr(outputs.weights), _ptr(outputs.counts), mode, _ptr(workspace),
-                                workspace.numel(), _stream()))
+            workspace = _scratch(self.slab, dev, self.workspace_bytes(t_count, mode), "layer")
+        layer = lib.pdx_mxfp4_moe_layer if is_mxfp4(self.slab) else lib.pdx_moe_layer
+        check(layer(_ptr(x), _ptr(self.gate), t_count, self.hidden, self.experts, self.top_k,
+                    int(self.normalize), ctypes.byref(self.slab.struct), self.inter, _ptr(residual),
+                    _ptr(outputs.out), _ptr(outputs.logits), _ptr(outputs.selected),
+                    _ptr(outputs.weights), _ptr(outputs.counts), mode, _ptr(workspace),
+                    workspace.numel(), _stream()))
         return outputs
 
 
@@ -446,8 +627,8 @@ def _reference_planner():
 class PDScopeCudaRuntime:
     """Layer-level drop-in for ``PDScopeCudaRuntime.forward`` with HBM-resident experts.
 
-    ``layers`` maps layer index -> ExpertSlab (slot e = expert e, or an
-    explicit ``slot_of_expert``).  ``forward`` keeps the reference's signature,
+    ``layers`` maps layer index -> ExpertSlab or Mxfp4ExpertSlab (slot e =
+    expert e, or an explicit ``slot_of_expert``).  ``forward`` keeps the reference's signature,
     checks and return value ``(output, Routing, row)``
     (expertbench/pdscope_runtime.py:208-512); ``row`` carries the keys the
     reference harness reads (benchmarks/pdscope_compare.py:412-420).
@@ -586,11 +767,8 @@ class PDScopeCudaRuntime:
             active[0] = len(gpu_ids)
             active[1:1 + len(gpu_ids)] = torch.tensor(gpu_ids, dtype=torch.int32)
             active = active.to(dev, non_blocking=True)
-            ws = _WS.get(dev, lib.pdx_ffn_workspace_bytes(rows_total, experts, hidden, slab.inter, _lib.FFN_AUTO),
-                         "ffn")
-            check(lib.pdx_moe_ffn_grouped(_ptr(inputs), t_count, _ptr(p.tokens), _ptr(p.offsets), _ptr(active),
-                                          experts, rows_total, ctypes.byref(slab.struct), hidden, slab.inter,
-                                          _ptr(y), _lib.FFN_AUTO, _ptr(ws), ws.numel(), _stream()))
+            ws = _scratch(slab, dev, ffn_workspace_bytes(slab, rows_total, experts), "ffn")
+            grouped_ffn(inputs, t_count, p.tokens, p.offsets, active, experts, rows_total, slab, y, ws)
         if cpu_ids:
             tokens_cpu = p.tokens.cpu().long()
             x_cpu = inputs.cpu()

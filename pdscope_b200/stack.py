@@ -24,7 +24,8 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .runtime import LN_EPS, ExpertSlab, _ptr, _stream
+from .runtime import (LN_EPS, BlockNorm, ExpertSlab, _ptr, _stream, block_norm, combine_block_norm,
+                      ffn_workspace_bytes, grouped_ffn, is_mxfp4, layer_workspace_bytes)
 
 
 @dataclass
@@ -43,11 +44,26 @@ class StageBuffers:
 
 
 class ResidentMoEStack:
-    """``layers`` MoE layers with all experts resident; one slab per layer."""
+    """``layers`` MoE layers with all experts resident; one slab per layer, each
+    an ``ExpertSlab`` or an ``Mxfp4ExpertSlab``.
 
-    def __init__(self, gates, slabs, top_k=8, normalize=True):
+    With ``norms`` (layers + 1 ``BlockNorm``s) the step runs a pre-norm residual
+    stream instead of the two-layer protocol's layer norm: ``norms[0]`` forms
+    the first block's input from ``input`` (its block terms do not apply), and
+    ``norms[l + 1]`` follows block l, fused into its combine (pdx_moe_block):
+    the norm after the block, gate, residual scale and the norm before the next
+    block.  ``output`` is then the last normed activation and ``residual`` the
+    stream; ``input`` and the stream have ``residual_dtype`` (BF16 or FP32)."""
+
+    def __init__(self, gates, slabs, top_k=8, normalize=True, norms=None, residual_dtype=torch.bfloat16):
         if len(gates) != len(slabs) or not gates:
             raise ValueError("one router per expert slab is required")
+        if norms is not None and (len(norms) != len(gates) + 1 or not all(isinstance(n, BlockNorm) for n in norms)):
+            raise ValueError("norms must be layers + 1 BlockNorm objects")
+        if residual_dtype not in (torch.bfloat16, torch.float32) or (norms is None
+                                                                     and residual_dtype != torch.bfloat16):
+            raise ValueError("residual_dtype is BF16, or FP32 with norms")
+        self.norms, self.residual_dtype = list(norms) if norms is not None else None, residual_dtype
         self.gates, self.slabs = list(gates), list(slabs)
         self.experts, self.hidden = self.gates[0].shape
         self.inter = self.slabs[0].inter
@@ -81,12 +97,15 @@ class ResidentMoEStack:
                                inverse=torch.empty(n, **i32), active=torch.empty(E + 1, **i32))
                   for l in range(L)]
         rows = torch.empty((n, H), **bf)  # expert outputs of the current layer (staged path)
-        ws_layer = lib.pdx_layer_workspace_bytes(t_count, H, E, k, self.inter, mode)
+        ws_layer = max(layer_workspace_bytes(s, t_count, E, k, mode) for s in self.slabs)
         ws_stage = max(lib.pdx_route_workspace_bytes(t_count, E), lib.pdx_pack_workspace_bytes(t_count, k, E),
-                       lib.pdx_ffn_workspace_bytes(n, E, H, self.inter, mode))
+                       *(ffn_workspace_bytes(s, n, E, mode) for s in self.slabs))
         ws = torch.empty(max(ws_layer, ws_stage), dtype=torch.uint8, device=dev)
         b = dict(acts=acts, stages=stages, ws=ws, rows=rows, counts=counts,
                  counts_host=torch.zeros((L, E), dtype=torch.int32).pin_memory(), counts_ready=torch.cuda.Event())
+        if self.norms is not None:
+            # the step input (never overwritten) and the residual stream, updated in place
+            b["stream"] = [torch.zeros((t_count, H), dtype=self.residual_dtype, device=dev) for _ in range(2)]
         self._bufs[key] = b
         return b
 
@@ -98,19 +117,36 @@ class ResidentMoEStack:
     def _act_out(acts, l):
         return acts[1 + l % 2]
 
+    def _first_norm(self, b):
+        """The norm before the first block: stream and acts[0] from the step input."""
+        block_norm(None, b["stream"][0], norm=self.norms[0], stream_out=b["stream"][1], out=b["acts"][0])
+
     # -- fused path: one C-ABI call per layer -------------------------------------
     def _step_fused(self, t_count, mode, counts_to_host=False):
         b = self.buffers(t_count, mode)
         acts, stages, ws = b["acts"], b["stages"], b["ws"]
         s = _stream()
+        if self.norms is not None:
+            self._first_norm(b)
         for l in range(self.num_layers):
-            st = stages[l]
+            st, slab = stages[l], self.slabs[l]
             x_in, x_out = self._act_in(acts, l), self._act_out(acts, l)
-            check(lib.pdx_moe_layer(_ptr(x_in), _ptr(self.gates[l]), t_count, self.hidden, self.experts,
-                                    self.top_k, int(self.normalize), ctypes.byref(self.slabs[l].struct), self.inter,
-                                    _ptr(x_in), _ptr(x_out), _ptr(st.logits), _ptr(st.selected),
-                                    _ptr(st.weights), _ptr(st.counts), mode | _lib.LAYER_OUT_NORM, _ptr(ws),
-                                    ws.numel(), s))
+            weights = ctypes.byref(slab.struct)
+            if self.norms is not None:
+                stream = b["stream"][1]
+                args = self.norms[l + 1].args(t_count, self.hidden, self.residual_dtype, self.device)
+                check(lib.pdx_moe_block(_ptr(x_in), _ptr(self.gates[l]), t_count, self.hidden, self.experts, self.top_k,
+                                        int(self.normalize), *((None, weights) if is_mxfp4(slab) else (weights, None)),
+                                        self.inter, _ptr(stream), ctypes.byref(args), _ptr(stream), _ptr(x_out),
+                                        _ptr(st.logits), _ptr(st.selected), _ptr(st.weights), _ptr(st.counts), mode,
+                                        _ptr(ws), ws.numel(), s))
+                continue
+            layer = lib.pdx_mxfp4_moe_layer if is_mxfp4(slab) else lib.pdx_moe_layer
+            check(layer(_ptr(x_in), _ptr(self.gates[l]), t_count, self.hidden, self.experts,
+                        self.top_k, int(self.normalize), weights, self.inter,
+                        _ptr(x_in), _ptr(x_out), _ptr(st.logits), _ptr(st.selected),
+                        _ptr(st.weights), _ptr(st.counts), mode | _lib.LAYER_OUT_NORM, _ptr(ws),
+                        ws.numel(), s))
         if counts_to_host:
             # one device-to-host copy of every layer's counts into pinned memory,
             # inside the step (and its graph): no per-layer host synchronisation
@@ -132,20 +168,25 @@ class ResidentMoEStack:
         b = self.buffers(t_count, mode)
         st, ws = b["stages"][l], b["ws"]
         n = t_count * self.top_k
-        check(lib.pdx_moe_ffn_grouped(_ptr(self._act_in(b["acts"], l)), t_count, _ptr(st.tokens),
-                                      _ptr(st.offsets), _ptr(st.active), self.experts, n,
-                                      ctypes.byref(self.slabs[l].struct), self.hidden, self.inter, _ptr(b["rows"]),
-                                      mode, _ptr(ws), ws.numel(), _stream()))
+        grouped_ffn(self._act_in(b["acts"], l), t_count, st.tokens, st.offsets, st.active, self.experts, n,
+                    self.slabs[l], b["rows"], ws, mode)
 
     def combine(self, l, t_count, mode=_lib.FFN_AUTO):
         """Weighted combine fused with the next-layer norm."""
         b = self.buffers(t_count, mode)
         st = b["stages"][l]
         x_in, x_out = self._act_in(b["acts"], l), self._act_out(b["acts"], l)
+        if self.norms is not None:
+            stream = b["stream"][1]
+            combine_block_norm(b["rows"], st.weights, st.inverse, stream, norm=self.norms[l + 1], stream_out=stream,
+                               out=x_out)
+            return
         check(lib.pdx_combine_layernorm(_ptr(b["rows"]), _ptr(st.weights), _ptr(st.inverse), t_count, self.top_k,
                                         self.hidden, _ptr(x_in), ctypes.c_float(LN_EPS), _ptr(x_out), _stream()))
 
     def _step_staged(self, t_count, mode):
+        if self.norms is not None:
+            self._first_norm(self.buffers(t_count, mode))
         for l in range(self.num_layers):
             self.route_and_pack(l, t_count, mode)
             self.ffn(l, t_count, mode)
@@ -153,7 +194,14 @@ class ResidentMoEStack:
 
     # -- public step --------------------------------------------------------------------
     def input(self, t_count, mode=_lib.FFN_AUTO):
-        return self.buffers(t_count, mode)["acts"][0]
+        b = self.buffers(t_count, mode)
+        return b["stream"][0] if self.norms is not None else b["acts"][0]
+
+    def residual(self, t_count, mode=_lib.FFN_AUTO):
+        """The residual stream after the last block (stacks with ``norms``)."""
+        if self.norms is None:
+            raise ValueError("only a stack with norms keeps a residual stream")
+        return self.buffers(t_count, mode)["stream"][1]
 
     def output(self, t_count, mode=_lib.FFN_AUTO):
         return self._act_out(self.buffers(t_count, mode)["acts"], self.num_layers - 1)

@@ -1,0 +1,158 @@
+"""Refusals of the MXFP4 and block-norm entry points, on the CPU: the Python
+checks raise ValueError, the C ABI returns its status, before any device work."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import pdscope_b200 as pdx
+from pdscope_b200 import _lib
+from pdscope_b200.stack import ResidentMoEStack
+from tests import mxfp4_ref as ref
+
+PTR, NULL = ctypes.c_void_p(256), ctypes.c_void_p(0)
+
+
+def test_definition_round_trip():
+    """The 64-bit definition: halves round to even, the largest value fills [4, 8)."""
+    x = np.array([4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9] + [0.0] * 23)
+    codes, scales = ref.quantize(x)
+    assert scales.tolist() == [127]
+    assert ref.dequantize(codes, scales)[:9].tolist() == [4.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0]
+
+
+@pytest.mark.parametrize("x", (torch.zeros(4, 64), torch.zeros(4, 64, dtype=torch.int32), None))
+def test_quantize_refuses(x):
+    with pytest.raises(ValueError):
+        pdx.quantize_mxfp4(x)
+
+
+def test_dequantize_refuses():
+    with pytest.raises(ValueError):
+        pdx.dequantize_mxfp4(torch.zeros(4, 32, dtype=torch.uint8))
+    with pytest.raises(ValueError):
+        pdx.dequantize_mxfp4(pdx.Mxfp4(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)))
+
+
+@pytest.mark.parametrize("cols,rows,ld,dtype", ((31, 4, 31, 0), (0, 4, 0, 0), (64, -1, 64, 0), (64, 4, 63, 0),
+                                                (64, 4, 64, 3), (64, 4, 64, -1)))
+def test_matrix_status(cols, rows, ld, dtype):
+    assert _lib.lib.pdx_mxfp4_quantize(PTR, dtype, rows, cols, ld, PTR, PTR, NULL) == _lib.PDX_ERR_INVALID
+    assert _lib.lib.pdx_mxfp4_dequantize(PTR, PTR, rows, cols, ld, dtype, PTR, NULL) == _lib.PDX_ERR_INVALID
+
+
+def test_null_and_unaligned_status():
+    assert _lib.lib.pdx_mxfp4_quantize(NULL, 0, 1, 32, 32, PTR, PTR, NULL) == _lib.PDX_ERR_INVALID
+    assert _lib.lib.pdx_mxfp4_quantize(PTR, 0, 1, 32, 32, ctypes.c_void_p(258), PTR, NULL) == _lib.PDX_ERR_INVALID
+    assert _lib.lib.pdx_mxfp4_quantize(NULL, 0, 0, 32, 32, NULL, NULL, NULL) == _lib.PDX_OK
+
+
+def _weights(**kw):
+    d = dict(codes=256, scales=256, code_stride=3 * 128 * 128 // 2, scale_stride=3 * 128 * 4, num_slots=2)
+    d.update(kw)
+    return _lib.Mxfp4Weights(**d)
+
+
+def _ffn(w, hidden=128, inter=128, tokens=2, rows=4, experts=2, gathered=True, ws=PTR, nbytes=1 << 40):
+    return _lib.lib.pdx_mxfp4_ffn_grouped(PTR, tokens, PTR if gathered else NULL, PTR, PTR, experts, rows,
+                                          ctypes.byref(w), hidden, inter, PTR, ws, nbytes, NULL)
+
+
+def test_ffn_status():
+    assert _ffn(_weights(), tokens=0) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(), rows=0) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(), hidden=48) == _lib.PDX_ERR_UNSUPPORTED
+    assert _ffn(_weights(), inter=16) == _lib.PDX_ERR_UNSUPPORTED
+    assert _ffn(_weights(), gathered=False) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(codes=None)) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(codes=264)) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(num_slots=0)) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(code_stride=128)) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(), ws=NULL) == _lib.PDX_ERR_WORKSPACE
+    assert _ffn(_weights(), ws=ctypes.c_void_p(128)) == _lib.PDX_ERR_WORKSPACE
+    assert _ffn(_weights(), nbytes=64) == _lib.PDX_ERR_WORKSPACE
+
+
+def test_workspace_queries():
+    lib = _lib.lib
+    for shape in ((1, 128, 32, 32), (512, 128, 2048, 768), (99600, 128, 2048, 768)):
+        assert lib.pdx_mxfp4_ffn_workspace_bytes(*shape) > 0
+    assert (lib.pdx_mxfp4_layer_workspace_bytes(64, 2048, 128, 8, 768)
+            >= lib.pdx_mxfp4_ffn_workspace_bytes(512, 128, 2048, 768) + 512 * 2048 * 2)
+
+
+def _norm(args, tokens=2, hidden=64, y=PTR, residual=PTR, stream=PTR, normed=PTR):
+    return _lib.lib.pdx_block_norm(y, residual, tokens, hidden, ctypes.byref(args), stream, normed, NULL)
+
+
+def test_block_norm_status():
+    def a(**kw):
+        return _lib.BlockNormArgs(**dict(dict(eps=1e-6, pre=1, residual_scale=1, block_scale=1), **kw))
+    assert _norm(a(), tokens=0) == _lib.PDX_ERR_INVALID
+    assert _norm(a(), residual=NULL) == _lib.PDX_ERR_INVALID
+    assert _norm(a(), stream=NULL, normed=NULL) == _lib.PDX_ERR_INVALID
+    assert _norm(a(), hidden=0) == _lib.PDX_ERR_UNSUPPORTED
+    assert _norm(a(), hidden=8193) == _lib.PDX_ERR_UNSUPPORTED
+    assert _norm(a(post=3)) == _lib.PDX_ERR_INVALID
+    assert _norm(a(pre=-1)) == _lib.PDX_ERR_INVALID
+    assert _norm(a(eps=0)) == _lib.PDX_ERR_INVALID
+    assert _norm(a(eps=float("nan"))) == _lib.PDX_ERR_INVALID
+    assert _norm(a(gate=256, gate_row=-1)) == _lib.PDX_ERR_INVALID
+    combine = _lib.lib.pdx_combine_block_norm
+    args = a()
+    assert combine(PTR, 4, PTR, NULL, 2, 2, 64, PTR, ctypes.byref(args), PTR, PTR, NULL) == _lib.PDX_ERR_INVALID
+    assert combine(PTR, 4, PTR, PTR, 2, 0, 64, PTR, ctypes.byref(args), PTR, PTR, NULL) == _lib.PDX_ERR_INVALID
+    assert combine(PTR, 4, PTR, PTR, 2, 33, 64, PTR, ctypes.byref(args), PTR, PTR, NULL) == _lib.PDX_ERR_UNSUPPORTED
+
+
+def test_block_status():
+    args = _lib.BlockNormArgs(eps=1e-6, pre=1)
+    w, w4 = _lib.ExpertWeights(), _weights()
+
+    def block(bf16, mx, mode=0):
+        return _lib.lib.pdx_moe_block(PTR, PTR, 2, 128, 4, 2, 1, ctypes.byref(w) if bf16 else None,
+                                      ctypes.byref(w4) if mx else None, 128, PTR, ctypes.byref(args), PTR, PTR, NULL,
+                                      NULL, NULL, NULL, mode, PTR, 1 << 40, NULL)
+    assert block(False, False) == _lib.PDX_ERR_INVALID
+    assert block(True, True) == _lib.PDX_ERR_INVALID
+    assert block(False, True, mode=2) == _lib.PDX_ERR_INVALID
+
+
+def test_block_norm_refuses():
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="residual"):
+        pdx.block_norm(x, x)
+    with pytest.raises(ValueError, match="either norm"):
+        pdx.block_norm(x, x, norm=pdx.BlockNorm(), post="rms")
+    for bad, match in ((dict(post="batch"), "post and pre"), (dict(gate_act="tanh"), "gate_act"),
+                       (dict(post_weight=x[0]), "post_weight"), (dict(gate=torch.zeros(3, 64)), "gate")):
+        with pytest.raises(ValueError, match=match):
+            pdx.BlockNorm(**bad).args(2, 64, torch.bfloat16, x.device)
+    for shape in ((3, 64), (2, 32), (1, 2, 64)):
+        with pytest.raises(ValueError, match="broadcast"):
+            pdx.BlockNorm(gate=torch.zeros(shape, dtype=torch.bfloat16)).args(2, 64, torch.bfloat16, x.device)
+    a = pdx.BlockNorm(gate=torch.zeros(2, 1, dtype=torch.bfloat16)).args(2, 64, torch.bfloat16, x.device)
+    assert (a.gate_row, a.gate_col) == (1, 0)
+
+
+def test_slab_refuses():
+    for hidden, inter in ((48, 64), (64, 0), (0, 64)):
+        with pytest.raises(ValueError):
+            pdx.Mxfp4ExpertSlab(1, hidden, inter, "cpu")
+    with pytest.raises(ValueError):
+        pdx.Mxfp4ExpertSlab(2, 64, 64, "cpu", slot_of_expert=torch.zeros(2))
+    slab = pdx.Mxfp4ExpertSlab(2, 64, 64, "cpu")
+    with pytest.raises(ValueError):
+        pdx.moe_ffn_mxfp4(torch.zeros(2, 64, dtype=torch.bfloat16), None, slab)
+
+
+def test_stack_refuses_norms():
+    gate = torch.zeros(4, 64, dtype=torch.bfloat16)
+    slab = pdx.Mxfp4ExpertSlab(4, 64, 64, "cpu")
+    with pytest.raises(ValueError, match="norms"):
+        ResidentMoEStack([gate], [slab], norms=[pdx.BlockNorm()])
+    with pytest.raises(ValueError, match="residual_dtype"):
+        ResidentMoEStack([gate], [slab], residual_dtype=torch.float32)
+    with pytest.raises(ValueError, match="residual stream"):
+        ResidentMoEStack([gate], [slab]).residual(1)
