@@ -1,109 +1,549 @@
-// Grouped SwiGLU experts on MXFP4 weights: y[p] = Wd (silu(Wg x) * (Wu x)) for
-// every packed row p, weights dequantised exactly, sums and h in FP32, one
-// rounding to BF16 at the end.  One warp per output value pair.
-#include "ffn_gemv.cu"
+// Grouped SwiGLU experts on MXFP4 weights, on the block-scaled tensor cores:
+//   y[p] = Wd (silu(Wg x) * (Wu x)),  x = x[tokens[p]], for every packed row p.
+//
+// The weights go to tcgen05.mma.kind::mxf8f6f4 as they are stored: E2M1 codes
+// as the M operand (TMA unpacks them to one code per byte on the way to shared
+// memory) and their E8M0 scales, one per 32 values of K, copied to TMEM.  No
+// instruction is spent on dequantising, and HBM is read at 4.25 bits a weight.
+//
+// The activations keep BF16's precision in that 8-bit product as TWO E4M3
+// pieces.  With v scaled by a power of two so that the largest value of its
+// scaling group lies in [128, 256):
+//   hi = e4m3(v),  lo = e4m3(v - hi)
+// e4m3 keeps 4 significant bits, so |v - hi| <= 2^-4 |v| and the rest after lo
+// is at most 2^-8 |v|: BF16's half step.  A BF16 v is represented exactly down
+// to 2^-10 of its group's largest value; below that the error is at most 2^-10
+// (half of e4m3's smallest step), 2^-17 of the largest value.  x is scaled per
+// row (a factor on the row of the result), h per 32 values of I (an E8M0 scale
+// of the second product).  W hi and W lo cost what one BF16 product would.
+//
+// Two launches of k_mx4_gemm: gate and up with the SwiGLU (two accumulators),
+// then down.  tokens are the N operand, NT packed rows of one expert a tile; up
+// to NT = 32 the two pieces are stacked along N (one pass over the weights in
+// shared memory), above that they accumulate into the same columns.
+// Work is cut evenly: the (tile, K step) pairs of the launch form one sequence
+// and CTA c takes an equal share of it, so a decode step of any batch keeps
+// every SM streaming; a tile that spans CTAs is summed in CTA order by the warp
+// that takes its last ticket (FP32, deterministic, nothing waits).
+// Roles (224 threads): warp 0 streams weights and scales, warp 6 the token
+// pieces, warp 1 issues the MMAs, warps 2..5 are the epilogue (32 weight rows,
+// = one scale block of h, each).  Neither launch waits for another CTA; the
+// weight stream of a launch starts before the launch before it has finished.
+#include <cuda.h>
+
+#include "ffn_decode.cu"
 #include "mxfp4.cu"
+#include "tcgen05.cuh"
 
 namespace pdx {
 
-// Expert weights: slot s holds, from codes + s * code_stride, gate [Ip, Hp/2],
-// up [Ip, Hp/2] and down [Hp, Ip/2] code bytes (Hp, Ip: H, I rounded up to
-// 128, padding zero), and from scales + s * scale_stride their scales as tiles
-// of 128 rows x 128 columns, 512 bytes each, row tiles outermost: byte
-// (r % 32) * 16 + (r / 32) * 4 + c / 32 of a tile is the scale of row r,
-// columns c .. c + 31.
-struct Mx4Slab {
-    const uint8_t* codes;
-    const uint8_t* scales;
-    int64_t code_stride, scale_stride, num_slots;
-    const int32_t* slot_of_expert;
+constexpr int kMx4Threads = 224;
+constexpr int kMx4BK = 128;                         // K step: 4 MMAs of 32
+constexpr uint32_t kMx4ABytes = 128 * kMx4BK;       // one weight tile, a byte per code
+constexpr uint32_t kMx4SfBytes = 512;               // scales of 128 rows x 128 columns
+constexpr int kMx4MaxActive = 1024;
+constexpr uint32_t kMx4TmemCols = 512;
+constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of (gate | up | token) scales, 4 columns each
+constexpr uint32_t kMx4OneCol = 496;                // token scales of 1 (x is scaled by its row factor)
+constexpr int kMx4SmemLimit = 227 * 1024;
+
+// byte -> 2^(byte - 127), the inverse as a factor for byte <= 253
+__device__ __forceinline__ uint32_t mx4_group_byte(uint32_t max_bits) {  // largest value -> [128, 256)
+    const uint32_t e = max_bits >> 23;
+    return e > 7u ? e - 7u : 0u;
+}
+__device__ __forceinline__ float mx4_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+// Two values -> their E4M3 pieces (a in the low byte); non-finite -> NaN.
+__device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint16_t& lo) {
+    // infinities become NaN (e4m3 has none, and saturating would hide them)
+    a = a - (a - a);
+    b = b - (b - b);
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b), "f"(a));
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(hi));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b - f.y), "f"(a - f.x));
+}
+
+// Token rows in packed order as E4M3 pieces, one warp per row: out [2][rows][Hp]
+// (hi rows, then lo rows, zero past H) and the row's factor 2^(byte - 127).
+// CTA 0 clears the tickets of the two products that follow.
+constexpr int kMx4SplitWarps = 4;
+__global__ void __launch_bounds__(kMx4SplitWarps * 32)
+    k_mx4_split(const uint16_t* __restrict__ x, const int32_t* __restrict__ tokens, int T, int rows, int H, int Hp,
+                uint8_t* __restrict__ out, float* __restrict__ row_scale, unsigned int* __restrict__ zero_ptr,
+                int zero_words) {
+    griddep_wait();
+    griddep_launch();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < zero_words; i += blockDim.x) zero_ptr[i] = 0u;
+    const int lane = static_cast<int>(lane_id());
+    for (int p = static_cast<int>(blockIdx.x) * kMx4SplitWarps + static_cast<int>(threadIdx.x >> 5); p < rows;
+         p += static_cast<int>(gridDim.x) * kMx4SplitWarps) {
+        int t = tokens ? tokens[p] : p;
+        if (t < 0 || t >= T) {
+            raise_error(PDX_DEVERR_BAD_EXPERT);
+            t = 0;
+        }
+        const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t) * H);
+        uint32_t top = 0;
+        for (int c = lane; c < H / 8; c += 32) {
+            const uint4 v = __ldg(src + c);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
+        }
+        const uint32_t byte = mx4_group_byte(__reduce_max_sync(0xffffffffu, top));
+        const float inv = mx4_inverse(byte);
+        uint8_t* hi_row = out + static_cast<int64_t>(p) * Hp;
+        uint8_t* lo_row = out + (static_cast<int64_t>(rows) + p) * Hp;
+        for (int c = lane; c < Hp / 16; c += 32) {
+            uint32_t hw[4] = {0, 0, 0, 0}, lw[4] = {0, 0, 0, 0};
+            if (c * 16 < H) {
+                float v[16];
+                load8<bf16, true>(reinterpret_cast<const bf16*>(src) + c * 16, v);
+                load8<bf16, true>(reinterpret_cast<const bf16*>(src) + c * 16 + 8, v + 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint16_t h0, l0, h1, l1;
+                    e4m3_split2(v[4 * i] * inv, v[4 * i + 1] * inv, h0, l0);
+                    e4m3_split2(v[4 * i + 2] * inv, v[4 * i + 3] * inv, h1, l1);
+                    hw[i] = h0 | (static_cast<uint32_t>(h1) << 16);
+                    lw[i] = l0 | (static_cast<uint32_t>(l1) << 16);
+                }
+            }
+            reinterpret_cast<uint4*>(hi_row)[c] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+            reinterpret_cast<uint4*>(lo_row)[c] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+        }
+        if (lane == 0) row_scale[p] = mx_scale(byte);
+    }
+}
+
+struct Mx4Args {
+    const int32_t* offsets;         // [E+1]
+    const int32_t* active;          // [E+1] active count, then the active expert ids
+    const int32_t* slot_of_expert;  // NULL = identity
+    int64_t num_slots;
+    const uint8_t* scales0;         // weight scales of slot 0: gate, or down
+    const uint8_t* scales1;         // up
+    int64_t scale_stride;           // bytes between slots
+    int64_t rows_per_slot;          // TMA-map rows between slots
+    int up_row;                     // TMA-map row of up relative to gate
+    int K, M;                       // multiples of 128: reduction length, weight rows
+    int rows;
+    const float* row_scale;         // [rows] factor of a packed row of x (SWIGLU)
+    uint8_t* sf;                    // h scales: [token tile][Ip / 128] tiles of 512 bytes (out of SWIGLU, else in)
+    uint8_t* h;                     // [2][rows][M] pieces (SWIGLU)
+    uint16_t* y;                    // [rows, ldy] (down)
+    int ldy;                        // H
+    float* partials;                // [gridDim.x][2][columns][128]
+    unsigned int* tickets;          // [tiles * 4], zero on entry
 };
 
-__device__ __forceinline__ int64_t mx4_tile_scale(int r, int c, int cols) {
-    return (static_cast<int64_t>(r >> 7) * (cols >> 7) + (c >> 7)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 +
-           ((c >> 5) & 3);
+__device__ __forceinline__ uint64_t mx4_sf_desc(uint32_t smem_addr) {  // 32 x 16 bytes, 8-row groups 128 bytes apart
+    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) |
+           (static_cast<uint64_t>(1) << 46);
 }
 
-// Expert of packed row p and its weight slot (flagged slots read slot 0).
-__device__ __forceinline__ int64_t mx4_row_slot(const Mx4Slab& w, const int32_t* offsets, const int32_t* active,
-                                                int p) {
-    int lo = 0, hi = active[0] - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (offsets[active[1 + mid]] <= p) lo = mid; else hi = mid - 1;
-    }
-    const int e = active[1 + lo];
-    if (p < offsets[e] || p >= offsets[e + 1]) return -1;   // a row of no active expert
-    const int64_t slot = w.slot_of_expert ? w.slot_of_expert[e] : e;
-    if (slot < 0 || slot >= w.num_slots) {
-        raise_error(PDX_DEVERR_BAD_SLOT);
-        return 0;
-    }
-    return slot;
+// A = E2M1 (5), B = E4M3 (0), E8M0 scales, M = 128; the scale byte of the K step is or'ed in.
+__host__ __device__ constexpr uint32_t mx4_idesc(int n) {
+    return (5u << 7) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (1u << 27);
 }
 
-__global__ void __launch_bounds__(256) k_mx4_gateup(const uint16_t* __restrict__ x, const int32_t* __restrict__ tokens,
-                                                    int T, const int32_t* __restrict__ offsets,
-                                                    const int32_t* __restrict__ active, Mx4Slab w, int rows, int H,
-                                                    int I, int Hp, int Ip, float* __restrict__ h) {
-    griddep_wait();
-    griddep_launch();
-    const int p = static_cast<int>(blockIdx.x);
-    const int64_t slot = mx4_row_slot(w, offsets, active, p);
-    if (slot < 0) return;
-    int t = tokens ? tokens[p] : p;
-    if (t < 0 || t >= T) {
-        raise_error(PDX_DEVERR_BAD_EXPERT);
-        t = 0;
+__device__ __forceinline__ void umma_mx4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
+}
+
+__device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            smem_u32(smem_dst)),
+        "l"(src), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y,
+                                            int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+template <int NT, bool SWIGLU>
+struct Mx4Shape {
+    static constexpr bool kStack = NT <= 32;                        // pieces side by side along N
+    static constexpr int kN = kStack ? 2 * NT : NT;                 // N of one MMA
+    static constexpr int kAcc = (SWIGLU ? 2 : 1) * kN;              // accumulator columns
+    static constexpr int kBufs = 2 * kAcc <= static_cast<int>(kMx4SfCol) ? 2 : 1;
+    static constexpr int kCols = (SWIGLU ? 2 : 1) * NT;             // FP32 columns of a partial tile
+    static constexpr uint32_t kA = (SWIGLU ? 2 : 1) * kMx4ABytes;
+    static constexpr uint32_t kATx = kA / 2;                        // the copy counts the packed bytes it reads
+    static constexpr uint32_t kB = 2 * NT * kMx4BK;
+    static constexpr uint32_t kStage = kA + kB;                     // multiple of 1024
+    static constexpr uint32_t kSf = 2 * kMx4SfBytes;                // gate | up, or down | tokens
+    static constexpr uint32_t kTables = 4 * (kMx4MaxActive + 1) * 4;
+    static constexpr int kStages = static_cast<int>((kMx4SmemLimit - 1024 - 512 - 512 - kTables) / (kStage + kSf));
+    static constexpr size_t kSmem = 1024 + kStages * (kStage + kSf) + 512 + 512 + kTables;
+    static_assert(NT % 16 == 0 && NT <= 128 && kStages >= 2 && kAcc <= static_cast<int>(kMx4SfCol), "token tile");
+};
+
+template <int NT, bool SWIGLU>
+__global__ void __launch_bounds__(kMx4Threads, 1)
+    k_mx4_gemm(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, Mx4Args args) {
+    using S = Mx4Shape<NT, SWIGLU>;
+    extern __shared__ __align__(1024) unsigned char smem_mx4[];
+    unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
+    unsigned char* s_sf = smem + S::kStages * S::kStage;             // kStages x kSf
+    unsigned char* s_one = s_sf + S::kStages * S::kSf;               // 512 bytes of scale 1
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_one + 512);
+    uint64_t* empty_bar = full_bar + S::kStages;
+    uint64_t* tmem_full = empty_bar + S::kStages;
+    uint64_t* tmem_empty = tmem_full + 2;
+    uint64_t* drain_bar = tmem_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* s_misc = reinterpret_cast<int*>(tmem_slot + 2);
+    int* prefix = reinterpret_cast<int*>(s_one + 1024);              // tiles before an active expert
+    int* t_seg0 = prefix + (kMx4MaxActive + 1);
+    int* t_rows = t_seg0 + (kMx4MaxActive + 1);
+    int* t_slot = t_rows + (kMx4MaxActive + 1);
+    static_assert(2 * S::kStages + 5 <= 56, "barriers and words fit 512 bytes");
+
+    const int warp = static_cast<int>(threadIdx.x >> 5);
+    const uint32_t lane = lane_id();
+    const int m_blocks = args.M / 128, nkb = args.K / kMx4BK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tmem_full[b], 1);
+            mbar_init(&tmem_empty[b], 128);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tm_w);
+        tma_prefetch_desc(&tm_x);
     }
-    const uint8_t* gc = w.codes + slot * w.code_stride;
-    const uint8_t* uc = gc + static_cast<int64_t>(Ip) * Hp / 2;
-    const uint8_t* gs = w.scales + slot * w.scale_stride;
-    const uint8_t* us = gs + static_cast<int64_t>(Ip) * Hp / 32;
-    for (int i = static_cast<int>(blockIdx.y) * 8 + static_cast<int>(threadIdx.x >> 5); i < I; i += 8 * gridDim.y) {
-        float g = 0.f, u = 0.f;
-        for (int k = static_cast<int>(lane_id()) * 8; k < H; k += 256) {
-            float xv[8], gv[8], uv[8];
-            load8<bf16, true>(reinterpret_cast<const bf16*>(x) + static_cast<int64_t>(t) * H + k, xv);
-            const int64_t at = (static_cast<int64_t>(i) * Hp + k) / 2, sc = mx4_tile_scale(i, k, Hp);
-            e2m1x8_to_float(*reinterpret_cast<const uint32_t*>(gc + at), gv);
-            e2m1x8_to_float(*reinterpret_cast<const uint32_t*>(uc + at), uv);
-            float a = 0.f, b = 0.f;
-            for (int j = 0; j < 8; ++j) {
-                a += xv[j] * gv[j];
-                b += xv[j] * uv[j];
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(kMx4TmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp >= 3)
+        for (int i = static_cast<int>(threadIdx.x) - 96; i < 128; i += kMx4Threads - 96)
+            reinterpret_cast<uint32_t*>(s_one)[i] = 0x7F7F7F7Fu;
+    fence_proxy_async_smem();
+    // The routing tables are older than the launch before this one, which has
+    // passed its own wait by the time this one starts; only that launch's
+    // output (the token pieces) has to be waited for, by the warps that read it.
+    const int n_active = max(0, min(__ldcg(args.active), kMx4MaxActive));
+    if (warp == 2) {
+        for (int i = static_cast<int>(lane); i < n_active; i += 32) {
+            const int e = __ldcg(args.active + 1 + i);
+            const int seg0 = __ldcg(args.offsets + e);
+            int64_t slot = args.slot_of_expert ? __ldcg(args.slot_of_expert + e) : e;
+            if (slot < 0 || slot >= args.num_slots) {
+                raise_error(PDX_DEVERR_BAD_SLOT);
+                slot = 0;
             }
-            g += a * mx_scale(gs[sc]);
-            u += b * mx_scale(us[sc]);
+            t_seg0[i] = seg0;
+            t_rows[i] = __ldcg(args.offsets + e + 1) - seg0;
+            t_slot[i] = static_cast<int>(slot);
         }
-        g = warp_sum(g);
-        u = warp_sum(u);
-        if (lane_id() == 0) h[static_cast<int64_t>(p) * I + i] = g / (1.f + expf(-g)) * u;
+        __syncwarp();
+        const int total = warp_tile_prefix(n_active, prefix,
+                                           [&](int a) { return m_blocks * ((t_rows[a] + NT - 1) / NT); });
+        if (lane == 0) s_misc[0] = total;
     }
-}
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    // this CTA's share [w0, w1) of the (tile, K step) sequence; at least one step
+    // per sharing CTA, so every CTA between two sharers of a tile shares it too
+    const int64_t work = static_cast<int64_t>(s_misc[0]) * nkb;
+    const int64_t shares = max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), work));
+    const int64_t w0 = blockIdx.x < shares ? work * blockIdx.x / shares : 0;
+    const int64_t w1 = blockIdx.x < shares ? work * (blockIdx.x + 1) / shares : 0;
 
-__global__ void __launch_bounds__(256) k_mx4_down(const float* __restrict__ h, const int32_t* __restrict__ offsets,
-                                                  const int32_t* __restrict__ active, Mx4Slab w, int rows, int H, int I,
-                                                  int Hp, int Ip, uint16_t* __restrict__ y) {
-    griddep_wait();
-    griddep_launch();
-    const int p = static_cast<int>(blockIdx.x);
-    const int64_t slot = mx4_row_slot(w, offsets, active, p);
-    if (slot < 0) return;
-    const uint8_t* dc = w.codes + slot * w.code_stride + static_cast<int64_t>(Ip) * Hp;
-    const uint8_t* ds = w.scales + slot * w.scale_stride + static_cast<int64_t>(Ip) * Hp / 16;
-    for (int c = static_cast<int>(blockIdx.y) * 8 + static_cast<int>(threadIdx.x >> 5); c < H; c += 8 * gridDim.y) {
-        float acc = 0.f;
-        for (int k = static_cast<int>(lane_id()) * 8; k < I; k += 256) {
-            float hv[8], dv[8];
-            load8<float, true>(h + static_cast<int64_t>(p) * I + k, hv);
-            e2m1x8_to_float(*reinterpret_cast<const uint32_t*>(dc + (static_cast<int64_t>(c) * Ip + k) / 2), dv);
-            float a = 0.f;
-            for (int j = 0; j < 8; ++j) a += hv[j] * dv[j];
-            acc += a * mx_scale(ds[mx4_tile_scale(c, k, Ip)]);
+    struct Tile {
+        int a, ib, nb, kb0, kb1;
+        int64_t index;
+    };
+    auto decode = [&](int64_t w) {
+        Tile t;
+        t.index = w / nkb;
+        t.kb0 = static_cast<int>(w - t.index * nkb);
+        t.kb1 = static_cast<int>(min(static_cast<int64_t>(nkb), t.kb0 + (w1 - w)));
+        t.a = find_expert(prefix, n_active, static_cast<int>(t.index));
+        const int local = static_cast<int>(t.index) - prefix[t.a];
+        t.nb = local / m_blocks;
+        t.ib = local - t.nb * m_blocks;
+        return t;
+    };
+
+    if (warp == 0) {
+        // ---------------- weight producer ----------------
+        if (elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int64_t w = w0; w < w1 && ok;) {
+                const Tile t = decode(w);
+                w += t.kb1 - t.kb0;
+                const int64_t slot = t_slot[t.a];
+                const int row = static_cast<int>(slot * args.rows_per_slot) + t.ib * 128;
+                const int64_t sf_at = slot * args.scale_stride + static_cast<int64_t>(t.ib) * nkb * kMx4SfBytes;
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                    if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+                    unsigned char* sa = smem + stage * S::kStage;
+                    unsigned char* ss = s_sf + stage * S::kSf;
+                    mbar_arrive_expect_tx(&full_bar[stage], S::kATx + S::kB + 2 * kMx4SfBytes);
+                    tma_load_2d(sa, &tm_w, &full_bar[stage], kb * kMx4BK, row);
+                    bulk_load(ss, args.scales0 + sf_at + kb * kMx4SfBytes, kMx4SfBytes, &full_bar[stage]);
+                    if (SWIGLU) {
+                        tma_load_2d(sa + kMx4ABytes, &tm_w, &full_bar[stage], kb * kMx4BK, row + args.up_row);
+                        bulk_load(ss + kMx4SfBytes, args.scales1 + sf_at + kb * kMx4SfBytes, kMx4SfBytes,
+                                  &full_bar[stage]);
+                    }
+                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
         }
-        acc = warp_sum(acc);
-        if (lane_id() == 0) y[static_cast<int64_t>(p) * H + c] = f2bits(acc);
+        __syncwarp();
+    } else if (warp == 6) {
+        // ---------------- token producer ----------------
+        griddep_wait();
+        griddep_launch();
+        if (elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int64_t w = w0; w < w1 && ok;) {
+                const Tile t = decode(w);
+                w += t.kb1 - t.kb0;
+                const int row = t_seg0[t.a] + t.nb * NT;
+                const int64_t tt = prefix[t.a] / m_blocks + t.nb;
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                    if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+                    tma_load_3d(smem + stage * S::kStage + S::kA, &tm_x, &full_bar[stage], kb * kMx4BK, row, 0);
+                    if (!SWIGLU)
+                        bulk_load(s_sf + stage * S::kSf + kMx4SfBytes, args.sf + (tt * nkb + kb) * kMx4SfBytes,
+                                  kMx4SfBytes, &full_bar[stage]);
+                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        constexpr uint32_t idesc = mx4_idesc(S::kN);
+        if (elect_one()) tmem_cp_sf(tmem_base + kMx4OneCol, mx4_sf_desc(smem_u32(s_one)));
+        __syncwarp();
+        int stage = 0, lt = 0, step = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int64_t w = w0; w < w1 && ok; ++lt) {
+            const Tile t = decode(w);
+            w += t.kb1 - t.kb0;
+            const int b = S::kBufs == 2 ? (lt & 1) : 0;
+            const uint32_t acc_phase = static_cast<uint32_t>(S::kBufs == 2 ? lt >> 1 : lt) & 1u;
+            if (!mbar_wait(&tmem_empty[b], acc_phase ^ 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d = tmem_base + static_cast<uint32_t>(b * S::kAcc);
+            for (int kb = t.kb0; kb < t.kb1; ++kb, ++step) {
+                if (!mbar_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t sa = smem_u32(smem + stage * S::kStage);
+                    const uint32_t ss = smem_u32(s_sf + stage * S::kSf);
+                    const uint32_t sf = tmem_base + kMx4SfCol + static_cast<uint32_t>(step & 3) * 12;
+                    tmem_cp_sf(sf, mx4_sf_desc(ss));
+                    tmem_cp_sf(sf + (SWIGLU ? 4 : 8), mx4_sf_desc(ss + kMx4SfBytes));
+                    const uint32_t sfb = SWIGLU ? tmem_base + kMx4OneCol : sf + 8;
+                    const uint64_t a0 = sw128_desc(sa), a1 = sw128_desc(sa + kMx4ABytes);
+                    const uint64_t hi = sw128_desc(sa + S::kA), lo = sw128_desc(sa + S::kA + NT * kMx4BK);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint32_t acc = (kb > t.kb0 || kk > 0) ? 1u : 0u;
+                        const uint32_t id = idesc | (static_cast<uint32_t>(kk) << 29) | (static_cast<uint32_t>(kk) << 4);
+                        umma_mx4(d, a0 + 2u * kk, hi + 2u * kk, id, sf, sfb, acc);
+                        if (!S::kStack) umma_mx4(d, a0 + 2u * kk, lo + 2u * kk, id, sf, sfb, 1u);
+                        if (SWIGLU) {
+                            umma_mx4(d + S::kN, a1 + 2u * kk, hi + 2u * kk, id, sf + 4, sfb, acc);
+                            if (!S::kStack) umma_mx4(d + S::kN, a1 + 2u * kk, lo + 2u * kk, id, sf + 4, sfb, 1u);
+                        }
+                    }
+                    umma_commit(&empty_bar[stage]);
+                }
+                __syncwarp();
+                if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+            }
+            if (!ok) break;
+            if (elect_one()) umma_commit(&tmem_full[b]);
+            __syncwarp();
+        }
+    } else {
+        // ---------------- epilogue (warps 2..5) ----------------
+        griddep_wait();
+        const int q = warp & 3;
+        const int i_row = q * 32 + static_cast<int>(lane);
+        // 16 token columns from column c0 of the tile: gate (or down) sums g, up sums v
+        auto finish = [&](const Tile& t, int c0, float* g, float* v) {
+            const int r0 = t.nb * NT + c0;                       // row of the expert's segment
+            const int n = min(16, t_rows[t.a] - r0);
+            if (n <= 0) return;
+            const int64_t p0 = static_cast<int64_t>(t_seg0[t.a]) + r0;
+            const int col = t.ib * 128 + i_row;
+            if (SWIGLU) {
+                const float rs = static_cast<int>(lane) < n ? __ldcg(args.row_scale + p0 + lane) : 0.f;
+                uint32_t byte = 0;                               // lane j: scale byte of column j
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    float h[2];
+                    uint32_t by[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float s = __shfl_sync(0xffffffffu, rs, j + i);
+                        const float gs = g[j + i] * s;
+                        h[i] = __fdiv_rn(gs, 1.0f + expf(-gs)) * (v[j + i] * s);
+                        // the 32 lanes are one scale block of h
+                        by[i] = mx4_group_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7FFFFFFFu));
+                        h[i] *= mx4_inverse(by[i]);
+                        if (static_cast<int>(lane) == j + i) byte = by[i];
+                    }
+                    uint16_t hi, lo;
+                    e4m3_split2(h[0], h[1], hi, lo);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (j + i < n) {
+                            uint8_t* at = args.h + (p0 + j + i) * args.M + col;
+                            at[0] = static_cast<uint8_t>(hi >> (8 * i));
+                            at[static_cast<int64_t>(args.rows) * args.M] = static_cast<uint8_t>(lo >> (8 * i));
+                        }
+                }
+                const int r = c0 + static_cast<int>(lane);       // row of the token tile
+                if (lane < 16) {
+                    const int64_t tt = prefix[t.a] / m_blocks + t.nb;
+                    uint8_t* sf = args.sf + (tt * m_blocks + t.ib) * kMx4SfBytes + q;
+                    sf[(r & 31) * 16 + (r >> 5) * 4] = static_cast<uint8_t>(byte);
+                    if (S::kStack) sf[((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4] = static_cast<uint8_t>(byte);
+                }
+            } else if (col < args.ldy) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (j < n) args.y[(p0 + j) * args.ldy + col] = f2bits(g[j]);
+            }
+        };
+        int lt = 0;
+        for (int64_t w = w0; w < w1; ++lt) {
+            const Tile t = decode(w);
+            w += t.kb1 - t.kb0;
+            const int b = S::kBufs == 2 ? (lt & 1) : 0;
+            const uint32_t acc_phase = static_cast<uint32_t>(S::kBufs == 2 ? lt >> 1 : lt) & 1u;
+            if (!mbar_wait(&tmem_full[b], acc_phase, abort_flag)) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(b * S::kAcc);
+            const bool whole = t.kb0 == 0 && t.kb1 == nkb;
+            // a share of a tile: the part with the tile's first K step is its CTA's
+            // last tile (slot 1), every other part its CTA's first (slot 0)
+            float* mine = args.partials +
+                          (static_cast<int64_t>(blockIdx.x) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
+#pragma unroll
+            for (int c0 = 0; c0 < NT; c0 += 16) {
+                uint32_t r[4][16];
+                tmem_ld16(taddr + c0, r[0]);
+                if (S::kStack) tmem_ld16(taddr + NT + c0, r[1]);
+                if (SWIGLU) {
+                    tmem_ld16(taddr + S::kN + c0, r[2]);
+                    if (S::kStack) tmem_ld16(taddr + S::kN + NT + c0, r[3]);
+                }
+                tmem_wait_ld();
+                float g[16], v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    g[j] = __uint_as_float(r[0][j]) + (S::kStack ? __uint_as_float(r[1][j]) : 0.f);
+                    v[j] = SWIGLU ? __uint_as_float(r[2][j]) + (S::kStack ? __uint_as_float(r[3][j]) : 0.f) : 0.f;
+                }
+                if (c0 + 16 == NT) {
+                    tc_fence_before();
+                    mbar_arrive(&tmem_empty[b]);
+                }
+                if (whole) {
+                    finish(t, c0, g, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        mine[(c0 + j) * 128] = g[j];
+                        if (SWIGLU) mine[(NT + c0 + j) * 128] = v[j];
+                    }
+                }
+            }
+            if (whole) continue;
+            // the CTAs that share the tile: step w belongs to CTA floor(((w + 1) shares - 1) / work)
+            const int64_t first = t.index * nkb, last = first + nkb - 1;
+            const int c_first = static_cast<int>(((first + 1) * shares - 1) / work);
+            const int c_last = static_cast<int>(((last + 1) * shares - 1) / work);
+            __threadfence();
+            __syncwarp();
+            unsigned int prev = 0;
+            if (lane == 0) prev = atomicAdd(&args.tickets[t.index * 4 + q], 1u);
+            prev = __shfl_sync(0xffffffffu, prev, 0);
+            if (prev != static_cast<unsigned int>(c_last - c_first)) continue;
+            __threadfence();
+            for (int c0 = 0; c0 < NT; c0 += 16) {
+                float g[16], v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) g[j] = v[j] = 0.f;
+                for (int c = c_first; c <= c_last; ++c) {
+                    // c_first holds the tile's first K step
+                    const float* p = args.partials +
+                                     (static_cast<int64_t>(c) * 2 + (c == c_first ? 1 : 0)) * S::kCols * 128 + i_row;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        g[j] += __ldcg(p + (c0 + j) * 128);
+                        if (SWIGLU) v[j] += __ldcg(p + (NT + c0 + j) * 128);
+                    }
+                }
+                finish(t, c0, g, v);
+            }
+        }
+    }
+
+    __syncthreads();
+    if (*abort_flag) {
+        if (warp == 1) {
+            if (elect_one()) umma_commit(drain_bar);
+            __syncwarp();
+            volatile int never = 0;
+            mbar_wait(drain_bar, 0, &never);
+        }
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kMx4TmemCols)
+                     : "memory");
     }
 }
 

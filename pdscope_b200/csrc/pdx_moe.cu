@@ -17,8 +17,8 @@
 
 #include "block_norm.cu"
 #include "combine.cu"
-#include "ffn_decode.cu"
 #include "ffn_gemm.cu"
+#include "ffn_gemv.cu"
 #include "ffn_mx4.cu"
 #include "ffn_stream.cu"
 #include "pack.cu"
@@ -202,6 +202,13 @@ int device_setup(int* sms_out) {
         PDX_DEC_ATTR(true, 64, 16); PDX_DEC_ATTR(true, 64, 32); PDX_DEC_ATTR(true, 64, 64);
         PDX_DEC_ATTR(false, 16, 16); PDX_DEC_ATTR(false, 32, 32); PDX_DEC_ATTR(false, 64, 64);
 #undef PDX_DEC_ATTR
+#define PDX_MX4_ATTR(NT)                                                                                           \
+    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,           \
+                                      static_cast<int>(Mx4Shape<NT, true>::kSmem)));                               \
+    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,          \
+                                      static_cast<int>(Mx4Shape<NT, false>::kSmem)))
+        PDX_MX4_ATTR(16); PDX_MX4_ATTR(32); PDX_MX4_ATTR(64); PDX_MX4_ATTR(112);
+#undef PDX_MX4_ATTR
         g_num_sms[dev] = sms;
         g_attrs_set[dev] = true;
     }
@@ -213,7 +220,7 @@ int device_setup(int* sms_out) {
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
-int encode_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+int load_encode() {
     std::call_once(g_encode_once, [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -223,6 +230,12 @@ int encode_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, 
             g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     });
     if (!g_encode) return fail(PDX_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+    return PDX_OK;
+}
+
+int encode_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+    int st = load_encode();
+    if (st) return st;
     if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0) return fail(PDX_ERR_INVALID, "TMA base not 16-byte aligned");
     const cuuint64_t dims[2] = {cols, rows};
     const cuuint64_t strides[1] = {cols * 2};
@@ -920,8 +933,9 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
     if (H < 32 || I < 32 || H % 32 || I % 32)
         return fail(PDX_ERR_UNSUPPORTED, "H=%lld, I=%lld must be positive multiples of 32", static_cast<long long>(H),
                     static_cast<long long>(I));
-    if (H > 65536 || I > 65536 || rows >= (int64_t(1) << 31) || T >= (int64_t(1) << 31) || E > (int64_t(1) << 20))
+    if (H > 65536 || I > 65536 || rows > (int64_t(1) << 26) || T >= (int64_t(1) << 31))
         return fail(PDX_ERR_UNSUPPORTED, "FFN batch too large");
+    if (E > kMaxExperts) return fail(PDX_ERR_UNSUPPORTED, "E=%lld > %d experts", static_cast<long long>(E), kMaxExperts);
     if (!gathered && T < rows) return fail(PDX_ERR_INVALID, "x has fewer rows than the packed order");
     if (!w || !w->codes || !w->scales) return fail(PDX_ERR_INVALID, "expert weights missing");
     if (w->num_slots < 1) return fail(PDX_ERR_INVALID, "num_slots must be >= 1");
@@ -931,28 +945,129 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
     if (w->num_slots > 1 && (w->code_stride < 3 * Hp * Ip / 2 || w->scale_stride < 3 * Hp * Ip / 32 ||
                              w->code_stride % (Hp / 2) || w->code_stride % (Ip / 2) || w->scale_stride % 16))
         return fail(PDX_ERR_INVALID, "slot strides must cover one expert and be whole rows");
+    if (w->num_slots > 1 && w->num_slots * (w->code_stride / (std::min(Hp, Ip) / 2)) >= (int64_t(1) << 31))
+        return fail(PDX_ERR_UNSUPPORTED, "expert slab too large for 32-bit TMA row coordinates");
     return PDX_OK;
 }
 
+// Token tile of the MXFP4 path: the smallest that holds an expert's average
+// rows with room to spare (a tile's MMAs cost its full width), 112 at most (two
+// gate/up accumulators of 2 x 112 columns and the scales fill TMEM).
+int mx4_tile(int64_t rows, int64_t E) {
+    const int64_t est = std::max<int64_t>(1, std::min(E, rows));
+    const int64_t avg = (rows + est - 1) / est;
+    return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 48 ? 64 : 112));
+}
+
+struct Mx4Bufs {
+    int nt;
+    int64_t tiles;          // token tiles at most, over all experts
+    uint8_t* x;             // [2][rows][Hp] pieces of the gathered rows
+    float* row_scale;       // [rows]
+    uint8_t* h;             // [2][rows][Ip] pieces
+    uint8_t* sf;            // [tiles][Ip / 128] scale tiles of h
+    float* partials;        // [kPlanSMs][2][2 nt][128]
+    unsigned int* tickets;  // gate/up tiles * 4, then down tiles * 4
+    int64_t words1, words2;
+};
+
+Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
+    const int64_t Hp = round128(H), Ip = round128(I);
+    Mx4Bufs b{};
+    b.nt = mx4_tile(rows, E);
+    b.tiles = rows / b.nt + std::min(E, rows);
+    b.x = static_cast<uint8_t*>(c.take(2 * rows * Hp));
+    b.row_scale = static_cast<float*>(c.take(rows * 4));
+    b.h = static_cast<uint8_t*>(c.take(2 * rows * Ip));
+    b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * kMx4SfBytes));
+    b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * 2 * b.nt * 128 * 4));
+    b.words1 = b.tiles * (Ip / 128) * 4;
+    b.words2 = b.tiles * (Hp / 128) * 4;
+    b.tickets = static_cast<unsigned int*>(c.take((b.words1 + b.words2) * 4));
+    return b;
+}
+
 size_t mx4_ffn_ws_bytes(int64_t rows, int64_t E, int64_t H, int64_t I) {
-    return align_up(static_cast<size_t>(rows) * I * 4);
+    Carver c{nullptr, SIZE_MAX};
+    carve_mx4(c, rows, E, H, I);
+    return c.used;
+}
+
+// Codes as a [rows, cols] matrix of 4-bit values, unpacked to bytes in shared memory; 128 x 128 boxes.
+int encode_mx4_weights(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols) {
+    int st = load_encode();
+    if (st) return st;
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {cols / 2};
+    const cuuint32_t box[2] = {kMx4BK, 128};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(base), dims, strides, box,
+                          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(PDX_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return PDX_OK;
+}
+
+// E4M3 pieces [2][rows][cols]; boxes of 128 columns x box_rows of both pieces.
+int encode_mx4_tokens(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+    int st = load_encode();
+    if (st) return st;
+    const cuuint64_t dims[3] = {cols, rows, 2};
+    const cuuint64_t strides[2] = {cols, cols * rows};
+    const cuuint32_t box[3] = {kMx4BK, box_rows, 2};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(PDX_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return PDX_OK;
+}
+
+template <int NT>
+int launch_mx4_pair(const CUtensorMap& tm_gu, const CUtensorMap& tm_x, const Mx4Args& gu, const CUtensorMap& tm_d,
+                    const CUtensorMap& tm_h, const Mx4Args& down, int64_t tiles, int sms, cudaStream_t stream) {
+    const int64_t most = std::min(sms, kPlanSMs);   // the partial sums are sized for kPlanSMs CTAs
+    const int64_t work1 = tiles * (gu.M / 128) * (gu.K / kMx4BK), work2 = tiles * (down.M / 128) * (down.K / kMx4BK);
+    PDX_PDL_TRY(launch_pdl(k_mx4_gemm<NT, true>, dim3(static_cast<unsigned>(std::min(most, work1))), dim3(kMx4Threads),
+                           Mx4Shape<NT, true>::kSmem, stream, tm_gu, tm_x, gu));
+    PDX_PDL_TRY(launch_pdl(k_mx4_gemm<NT, false>, dim3(static_cast<unsigned>(std::min(most, work2))), dim3(kMx4Threads),
+                           Mx4Shape<NT, false>::kSmem, stream, tm_d, tm_h, down));
+    return PDX_OK;
 }
 
 int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_t* offsets, const int32_t* active,
                    int64_t E, int64_t rows, const pdx_mxfp4_weights* w, int64_t H, int64_t I, void* y, Carver& ws,
                    cudaStream_t stream) {
-    float* h = static_cast<float*>(ws.take(static_cast<size_t>(rows) * I * 4));
+    const Mx4Bufs b = carve_mx4(ws, rows, E, H, I);
     if (ws.overflow) return fail(PDX_ERR_WORKSPACE, "FFN workspace too small (%zu > %zu bytes)", ws.used, ws.cap);
-    const Mx4Slab slab{static_cast<const uint8_t*>(w->codes), static_cast<const uint8_t*>(w->scales), w->code_stride,
-                       w->scale_stride, w->num_slots, w->slot_of_expert};
-    const int Hi = static_cast<int>(H), Ii = static_cast<int>(I), n = static_cast<int>(rows);
-    const int Hp = static_cast<int>(round128(H)), Ip = static_cast<int>(round128(I));
-    const unsigned split = rows < 1024 ? 16 : 1;
-    PDX_PDL_TRY(launch_pdl(k_mx4_gateup, dim3(n, split), dim3(256), 0, stream, static_cast<const uint16_t*>(x), tokens,
-                           static_cast<int>(T), offsets, active, slab, n, Hi, Ii, Hp, Ip, h));
-    PDX_PDL_TRY(launch_pdl(k_mx4_down, dim3(n, split), dim3(256), 0, stream, static_cast<const float*>(h), offsets,
-                           active, slab, n, Hi, Ii, Hp, Ip, static_cast<uint16_t*>(y)));
-    return PDX_OK;
+    int sms = 0;
+    int st = device_setup(&sms);
+    if (st) return st;
+    const int Hp = static_cast<int>(round128(H)), Ip = static_cast<int>(round128(I)), n = static_cast<int>(rows);
+    const int64_t per = static_cast<int64_t>(Hp) * Ip;
+    const int64_t slots = w->num_slots, cs = slots > 1 ? w->code_stride : 0, ss = slots > 1 ? w->scale_stride : 0;
+    const uint8_t* codes = static_cast<const uint8_t*>(w->codes);
+    const uint8_t* scales = static_cast<const uint8_t*>(w->scales);
+    const int64_t gu_rows = cs / (Hp / 2), down_rows = cs / (Ip / 2);   // map rows between slots
+    CUtensorMap tm_gu, tm_x, tm_d, tm_h;
+    if ((st = encode_mx4_weights(&tm_gu, codes, (slots - 1) * gu_rows + 2 * Ip, Hp))) return st;
+    if ((st = encode_mx4_weights(&tm_d, codes + per, (slots - 1) * down_rows + Hp, Ip))) return st;
+    if ((st = encode_mx4_tokens(&tm_x, b.x, rows, Hp, b.nt))) return st;
+    if ((st = encode_mx4_tokens(&tm_h, b.h, rows, Ip, b.nt))) return st;
+    const dim3 split_grid(static_cast<unsigned>(std::min<int64_t>((rows + kMx4SplitWarps - 1) / kMx4SplitWarps,
+                                                                  16 * kPlanSMs)));
+    PDX_PDL_TRY(launch_pdl(k_mx4_split, split_grid, dim3(kMx4SplitWarps * 32), 0, stream,
+                           static_cast<const uint16_t*>(x), tokens, static_cast<int>(T), n, static_cast<int>(H), Hp,
+                           b.x, b.row_scale, b.tickets, static_cast<int>(b.words1 + b.words2)));
+    Mx4Args gu{offsets, active, w->slot_of_expert, slots, scales, scales + per / 32, ss, gu_rows, Ip, Hp, Ip, n,
+               b.row_scale, b.sf, b.h, nullptr, 0, b.partials, b.tickets};
+    Mx4Args down{offsets, active, w->slot_of_expert, slots, scales + per / 16, nullptr, ss, down_rows, 0, Ip, Hp, n,
+                 nullptr, b.sf, nullptr, static_cast<uint16_t*>(y), static_cast<int>(H), b.partials,
+                 b.tickets + b.words1};
+    if (b.nt == 16) return launch_mx4_pair<16>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
+    if (b.nt == 32) return launch_mx4_pair<32>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
+    if (b.nt == 64) return launch_mx4_pair<64>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
+    return launch_mx4_pair<112>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
 }
 
 // ---- block norms ---------------------------------------------------------------------
