@@ -327,15 +327,14 @@ int pdx_mxfp4_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols,
 int pdx_mxfp4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t cols, int64_t ld,
                          int32_t dtype, void *out, pdx_stream_t stream);
 
-/* MXFP4 experts, the 4-bit form of pdx_expert_weights.  With Hp, Ip = H, I
- * rounded up to 128, slot s holds
- *   codes  + s*code_stride:  gate [Ip, Hp/2] | up [Ip, Hp/2] | down [Hp, Ip/2]
- *   scales + s*scale_stride: the scales of gate | up | down, 3*Ip*Hp/32 bytes
- * (strides in bytes, padding rows and columns zero).  A projection's scales
- * are stored as tiles of 128 rows x 128 columns, 512 bytes each, row tiles
- * outermost: byte (r % 32)*16 + (r / 32)*4 + c / 32 of a tile belongs to row r
- * and columns c .. c + 31.  codes 128-byte, scales 16-byte aligned;
- * code_stride a multiple of Hp/2 and of Ip/2, scale_stride of 16. */
+/* MXFP4 experts, the 4-bit form of pdx_expert_weights.  A projection [N, K] is
+ * stored as tiles of 128 rows x 128 columns (N, K rounded up to 128, padding
+ * zero), row tiles outermost.  A tile's codes are 8192 bytes, 128 rows of 64;
+ * its scales are 512 bytes: byte (r % 32)*16 + (r / 32)*4 + c / 32 belongs to
+ * row r and columns c .. c + 31.  Slot s holds the tiles of gate [I, H], up
+ * [I, H] and down [H, I] back to back from codes + s*code_stride, and their
+ * scales from scales + s*scale_stride (strides in bytes).  codes 128-byte,
+ * scales 16-byte aligned; code_stride a multiple of 8192, scale_stride of 16. */
 typedef struct pdx_mxfp4_weights {
     const void *codes;
     const void *scales;

@@ -17,17 +17,19 @@
 // row (a factor on the row of the result), h per 32 values of I (an E8M0 scale
 // of the second product).  W hi and W lo cost what one BF16 product would.
 //
-// Two launches of k_mx4_gemm: gate and up with the SwiGLU (two accumulators),
-// then down.  tokens are the N operand, NT packed rows of one expert a tile; up
-// to NT = 32 the two pieces are stacked along N (one pass over the weights in
-// shared memory), above that they accumulate into the same columns.
+// Two launches of k_mx4_gemm, each on tiles of 256 weight rows (two accumulators
+// over one token operand): 128 rows of gate and the same 128 of up with the
+// SwiGLU, then 256 rows of down.  Tokens are the N operand, NT packed rows of
+// one expert a tile; up to NT = 32 the two pieces are stacked along N (one pass
+// over the weights in shared memory), above that they accumulate into the same
+// columns.
 // Work is cut evenly: the (tile, K step) pairs of the launch form one sequence
 // and CTA c takes an equal share of it, so a decode step of any batch keeps
 // every SM streaming; a tile that spans CTAs is summed in CTA order by the warp
 // that takes its last ticket (FP32, deterministic, nothing waits).
-// Roles (224 threads): warp 0 streams weights and scales, warp 6 the token
-// pieces, warp 1 issues the MMAs, warps 2..5 are the epilogue (32 weight rows,
-// = one scale block of h, each).  Neither launch waits for another CTA; the
+// Roles (352 threads): warp 0 streams weights and scales, warp 10 the token
+// pieces, warp 1 issues the MMAs, warps 2..9 are the epilogue (32 weight rows,
+// = one scale block of h, and every other 8 token columns each).  Neither launch waits for another CTA; the
 // weight stream of a launch starts before the launch before it has finished.
 #include <cuda.h>
 
@@ -37,9 +39,12 @@
 
 namespace pdx {
 
-constexpr int kMx4Threads = 224;
+constexpr int kMx4Threads = 352;
+constexpr int kMx4EpiWarps = 8;
+constexpr int kMx4Chunk = 8;                        // token columns an epilogue warp takes at a time
 constexpr int kMx4BK = 128;                         // K step: 4 MMAs of 32
 constexpr uint32_t kMx4ABytes = 128 * kMx4BK;       // one weight tile, a byte per code
+constexpr int kMx4TileBytes = 128 * kMx4BK / 2;     // its codes in memory
 constexpr uint32_t kMx4SfBytes = 512;               // scales of 128 rows x 128 columns
 constexpr int kMx4MaxActive = 1024;
 constexpr uint32_t kMx4TmemCols = 512;
@@ -47,18 +52,20 @@ constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of (gate | up | t
 constexpr uint32_t kMx4OneCol = 496;                // token scales of 1 (x is scaled by its row factor)
 constexpr int kMx4SmemLimit = 227 * 1024;
 
-// byte -> 2^(byte - 127), the inverse as a factor for byte <= 253
-__device__ __forceinline__ uint32_t mx4_group_byte(uint32_t max_bits) {  // largest value -> [128, 256)
+// Scale byte b of a group from the bits of its largest magnitude, which 2^(127 - b)
+// takes into [128, 256); 248 if the group holds an infinity or NaN.
+__device__ __forceinline__ uint32_t mx4_group_byte(uint32_t max_bits) {
     const uint32_t e = max_bits >> 23;
     return e > 7u ? e - 7u : 0u;
 }
-__device__ __forceinline__ float mx4_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// 2^(127 - b), or NaN for a non-finite group: e4m3 has no infinity, and
+// saturating would hide one.
+__device__ __forceinline__ float mx4_inverse(uint32_t b) {
+    return __uint_as_float(b < 248u ? (254u - b) << 23 : 0x7FC00000u);
+}
 
-// Two values -> their E4M3 pieces (a in the low byte); non-finite -> NaN.
+// Two values -> their E4M3 pieces (a in the low byte).
 __device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint16_t& lo) {
-    // infinities become NaN (e4m3 has none, and saturating would hide them)
-    a = a - (a - a);
-    b = b - (b - b);
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b), "f"(a));
     uint32_t h2;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(hi));
@@ -125,21 +132,26 @@ struct Mx4Args {
     const int32_t* active;          // [E+1] active count, then the active expert ids
     const int32_t* slot_of_expert;  // NULL = identity
     int64_t num_slots;
-    const uint8_t* scales0;         // weight scales of slot 0: gate, or down
-    const uint8_t* scales1;         // up
+    const uint8_t* scales;          // weight scales of slot 0
     int64_t scale_stride;           // bytes between slots
-    int64_t rows_per_slot;          // TMA-map rows between slots
-    int up_row;                     // TMA-map row of up relative to gate
+    int64_t tiles_per_slot;         // weight tiles between slots
+    int tile0, tile1;               // first weight tile of gate and up, or of down (tile0)
     int K, M;                       // multiples of 128: reduction length, weight rows
-    int rows;
+    int rows, experts;
     const float* row_scale;         // [rows] factor of a packed row of x (SWIGLU)
     uint8_t* sf;                    // h scales: [token tile][Ip / 128] tiles of 512 bytes (out of SWIGLU, else in)
     uint8_t* h;                     // [2][rows][M] pieces (SWIGLU)
     uint16_t* y;                    // [rows, ldy] (down)
     int ldy;                        // H
     float* partials;                // [gridDim.x][2][columns][128]
-    unsigned int* tickets;          // [tiles * 4], zero on entry
+    unsigned int* tickets;          // [tiles * kMx4EpiWarps], zero on entry
 };
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
 
 __device__ __forceinline__ uint64_t mx4_sf_desc(uint32_t smem_addr) {  // 32 x 16 bytes, 8-row groups 128 bytes apart
     return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) |
@@ -182,28 +194,27 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, ui
         : "memory");
 }
 
-template <int NT, bool SWIGLU>
+template <int NT>
 struct Mx4Shape {
     static constexpr bool kStack = NT <= 32;                        // pieces side by side along N
     static constexpr int kN = kStack ? 2 * NT : NT;                 // N of one MMA
-    static constexpr int kAcc = (SWIGLU ? 2 : 1) * kN;              // accumulator columns
-    static constexpr int kBufs = 2 * kAcc <= static_cast<int>(kMx4SfCol) ? 2 : 1;
-    static constexpr int kCols = (SWIGLU ? 2 : 1) * NT;             // FP32 columns of a partial tile
-    static constexpr uint32_t kA = (SWIGLU ? 2 : 1) * kMx4ABytes;
+    static constexpr int kAcc = 2 * kN;                             // accumulator columns of a tile
+    static constexpr int kCols = 2 * NT;                            // FP32 columns of a partial tile
+    static constexpr uint32_t kA = 2 * kMx4ABytes;
     static constexpr uint32_t kATx = kA / 2;                        // the copy counts the packed bytes it reads
     static constexpr uint32_t kB = 2 * NT * kMx4BK;
     static constexpr uint32_t kStage = kA + kB;                     // multiple of 1024
-    static constexpr uint32_t kSf = 2 * kMx4SfBytes;                // gate | up, or down | tokens
+    static constexpr uint32_t kSf = 3 * kMx4SfBytes;                // both weight halves | tokens
     static constexpr uint32_t kTables = 4 * (kMx4MaxActive + 1) * 4;
     static constexpr int kStages = static_cast<int>((kMx4SmemLimit - 1024 - 512 - 512 - kTables) / (kStage + kSf));
     static constexpr size_t kSmem = 1024 + kStages * (kStage + kSf) + 512 + 512 + kTables;
-    static_assert(NT % 16 == 0 && NT <= 128 && kStages >= 2 && kAcc <= static_cast<int>(kMx4SfCol), "token tile");
+    static_assert(NT % 16 == 0 && kStages >= 2 && 2 * kAcc <= static_cast<int>(kMx4SfCol), "token tile");
 };
 
 template <int NT, bool SWIGLU>
 __global__ void __launch_bounds__(kMx4Threads, 1)
     k_mx4_gemm(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, Mx4Args args) {
-    using S = Mx4Shape<NT, SWIGLU>;
+    using S = Mx4Shape<NT>;
     extern __shared__ __align__(1024) unsigned char smem_mx4[];
     unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
     unsigned char* s_sf = smem + S::kStages * S::kStage;             // kStages x kSf
@@ -225,6 +236,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     const int warp = static_cast<int>(threadIdx.x >> 5);
     const uint32_t lane = lane_id();
     const int m_blocks = args.M / 128, nkb = args.K / kMx4BK;
+    const int m_tiles = SWIGLU ? m_blocks : (m_blocks + 1) / 2;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -233,7 +245,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tmem_full[b], 1);
-            mbar_init(&tmem_empty[b], 128);
+            mbar_init(&tmem_empty[b], kMx4EpiWarps * 32);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -254,28 +266,28 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     // The routing tables are older than the launch before this one, which has
     // passed its own wait by the time this one starts; only that launch's
     // output (the token pieces) has to be waited for, by the warps that read it.
-    const int n_active = max(0, min(__ldcg(args.active), kMx4MaxActive));
-    if (warp == 2) {
-        for (int i = static_cast<int>(lane); i < n_active; i += 32) {
-            const int e = __ldcg(args.active + 1 + i);
-            const int seg0 = __ldcg(args.offsets + e);
-            int64_t slot = args.slot_of_expert ? __ldcg(args.slot_of_expert + e) : e;
-            if (slot < 0 || slot >= args.num_slots) {
-                raise_error(PDX_DEVERR_BAD_SLOT);
-                slot = 0;
-            }
-            t_seg0[i] = seg0;
-            t_rows[i] = __ldcg(args.offsets + e + 1) - seg0;
-            t_slot[i] = static_cast<int>(slot);
+    const int n_active = max(0, min(__ldcg(args.active), min(args.experts, kMx4MaxActive)));
+    for (int i = static_cast<int>(threadIdx.x); i < n_active; i += kMx4Threads) {
+        const int e = __ldcg(args.active + 1 + i);
+        const int seg0 = __ldcg(args.offsets + e);
+        int64_t slot = args.slot_of_expert ? __ldcg(args.slot_of_expert + e) : e;
+        if (slot < 0 || slot >= args.num_slots) {
+            raise_error(PDX_DEVERR_BAD_SLOT);
+            slot = 0;
         }
-        __syncwarp();
-        const int total = warp_tile_prefix(n_active, prefix,
-                                           [&](int a) { return m_blocks * ((t_rows[a] + NT - 1) / NT); });
-        if (lane == 0) s_misc[0] = total;
+        t_seg0[i] = seg0;
+        t_rows[i] = __ldcg(args.offsets + e + 1) - seg0;
+        t_slot[i] = static_cast<int>(slot);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (warp == 2) {
+        const int total = warp_tile_prefix(n_active, prefix,
+                                           [&](int a) { return m_tiles * ((t_rows[a] + NT - 1) / NT); });
+        if (lane == 0) s_misc[0] = total;
+    }
+    __syncthreads();
     const uint32_t tmem_base = *tmem_slot;
     // this CTA's share [w0, w1) of the (tile, K step) sequence; at least one step
     // per sharing CTA, so every CTA between two sharers of a tile shares it too
@@ -285,7 +297,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     const int64_t w1 = blockIdx.x < shares ? work * (blockIdx.x + 1) / shares : 0;
 
     struct Tile {
-        int a, ib, nb, kb0, kb1;
+        int a, mt, nb, kb0, kb1;
         int64_t index;
     };
     auto decode = [&](int64_t w) {
@@ -295,8 +307,8 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         t.kb1 = static_cast<int>(min(static_cast<int64_t>(nkb), t.kb0 + (w1 - w)));
         t.a = find_expert(prefix, n_active, static_cast<int>(t.index));
         const int local = static_cast<int>(t.index) - prefix[t.a];
-        t.nb = local / m_blocks;
-        t.ib = local - t.nb * m_blocks;
+        t.nb = local / m_tiles;
+        t.mt = local - t.nb * m_tiles;
         return t;
     };
 
@@ -310,26 +322,28 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 const Tile t = decode(w);
                 w += t.kb1 - t.kb0;
                 const int64_t slot = t_slot[t.a];
-                const int row = static_cast<int>(slot * args.rows_per_slot) + t.ib * 128;
-                const int64_t sf_at = slot * args.scale_stride + static_cast<int64_t>(t.ib) * nkb * kMx4SfBytes;
+                // weight tiles of both halves; down's odd last block is loaded twice, its second half unused
+                const int b0 = SWIGLU ? args.tile0 + t.mt * nkb : args.tile0 + 2 * t.mt * nkb;
+                const int b1 = SWIGLU ? args.tile1 + t.mt * nkb : args.tile0 + min(2 * t.mt + 1, m_blocks - 1) * nkb;
+                const int row = static_cast<int>(slot * args.tiles_per_slot) * 128;
+                const uint8_t* sf = args.scales + slot * args.scale_stride;
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
                     unsigned char* sa = smem + stage * S::kStage;
                     unsigned char* ss = s_sf + stage * S::kSf;
-                    mbar_arrive_expect_tx(&full_bar[stage], S::kATx + S::kB + 2 * kMx4SfBytes);
-                    tma_load_2d(sa, &tm_w, &full_bar[stage], kb * kMx4BK, row);
-                    bulk_load(ss, args.scales0 + sf_at + kb * kMx4SfBytes, kMx4SfBytes, &full_bar[stage]);
-                    if (SWIGLU) {
-                        tma_load_2d(sa + kMx4ABytes, &tm_w, &full_bar[stage], kb * kMx4BK, row + args.up_row);
-                        bulk_load(ss + kMx4SfBytes, args.scales1 + sf_at + kb * kMx4SfBytes, kMx4SfBytes,
-                                  &full_bar[stage]);
-                    }
+                    mbar_arrive_expect_tx(&full_bar[stage],
+                                          S::kATx + S::kB + (SWIGLU ? 2 : 3) * kMx4SfBytes);
+                    tma_load_2d(sa, &tm_w, &full_bar[stage], 0, row + (b0 + kb) * 128);
+                    tma_load_2d(sa + kMx4ABytes, &tm_w, &full_bar[stage], 0, row + (b1 + kb) * 128);
+                    bulk_load(ss, sf + static_cast<int64_t>(b0 + kb) * kMx4SfBytes, kMx4SfBytes, &full_bar[stage]);
+                    bulk_load(ss + kMx4SfBytes, sf + static_cast<int64_t>(b1 + kb) * kMx4SfBytes, kMx4SfBytes,
+                              &full_bar[stage]);
                     if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
                 }
             }
         }
         __syncwarp();
-    } else if (warp == 6) {
+    } else if (warp == 2 + kMx4EpiWarps) {
         // ---------------- token producer ----------------
         griddep_wait();
         griddep_launch();
@@ -341,12 +355,12 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 const Tile t = decode(w);
                 w += t.kb1 - t.kb0;
                 const int row = t_seg0[t.a] + t.nb * NT;
-                const int64_t tt = prefix[t.a] / m_blocks + t.nb;
+                const int64_t tt = prefix[t.a] / m_tiles + t.nb;
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
                     tma_load_3d(smem + stage * S::kStage + S::kA, &tm_x, &full_bar[stage], kb * kMx4BK, row, 0);
                     if (!SWIGLU)
-                        bulk_load(s_sf + stage * S::kSf + kMx4SfBytes, args.sf + (tt * nkb + kb) * kMx4SfBytes,
+                        bulk_load(s_sf + stage * S::kSf + 2 * kMx4SfBytes, args.sf + (tt * nkb + kb) * kMx4SfBytes,
                                   kMx4SfBytes, &full_bar[stage]);
                     if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -364,8 +378,8 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         for (int64_t w = w0; w < w1 && ok; ++lt) {
             const Tile t = decode(w);
             w += t.kb1 - t.kb0;
-            const int b = S::kBufs == 2 ? (lt & 1) : 0;
-            const uint32_t acc_phase = static_cast<uint32_t>(S::kBufs == 2 ? lt >> 1 : lt) & 1u;
+            const int b = lt & 1;
+            const uint32_t acc_phase = static_cast<uint32_t>(lt >> 1) & 1u;
             if (!mbar_wait(&tmem_empty[b], acc_phase ^ 1u, abort_flag)) { ok = false; break; }
             tc_fence_after();
             const uint32_t d = tmem_base + static_cast<uint32_t>(b * S::kAcc);
@@ -377,7 +391,8 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     const uint32_t ss = smem_u32(s_sf + stage * S::kSf);
                     const uint32_t sf = tmem_base + kMx4SfCol + static_cast<uint32_t>(step & 3) * 12;
                     tmem_cp_sf(sf, mx4_sf_desc(ss));
-                    tmem_cp_sf(sf + (SWIGLU ? 4 : 8), mx4_sf_desc(ss + kMx4SfBytes));
+                    tmem_cp_sf(sf + 4, mx4_sf_desc(ss + kMx4SfBytes));
+                    if (!SWIGLU) tmem_cp_sf(sf + 8, mx4_sf_desc(ss + 2 * kMx4SfBytes));
                     const uint32_t sfb = SWIGLU ? tmem_base + kMx4OneCol : sf + 8;
                     const uint64_t a0 = sw128_desc(sa), a1 = sw128_desc(sa + kMx4ABytes);
                     const uint64_t hi = sw128_desc(sa + S::kA), lo = sw128_desc(sa + S::kA + NT * kMx4BK);
@@ -387,10 +402,8 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                         const uint32_t id = idesc | (static_cast<uint32_t>(kk) << 29) | (static_cast<uint32_t>(kk) << 4);
                         umma_mx4(d, a0 + 2u * kk, hi + 2u * kk, id, sf, sfb, acc);
                         if (!S::kStack) umma_mx4(d, a0 + 2u * kk, lo + 2u * kk, id, sf, sfb, 1u);
-                        if (SWIGLU) {
-                            umma_mx4(d + S::kN, a1 + 2u * kk, hi + 2u * kk, id, sf + 4, sfb, acc);
-                            if (!S::kStack) umma_mx4(d + S::kN, a1 + 2u * kk, lo + 2u * kk, id, sf + 4, sfb, 1u);
-                        }
+                        umma_mx4(d + S::kN, a1 + 2u * kk, hi + 2u * kk, id, sf + 4, sfb, acc);
+                        if (!S::kStack) umma_mx4(d + S::kN, a1 + 2u * kk, lo + 2u * kk, id, sf + 4, sfb, 1u);
                     }
                     umma_commit(&empty_bar[stage]);
                 }
@@ -402,63 +415,74 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             __syncwarp();
         }
     } else {
-        // ---------------- epilogue (warps 2..5) ----------------
+        // ---------------- epilogue (warps 2..9) ----------------
         griddep_wait();
-        const int q = warp & 3;
+        const int q = warp & 3;                                  // TMEM lane quadrant
+        const int half = (warp - 2) >> 2;                        // this warp's chunks: half, half + 2, ...
         const int i_row = q * 32 + static_cast<int>(lane);
-        // 16 token columns from column c0 of the tile: gate (or down) sums g, up sums v
-        auto finish = [&](const Tile& t, int c0, float* g, float* v) {
+        // Token columns [c0, c0 + 8) of a tile: the sums g of the first, u of the second 128 weight rows.
+        auto finish = [&](const Tile& t, int c0, float (&g)[kMx4Chunk], float (&u)[kMx4Chunk]) {
             const int r0 = t.nb * NT + c0;                       // row of the expert's segment
-            const int n = min(16, t_rows[t.a] - r0);
+            const int n = min(kMx4Chunk, t_rows[t.a] - r0);
             if (n <= 0) return;
             const int64_t p0 = static_cast<int64_t>(t_seg0[t.a]) + r0;
-            const int col = t.ib * 128 + i_row;
             if (SWIGLU) {
                 const float rs = static_cast<int>(lane) < n ? __ldcg(args.row_scale + p0 + lane) : 0.f;
                 uint32_t byte = 0;                               // lane j: scale byte of column j
+                uint8_t* at = args.h + p0 * args.M + t.mt * 128 + i_row;
+                const int64_t lo_at = static_cast<int64_t>(args.rows) * args.M;
+                uint32_t top[kMx4Chunk];
 #pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    float h[2];
-                    uint32_t by[2];
+                for (int j = 0; j < kMx4Chunk; ++j) {
+                    const float s = __shfl_sync(0xffffffffu, rs, j);
+                    const float gs = g[j] * s;
+                    g[j] = __fdividef(gs, 1.0f + __expf(-gs)) * (u[j] * s);
+                    // the 32 lanes are one scale block of h
+                    top[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(g[j]) & 0x7FFFFFFFu);
+                }
+#pragma unroll
+                for (int j = 0; j < kMx4Chunk; ++j) {
+                    const uint32_t by = mx4_group_byte(top[j]);
+                    g[j] *= mx4_inverse(by);
+                    if (static_cast<int>(lane) == j) byte = by;
+                }
+#pragma unroll
+                for (int j = 0; j < kMx4Chunk; j += 2) {
+                    uint16_t hi, lo;
+                    e4m3_split2(g[j], g[j + 1], hi, lo);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float s = __shfl_sync(0xffffffffu, rs, j + i);
-                        const float gs = g[j + i] * s;
-                        h[i] = __fdiv_rn(gs, 1.0f + expf(-gs)) * (v[j + i] * s);
-                        // the 32 lanes are one scale block of h
-                        by[i] = mx4_group_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7FFFFFFFu));
-                        h[i] *= mx4_inverse(by[i]);
-                        if (static_cast<int>(lane) == j + i) byte = by[i];
-                    }
-                    uint16_t hi, lo;
-                    e4m3_split2(h[0], h[1], hi, lo);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
                         if (j + i < n) {
-                            uint8_t* at = args.h + (p0 + j + i) * args.M + col;
                             at[0] = static_cast<uint8_t>(hi >> (8 * i));
-                            at[static_cast<int64_t>(args.rows) * args.M] = static_cast<uint8_t>(lo >> (8 * i));
+                            at[lo_at] = static_cast<uint8_t>(lo >> (8 * i));
                         }
+                        at += args.M;
+                    }
                 }
-                const int r = c0 + static_cast<int>(lane);       // row of the token tile
-                if (lane < 16) {
-                    const int64_t tt = prefix[t.a] / m_blocks + t.nb;
-                    uint8_t* sf = args.sf + (tt * m_blocks + t.ib) * kMx4SfBytes + q;
+                if (lane < kMx4Chunk) {
+                    const int r = c0 + static_cast<int>(lane);   // row of the token tile
+                    const int64_t tt = prefix[t.a] / m_tiles + t.nb;
+                    uint8_t* sf = args.sf + (tt * m_blocks + t.mt) * kMx4SfBytes + q;
                     sf[(r & 31) * 16 + (r >> 5) * 4] = static_cast<uint8_t>(byte);
                     if (S::kStack) sf[((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4] = static_cast<uint8_t>(byte);
                 }
-            } else if (col < args.ldy) {
+            } else {
+                const int col = t.mt * 256 + i_row;
+                uint16_t* at = args.y + p0 * args.ldy + col;
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (j < n) args.y[(p0 + j) * args.ldy + col] = f2bits(g[j]);
+                for (int j = 0; j < kMx4Chunk; ++j) {
+                    if (j < n && col < args.ldy) at[0] = f2bits(g[j]);
+                    if (j < n && col + 128 < args.ldy) at[128] = f2bits(u[j]);
+                    at += args.ldy;
+                }
             }
         };
         int lt = 0;
         for (int64_t w = w0; w < w1; ++lt) {
             const Tile t = decode(w);
             w += t.kb1 - t.kb0;
-            const int b = S::kBufs == 2 ? (lt & 1) : 0;
-            const uint32_t acc_phase = static_cast<uint32_t>(S::kBufs == 2 ? lt >> 1 : lt) & 1u;
+            const int b = lt & 1;
+            const uint32_t acc_phase = static_cast<uint32_t>(lt >> 1) & 1u;
             if (!mbar_wait(&tmem_full[b], acc_phase, abort_flag)) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(b * S::kAcc);
@@ -467,33 +491,32 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             // last tile (slot 1), every other part its CTA's first (slot 0)
             float* mine = args.partials +
                           (static_cast<int64_t>(blockIdx.x) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
-#pragma unroll
-            for (int c0 = 0; c0 < NT; c0 += 16) {
-                uint32_t r[4][16];
-                tmem_ld16(taddr + c0, r[0]);
-                if (S::kStack) tmem_ld16(taddr + NT + c0, r[1]);
-                if (SWIGLU) {
-                    tmem_ld16(taddr + S::kN + c0, r[2]);
-                    if (S::kStack) tmem_ld16(taddr + S::kN + NT + c0, r[3]);
+            for (int c0 = half * kMx4Chunk; c0 < NT; c0 += 2 * kMx4Chunk) {
+                uint32_t r[4][kMx4Chunk];
+                tmem_ld8(taddr + c0, r[0]);
+                tmem_ld8(taddr + S::kN + c0, r[1]);
+                if (S::kStack) {
+                    tmem_ld8(taddr + NT + c0, r[2]);
+                    tmem_ld8(taddr + S::kN + NT + c0, r[3]);
                 }
                 tmem_wait_ld();
-                float g[16], v[16];
+                float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    g[j] = __uint_as_float(r[0][j]) + (S::kStack ? __uint_as_float(r[1][j]) : 0.f);
-                    v[j] = SWIGLU ? __uint_as_float(r[2][j]) + (S::kStack ? __uint_as_float(r[3][j]) : 0.f) : 0.f;
+                for (int j = 0; j < kMx4Chunk; ++j) {
+                    g[j] = __uint_as_float(r[0][j]) + (S::kStack ? __uint_as_float(r[2][j]) : 0.f);
+                    u[j] = __uint_as_float(r[1][j]) + (S::kStack ? __uint_as_float(r[3][j]) : 0.f);
                 }
-                if (c0 + 16 == NT) {
+                if (c0 + 2 * kMx4Chunk >= NT) {
                     tc_fence_before();
                     mbar_arrive(&tmem_empty[b]);
                 }
                 if (whole) {
-                    finish(t, c0, g, v);
+                    finish(t, c0, g, u);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
+                    for (int j = 0; j < kMx4Chunk; ++j) {
                         mine[(c0 + j) * 128] = g[j];
-                        if (SWIGLU) mine[(NT + c0 + j) * 128] = v[j];
+                        mine[(NT + c0 + j) * 128] = u[j];
                     }
                 }
             }
@@ -505,25 +528,26 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             __threadfence();
             __syncwarp();
             unsigned int prev = 0;
-            if (lane == 0) prev = atomicAdd(&args.tickets[t.index * 4 + q], 1u);
+            if (lane == 0) prev = atomicAdd(&args.tickets[t.index * kMx4EpiWarps + warp - 2], 1u);
             prev = __shfl_sync(0xffffffffu, prev, 0);
             if (prev != static_cast<unsigned int>(c_last - c_first)) continue;
             __threadfence();
-            for (int c0 = 0; c0 < NT; c0 += 16) {
-                float g[16], v[16];
+            for (int c0 = half * kMx4Chunk; c0 < NT; c0 += 2 * kMx4Chunk) {
+                float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) g[j] = v[j] = 0.f;
+                for (int j = 0; j < kMx4Chunk; ++j) g[j] = u[j] = 0.f;
+#pragma unroll 4
                 for (int c = c_first; c <= c_last; ++c) {
                     // c_first holds the tile's first K step
                     const float* p = args.partials +
                                      (static_cast<int64_t>(c) * 2 + (c == c_first ? 1 : 0)) * S::kCols * 128 + i_row;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
+                    for (int j = 0; j < kMx4Chunk; ++j) {
                         g[j] += __ldcg(p + (c0 + j) * 128);
-                        if (SWIGLU) v[j] += __ldcg(p + (NT + c0 + j) * 128);
+                        u[j] += __ldcg(p + (NT + c0 + j) * 128);
                     }
                 }
-                finish(t, c0, g, v);
+                finish(t, c0, g, u);
             }
         }
     }

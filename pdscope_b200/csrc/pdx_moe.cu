@@ -204,9 +204,9 @@ int device_setup(int* sms_out) {
 #undef PDX_DEC_ATTR
 #define PDX_MX4_ATTR(NT)                                                                                           \
     PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,           \
-                                      static_cast<int>(Mx4Shape<NT, true>::kSmem)));                               \
+                                      static_cast<int>(Mx4Shape<NT>::kSmem)));                               \
     PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,          \
-                                      static_cast<int>(Mx4Shape<NT, false>::kSmem)))
+                                      static_cast<int>(Mx4Shape<NT>::kSmem)))
         PDX_MX4_ATTR(16); PDX_MX4_ATTR(32); PDX_MX4_ATTR(64); PDX_MX4_ATTR(112);
 #undef PDX_MX4_ATTR
         g_num_sms[dev] = sms;
@@ -943,9 +943,9 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
     if ((reinterpret_cast<uintptr_t>(w->codes) & 127u) || (reinterpret_cast<uintptr_t>(w->scales) & 15u))
         return fail(PDX_ERR_INVALID, "codes must be 128-byte and scales 16-byte aligned");
     if (w->num_slots > 1 && (w->code_stride < 3 * Hp * Ip / 2 || w->scale_stride < 3 * Hp * Ip / 32 ||
-                             w->code_stride % (Hp / 2) || w->code_stride % (Ip / 2) || w->scale_stride % 16))
-        return fail(PDX_ERR_INVALID, "slot strides must cover one expert and be whole rows");
-    if (w->num_slots > 1 && w->num_slots * (w->code_stride / (std::min(Hp, Ip) / 2)) >= (int64_t(1) << 31))
+                             w->code_stride % kMx4TileBytes || w->scale_stride % 16))
+        return fail(PDX_ERR_INVALID, "slot strides must cover one expert and be whole tiles");
+    if (w->num_slots * (std::max(w->code_stride, 3 * Hp * Ip / 2) / (kMx4BK / 2)) >= (int64_t(1) << 31))
         return fail(PDX_ERR_UNSUPPORTED, "expert slab too large for 32-bit TMA row coordinates");
     return PDX_OK;
 }
@@ -967,7 +967,7 @@ struct Mx4Bufs {
     uint8_t* h;             // [2][rows][Ip] pieces
     uint8_t* sf;            // [tiles][Ip / 128] scale tiles of h
     float* partials;        // [kPlanSMs][2][2 nt][128]
-    unsigned int* tickets;  // gate/up tiles * 4, then down tiles * 4
+    unsigned int* tickets;  // words1 of the gate/up tiles, words2 of the down tiles
     int64_t words1, words2;
 };
 
@@ -981,8 +981,8 @@ Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
     b.h = static_cast<uint8_t*>(c.take(2 * rows * Ip));
     b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * kMx4SfBytes));
     b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * 2 * b.nt * 128 * 4));
-    b.words1 = b.tiles * (Ip / 128) * 4;
-    b.words2 = b.tiles * (Hp / 128) * 4;
+    b.words1 = b.tiles * (Ip / 128) * kMx4EpiWarps;
+    b.words2 = b.tiles * ((Hp + 255) / 256) * kMx4EpiWarps;
     b.tickets = static_cast<unsigned int*>(c.take((b.words1 + b.words2) * 4));
     return b;
 }
@@ -993,12 +993,13 @@ size_t mx4_ffn_ws_bytes(int64_t rows, int64_t E, int64_t H, int64_t I) {
     return c.used;
 }
 
-// Codes as a [rows, cols] matrix of 4-bit values, unpacked to bytes in shared memory; 128 x 128 boxes.
-int encode_mx4_weights(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols) {
+// The slab's code tiles (128 rows of 64 bytes, back to back), one box a tile,
+// unpacked to a byte per code in shared memory.
+int encode_mx4_weights(CUtensorMap* map, const void* base, uint64_t tiles) {
     int st = load_encode();
     if (st) return st;
-    const cuuint64_t dims[2] = {cols, rows};
-    const cuuint64_t strides[1] = {cols / 2};
+    const cuuint64_t dims[2] = {kMx4BK, tiles * 128};
+    const cuuint64_t strides[1] = {kMx4BK / 2};
     const cuuint32_t box[2] = {kMx4BK, 128};
     const cuuint32_t estr[2] = {1, 1};
     CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(base), dims, strides, box,
@@ -1024,14 +1025,16 @@ int encode_mx4_tokens(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 }
 
 template <int NT>
-int launch_mx4_pair(const CUtensorMap& tm_gu, const CUtensorMap& tm_x, const Mx4Args& gu, const CUtensorMap& tm_d,
-                    const CUtensorMap& tm_h, const Mx4Args& down, int64_t tiles, int sms, cudaStream_t stream) {
+int launch_mx4_pair(const CUtensorMap& tm_w, const CUtensorMap& tm_x, const Mx4Args& gu, const CUtensorMap& tm_h,
+                    const Mx4Args& down, int64_t tiles, int sms, cudaStream_t stream) {
     const int64_t most = std::min(sms, kPlanSMs);   // the partial sums are sized for kPlanSMs CTAs
-    const int64_t work1 = tiles * (gu.M / 128) * (gu.K / kMx4BK), work2 = tiles * (down.M / 128) * (down.K / kMx4BK);
+    const int64_t work1 = tiles * (gu.M / 128) * (gu.K / kMx4BK);
+    const int64_t work2 = tiles * ((down.M + 255) / 256) * (down.K / kMx4BK);
+    constexpr size_t smem = Mx4Shape<NT>::kSmem;
     PDX_PDL_TRY(launch_pdl(k_mx4_gemm<NT, true>, dim3(static_cast<unsigned>(std::min(most, work1))), dim3(kMx4Threads),
-                           Mx4Shape<NT, true>::kSmem, stream, tm_gu, tm_x, gu));
+                           smem, stream, tm_w, tm_x, gu));
     PDX_PDL_TRY(launch_pdl(k_mx4_gemm<NT, false>, dim3(static_cast<unsigned>(std::min(most, work2))), dim3(kMx4Threads),
-                           Mx4Shape<NT, false>::kSmem, stream, tm_d, tm_h, down));
+                           smem, stream, tm_w, tm_h, down));
     return PDX_OK;
 }
 
@@ -1044,14 +1047,11 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     int st = device_setup(&sms);
     if (st) return st;
     const int Hp = static_cast<int>(round128(H)), Ip = static_cast<int>(round128(I)), n = static_cast<int>(rows);
-    const int64_t per = static_cast<int64_t>(Hp) * Ip;
-    const int64_t slots = w->num_slots, cs = slots > 1 ? w->code_stride : 0, ss = slots > 1 ? w->scale_stride : 0;
-    const uint8_t* codes = static_cast<const uint8_t*>(w->codes);
-    const uint8_t* scales = static_cast<const uint8_t*>(w->scales);
-    const int64_t gu_rows = cs / (Hp / 2), down_rows = cs / (Ip / 2);   // map rows between slots
-    CUtensorMap tm_gu, tm_x, tm_d, tm_h;
-    if ((st = encode_mx4_weights(&tm_gu, codes, (slots - 1) * gu_rows + 2 * Ip, Hp))) return st;
-    if ((st = encode_mx4_weights(&tm_d, codes + per, (slots - 1) * down_rows + Hp, Ip))) return st;
+    const int per = (Hp / 128) * (Ip / 128);        // weight tiles of a projection
+    const int64_t slots = w->num_slots, ss = slots > 1 ? w->scale_stride : 0;
+    const int64_t tps = slots > 1 ? w->code_stride / kMx4TileBytes : 0;
+    CUtensorMap tm_w, tm_x, tm_h;
+    if ((st = encode_mx4_weights(&tm_w, w->codes, (slots - 1) * tps + 3 * per))) return st;
     if ((st = encode_mx4_tokens(&tm_x, b.x, rows, Hp, b.nt))) return st;
     if ((st = encode_mx4_tokens(&tm_h, b.h, rows, Ip, b.nt))) return st;
     const dim3 split_grid(static_cast<unsigned>(std::min<int64_t>((rows + kMx4SplitWarps - 1) / kMx4SplitWarps,
@@ -1059,15 +1059,16 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     PDX_PDL_TRY(launch_pdl(k_mx4_split, split_grid, dim3(kMx4SplitWarps * 32), 0, stream,
                            static_cast<const uint16_t*>(x), tokens, static_cast<int>(T), n, static_cast<int>(H), Hp,
                            b.x, b.row_scale, b.tickets, static_cast<int>(b.words1 + b.words2)));
-    Mx4Args gu{offsets, active, w->slot_of_expert, slots, scales, scales + per / 32, ss, gu_rows, Ip, Hp, Ip, n,
+    const uint8_t* scales = static_cast<const uint8_t*>(w->scales);
+    Mx4Args gu{offsets, active, w->slot_of_expert, slots, scales, ss, tps, 0, per, Hp, Ip, n, static_cast<int>(E),
                b.row_scale, b.sf, b.h, nullptr, 0, b.partials, b.tickets};
-    Mx4Args down{offsets, active, w->slot_of_expert, slots, scales + per / 16, nullptr, ss, down_rows, 0, Ip, Hp, n,
-                 nullptr, b.sf, nullptr, static_cast<uint16_t*>(y), static_cast<int>(H), b.partials,
-                 b.tickets + b.words1};
-    if (b.nt == 16) return launch_mx4_pair<16>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
-    if (b.nt == 32) return launch_mx4_pair<32>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
-    if (b.nt == 64) return launch_mx4_pair<64>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
-    return launch_mx4_pair<112>(tm_gu, tm_x, gu, tm_d, tm_h, down, b.tiles, sms, stream);
+    Mx4Args down{offsets, active, w->slot_of_expert, slots, scales, ss, tps, 2 * per, 0, Ip, Hp, n,
+                 static_cast<int>(E), nullptr, b.sf, nullptr, static_cast<uint16_t*>(y), static_cast<int>(H),
+                 b.partials, b.tickets + b.words1};
+    if (b.nt == 16) return launch_mx4_pair<16>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
+    if (b.nt == 32) return launch_mx4_pair<32>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
+    if (b.nt == 64) return launch_mx4_pair<64>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
+    return launch_mx4_pair<112>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
 }
 
 // ---- block norms ---------------------------------------------------------------------

@@ -97,8 +97,8 @@ class Mxfp4ExpertSlab:
     and the PDScope runtime take a slab.
 
     ``hidden`` and ``inter`` are multiples of 32; a slot's rows and columns are
-    padded with zeros to multiples of 128, and its scales are stored as the
-    128 x 128 tiles the tensor cores read.  ``slot_of_expert`` (int32 CUDA [E],
+    padded with zeros to multiples of 128, and codes and scales are stored as
+    the 128 x 128 tiles that a product streams (each tile one run of memory).  ``slot_of_expert`` (int32 CUDA [E],
     optional) maps expert ids to slots."""
 
     def __init__(self, num_slots, hidden, inter, device, slot_of_expert=None):
@@ -118,13 +118,13 @@ class Mxfp4ExpertSlab:
                                    code_stride=3 * per // 2, scale_stride=3 * per // BLOCK, num_slots=num_slots,
                                    slot_of_expert=slot_of_expert.data_ptr() if slot_of_expert is not None else None)
 
-    def _views(self, slots, j):
-        """Codes [n, rows, cols/2] and scale tiles [n, row tile, column tile, r % 32, r / 32, c / 32] of projection j."""
+    def _tiles(self, slots, j):
+        """Code tiles [n, row tile, column tile, r, byte] and scale tiles
+        [n, row tile, column tile, r % 32, r / 32, c / 32] of projection j."""
         rows, cols = (self._ip, self._hp) if j < 2 else (self._hp, self._ip)
-        per = self._hp * self._ip
-        codes = self.codes[slots, j * per // 2:(j + 1) * per // 2].view(-1, rows, cols // 2)
-        tiles = self.scales[slots, j * per // BLOCK:(j + 1) * per // BLOCK].view(-1, rows // 128, cols // 128, 32, 4, 4)
-        return codes, tiles
+        grid, per = (-1, rows // 128, cols // 128), self._hp * self._ip
+        return (self.codes[slots, j * per // 2:(j + 1) * per // 2].view(*grid, 128, 64),
+                self.scales[slots, j * per // BLOCK:(j + 1) * per // BLOCK].view(*grid, 32, 4, 4))
 
     def _shape(self, j):
         return (self.inter, self.hidden) if j < 2 else (self.hidden, self.inter)
@@ -137,20 +137,25 @@ class Mxfp4ExpertSlab:
             if q.shape[1:] != self._shape(j) or n != gate.codes.shape[0] or first < 0 or first + n > self.num_slots:
                 raise ValueError(f"{name} does not fit the slab's slots")
             rows, cols = self._shape(j)
-            codes, tiles = self._views(slice(first, first + n), j)
-            codes[:, :rows, :cols // 2] = q.codes
-            s = torch.zeros((n, tiles.shape[1] * 128, tiles.shape[2] * 4), dtype=torch.uint8, device=q.scales.device)
+            codes, scales = self._tiles(slice(first, first + n), j)
+            nr, nc = codes.shape[1:3]
+            c = torch.zeros((n, nr * 128, nc * 64), dtype=torch.uint8, device=q.codes.device)
+            c[:, :rows, :cols // 2] = q.codes
+            codes.copy_(c.view(n, nr, 128, nc, 64).transpose(2, 3))
+            s = torch.zeros((n, nr * 128, nc * 4), dtype=torch.uint8, device=q.scales.device)
             s[:, :rows, :cols // BLOCK] = q.scales
-            tiles.copy_(s.view(n, tiles.shape[1], 4, 32, tiles.shape[2], 4).permute(0, 1, 4, 3, 2, 5))
+            scales.copy_(s.view(n, nr, 4, 32, nc, 4).permute(0, 1, 4, 3, 2, 5))
 
     def load(self, slot):
         """The slot's experts as {gate_proj, up_proj, down_proj} Mxfp4 matrices."""
         out = {}
         for j, name in enumerate(PROJECTIONS):
             rows, cols = self._shape(j)
-            codes, tiles = self._views(slice(slot, slot + 1), j)
-            s = tiles[0].permute(0, 3, 2, 1, 4).reshape(tiles.shape[1] * 128, tiles.shape[2] * 4)
-            out[name] = Mxfp4(codes[0, :rows, :cols // 2].contiguous(), s[:rows, :cols // BLOCK].contiguous())
+            codes, scales = self._tiles(slice(slot, slot + 1), j)
+            nr, nc = codes.shape[1:3]
+            c = codes[0].transpose(1, 2).reshape(nr * 128, nc * 64)
+            s = scales[0].permute(0, 3, 2, 1, 4).reshape(nr * 128, nc * 4)
+            out[name] = Mxfp4(c[:rows, :cols // 2].contiguous(), s[:rows, :cols // BLOCK].contiguous())
         return out
 
     def expert_tensors(self, slot):
