@@ -23,8 +23,9 @@
 // one expert a tile; up to NT = 32 the two pieces are stacked along N (one pass
 // over the weights in shared memory), above that they accumulate into the same
 // columns.
-// Work is cut evenly: the (tile, K step) pairs of the launch form one sequence
-// and CTA c takes an equal share of it, so a decode step of any batch keeps
+// Work is cut evenly: full waves of tiles go round robin (neighbouring CTAs share
+// a token tile in L2), and the (tile, K step) pairs of the rest form one sequence
+// of which every CTA takes an equal share, so a decode step of any batch keeps
 // every SM streaming; a tile that spans CTAs is summed in CTA order by the warp
 // that takes its last ticket (FP32, deterministic, nothing waits).
 // Roles (352 threads): warp 0 streams weights and scales, warp 10 the token
@@ -289,27 +290,47 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     }
     __syncthreads();
     const uint32_t tmem_base = *tmem_slot;
-    // this CTA's share [w0, w1) of the (tile, K step) sequence; at least one step
-    // per sharing CTA, so every CTA between two sharers of a tile shares it too
-    const int64_t work = static_cast<int64_t>(s_misc[0]) * nkb;
-    const int64_t shares = max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), work));
-    const int64_t w0 = blockIdx.x < shares ? work * blockIdx.x / shares : 0;
-    const int64_t w1 = blockIdx.x < shares ? work * (blockIdx.x + 1) / shares : 0;
+    // CTA c takes the whole tiles c, c + G, ... of the full waves of G tiles, and
+    // before them its share [w0, w1) of the (tile, K step) sequence of the rest
+    // (`work` steps), at least one step per sharing CTA, so every CTA between two
+    // sharers of a tile shares it too.
+    const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+    const int waves = s_misc[0] / grid, whole_tiles = waves * grid;
+    const int64_t work = static_cast<int64_t>(s_misc[0] - whole_tiles) * nkb;
+    const int64_t shares = max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), work));
+    const int64_t w0 = cta < shares ? work * cta / shares : 0;
+    const int64_t w1 = cta < shares ? work * (cta + 1) / shares : 0;
 
     struct Tile {
-        int a, mt, nb, kb0, kb1;
-        int64_t index;
+        int index, a, mt, nb, kb0, kb1;
+        int64_t w;    // next step of the share
+        int wave;     // next wave
     };
-    auto decode = [&](int64_t w) {
+    auto begin = [&]() {
         Tile t;
-        t.index = w / nkb;
-        t.kb0 = static_cast<int>(w - t.index * nkb);
-        t.kb1 = static_cast<int>(min(static_cast<int64_t>(nkb), t.kb0 + (w1 - w)));
-        t.a = find_expert(prefix, n_active, static_cast<int>(t.index));
-        const int local = static_cast<int>(t.index) - prefix[t.a];
+        t.w = w0;
+        t.wave = 0;
+        return t;
+    };
+    auto next = [&](Tile& t) {
+        if (t.w < w1) {
+            const int at = static_cast<int>(t.w / nkb);
+            t.index = whole_tiles + at;
+            t.kb0 = static_cast<int>(t.w - static_cast<int64_t>(at) * nkb);
+            t.kb1 = static_cast<int>(min(static_cast<int64_t>(nkb), t.kb0 + (w1 - t.w)));
+            t.w += t.kb1 - t.kb0;
+        } else if (t.wave < waves) {
+            t.index = t.wave++ * grid + cta;
+            t.kb0 = 0;
+            t.kb1 = nkb;
+        } else {
+            return false;
+        }
+        t.a = find_expert(prefix, n_active, t.index);
+        const int local = t.index - prefix[t.a];
         t.nb = local / m_tiles;
         t.mt = local - t.nb * m_tiles;
-        return t;
+        return true;
     };
 
     if (warp == 0) {
@@ -318,9 +339,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int64_t w = w0; w < w1 && ok;) {
-                const Tile t = decode(w);
-                w += t.kb1 - t.kb0;
+            for (Tile t = begin(); ok && next(t);) {
                 const int64_t slot = t_slot[t.a];
                 // weight tiles of both halves; down's odd last block is loaded twice, its second half unused
                 const int b0 = SWIGLU ? args.tile0 + t.mt * nkb : args.tile0 + 2 * t.mt * nkb;
@@ -351,9 +370,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int64_t w = w0; w < w1 && ok;) {
-                const Tile t = decode(w);
-                w += t.kb1 - t.kb0;
+            for (Tile t = begin(); ok && next(t);) {
                 const int row = t_seg0[t.a] + t.nb * NT;
                 const int64_t tt = prefix[t.a] / m_tiles + t.nb;
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
@@ -375,9 +392,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         int stage = 0, lt = 0, step = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int64_t w = w0; w < w1 && ok; ++lt) {
-            const Tile t = decode(w);
-            w += t.kb1 - t.kb0;
+        for (Tile t = begin(); ok && next(t); ++lt) {
             const int b = lt & 1;
             const uint32_t acc_phase = static_cast<uint32_t>(lt >> 1) & 1u;
             if (!mbar_wait(&tmem_empty[b], acc_phase ^ 1u, abort_flag)) { ok = false; break; }
@@ -478,9 +493,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             }
         };
         int lt = 0;
-        for (int64_t w = w0; w < w1; ++lt) {
-            const Tile t = decode(w);
-            w += t.kb1 - t.kb0;
+        for (Tile t = begin(); next(t); ++lt) {
             const int b = lt & 1;
             const uint32_t acc_phase = static_cast<uint32_t>(lt >> 1) & 1u;
             if (!mbar_wait(&tmem_full[b], acc_phase, abort_flag)) break;
@@ -490,7 +503,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             // a share of a tile: the part with the tile's first K step is its CTA's
             // last tile (slot 1), every other part its CTA's first (slot 0)
             float* mine = args.partials +
-                          (static_cast<int64_t>(blockIdx.x) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
+                          (static_cast<int64_t>(cta) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
             for (int c0 = half * kMx4Chunk; c0 < NT; c0 += 2 * kMx4Chunk) {
                 uint32_t r[4][kMx4Chunk];
                 tmem_ld8(taddr + c0, r[0]);
@@ -522,7 +535,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             }
             if (whole) continue;
             // the CTAs that share the tile: step w belongs to CTA floor(((w + 1) shares - 1) / work)
-            const int64_t first = t.index * nkb, last = first + nkb - 1;
+            const int64_t first = static_cast<int64_t>(t.index - whole_tiles) * nkb, last = first + nkb - 1;
             const int c_first = static_cast<int>(((first + 1) * shares - 1) / work);
             const int c_last = static_cast<int>(((last + 1) * shares - 1) / work);
             __threadfence();
