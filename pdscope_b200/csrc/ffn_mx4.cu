@@ -74,56 +74,78 @@ __device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b - f.y), "f"(a - f.x));
 }
 
-// Token rows in packed order as E4M3 pieces, one warp per row: out [2][rows][Hp]
-// (hi rows, then lo rows, zero past H) and the row's factor 2^(byte - 127).
-// CTA 0 clears the tickets of the two products that follow.
-constexpr int kMx4SplitWarps = 4;
-__global__ void __launch_bounds__(kMx4SplitWarps * 32)
+// Token rows in packed order as E4M3 pieces: out [2][rows][Hp] (hi rows, then lo
+// rows, zero past H) and the row's factor 2^(b - 127).  HBM-bound (the pieces
+// are written once, x comes from L2).  A group of WARPS warps takes a row, eight
+// values a lane at a time; up to kMx4SplitHeld of those stay in registers
+// between finding the row's largest value and splitting, longer rows are read
+// again.  One warp a row for many rows, four for few, where the trip to memory
+// is what a row costs.  CTA 0 clears the tickets of the two products that follow.
+constexpr int kMx4SplitWarps = 4;     // warps per CTA
+constexpr int kMx4SplitHeld = 8;
+template <int WARPS>
+__global__ void __launch_bounds__(kMx4SplitWarps * 32, 8)
     k_mx4_split(const uint16_t* __restrict__ x, const int32_t* __restrict__ tokens, int T, int rows, int H, int Hp,
                 uint8_t* __restrict__ out, float* __restrict__ row_scale, unsigned int* __restrict__ zero_ptr,
                 int zero_words) {
     griddep_wait();
     griddep_launch();
+    __shared__ uint32_t s_top[kMx4SplitWarps];
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < zero_words; i += blockDim.x) zero_ptr[i] = 0u;
-    const int lane = static_cast<int>(lane_id());
-    for (int p = static_cast<int>(blockIdx.x) * kMx4SplitWarps + static_cast<int>(threadIdx.x >> 5); p < rows;
-         p += static_cast<int>(gridDim.x) * kMx4SplitWarps) {
-        int t = tokens ? tokens[p] : p;
+    constexpr int kGroups = kMx4SplitWarps / WARPS, kLanes = 32 * WARPS;
+    const int group = static_cast<int>(threadIdx.x) / kLanes, lane = static_cast<int>(threadIdx.x) % kLanes;
+    const int chunks = H / 8, chunks_p = Hp / 8;
+    // WARPS > 1: one group per CTA, so the loop below is uniform over the CTA
+    static_assert(WARPS == 1 || kGroups == 1, "the barriers need whole CTAs");
+    for (int p = static_cast<int>(blockIdx.x) * kGroups + group; p < rows; p += static_cast<int>(gridDim.x) * kGroups) {
+        int t = tokens ? __ldg(tokens + p) : p;
         if (t < 0 || t >= T) {
             raise_error(PDX_DEVERR_BAD_EXPERT);
             t = 0;
         }
         const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t) * H);
+        uint4 held[kMx4SplitHeld];
         uint32_t top = 0;
-        for (int c = lane; c < H / 8; c += 32) {
-            const uint4 v = __ldg(src + c);
+        auto widen = [&](const uint4& v) {
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
-        }
-        const uint32_t byte = mx4_group_byte(__reduce_max_sync(0xffffffffu, top));
-        const float inv = mx4_inverse(byte);
-        uint8_t* hi_row = out + static_cast<int64_t>(p) * Hp;
-        uint8_t* lo_row = out + (static_cast<int64_t>(rows) + p) * Hp;
-        for (int c = lane; c < Hp / 16; c += 32) {
-            uint32_t hw[4] = {0, 0, 0, 0}, lw[4] = {0, 0, 0, 0};
-            if (c * 16 < H) {
-                float v[16];
-                load8<bf16, true>(reinterpret_cast<const bf16*>(src) + c * 16, v);
-                load8<bf16, true>(reinterpret_cast<const bf16*>(src) + c * 16 + 8, v + 8);
+        };
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint16_t h0, l0, h1, l1;
-                    e4m3_split2(v[4 * i] * inv, v[4 * i + 1] * inv, h0, l0);
-                    e4m3_split2(v[4 * i + 2] * inv, v[4 * i + 3] * inv, h1, l1);
-                    hw[i] = h0 | (static_cast<uint32_t>(h1) << 16);
-                    lw[i] = l0 | (static_cast<uint32_t>(l1) << 16);
-                }
-            }
-            reinterpret_cast<uint4*>(hi_row)[c] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-            reinterpret_cast<uint4*>(lo_row)[c] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+        for (int j = 0; j < kMx4SplitHeld; ++j) {
+            const int c = j * kLanes + lane;
+            held[j] = c < chunks ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
         }
+#pragma unroll
+        for (int j = 0; j < kMx4SplitHeld; ++j) widen(held[j]);
+        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks; c += kLanes) widen(__ldg(src + c));
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (WARPS > 1) {
+            __syncthreads();   // s_top free from the previous row
+            if (lane_id() == 0) s_top[threadIdx.x >> 5] = top;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) top = max(top, s_top[i]);
+        }
+        const uint32_t byte = mx4_group_byte(top);
+        const float inv = mx4_inverse(byte);
+        uint2* hi_row = reinterpret_cast<uint2*>(out + static_cast<int64_t>(p) * Hp);
+        uint2* lo_row = reinterpret_cast<uint2*>(out + (static_cast<int64_t>(rows) + p) * Hp);
+        auto split = [&](const uint4& v, int c) {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint16_t h[4], l[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                e4m3_split2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xFFFF0000u) * inv, h[i], l[i]);
+            hi_row[c] = make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+            lo_row[c] = make_uint2(l[0] | (static_cast<uint32_t>(l[1]) << 16), l[2] | (static_cast<uint32_t>(l[3]) << 16));
+        };
+#pragma unroll
+        for (int j = 0; j < kMx4SplitHeld; ++j)
+            if (j * kLanes + lane < chunks_p) split(held[j], j * kLanes + lane);
+        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks_p; c += kLanes)
+            split(c < chunks ? __ldg(src + c) : make_uint4(0, 0, 0, 0), c);
         if (lane == 0) row_scale[p] = mx_scale(byte);
     }
 }

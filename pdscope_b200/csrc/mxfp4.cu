@@ -94,25 +94,42 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
     }
 }
 
-// Four lanes per block, eight values each.  rows x cols values with row
-// stride ld (elements); codes and scales dense.
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kMxThreads) k_mx4_quantize(const T* __restrict__ x, int64_t rows, int64_t cols,
+// Both kernels are copies with a conversion: HBM-bound.  A thread takes
+// kMxUnroll pieces of eight values, a CTA's threads neighbouring pieces, and
+// issues all its loads before converting.  FLAT: rows without gaps, so a piece's
+// place needs no division by the row length.
+constexpr int kMxUnroll = 4;
+
+template <bool FLAT>
+__device__ __forceinline__ int64_t mx_at(int64_t c, int64_t per_row, int64_t ld) {
+    if (FLAT) return c * 8;
+    const int64_t row = c / per_row;
+    return row * ld + (c - row * per_row) * 8;
+}
+
+// Four lanes per block, eight values each.  rows x cols values with row stride
+// ld (elements), cols / 8 = per_row; codes and scales dense.  chunks is a
+// multiple of 4, so the four lanes of a block are in range together.
+template <typename T, bool ALIGNED, bool FLAT>
+__global__ void __launch_bounds__(kMxThreads) k_mx4_quantize(const T* __restrict__ x, int64_t chunks, int64_t per_row,
                                                              int64_t ld, uint32_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
     griddep_wait();
     griddep_launch();
-    const int64_t per_row = cols / 8;
-    const int64_t chunks = rows * per_row;   // a multiple of 4
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kMxThreads;
-    for (int64_t c = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x; c < chunks; c += step) {
-        const int64_t row = c / per_row;
-        float v[8];
-        load8<T, ALIGNED>(x + row * ld + (c - row * per_row) * 8, v);
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * (kMxThreads * kMxUnroll) + threadIdx.x;
+    float v[kMxUnroll][8];
+#pragma unroll
+    for (int j = 0; j < kMxUnroll; ++j) {
+        const int64_t c = c0 + j * kMxThreads;
+        if (c < chunks) load8<T, ALIGNED>(x + mx_at<FLAT>(c, per_row, ld), v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kMxUnroll; ++j) {
+        const int64_t c = c0 + j * kMxThreads;
+        if (c >= chunks) return;
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        // the four lanes of a block are in the loop together: chunks % 4 == 0
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
         const uint32_t mask = 0xFu << (lane_id() & 28u);
         m = max(m, __shfl_xor_sync(mask, m, 1));
         m = max(m, __shfl_xor_sync(mask, m, 2));
@@ -120,29 +137,38 @@ __global__ void __launch_bounds__(kMxThreads) k_mx4_quantize(const T* __restrict
         const uint32_t b = exp == 255u ? 255u : (exp > 2u ? exp - 2u : 0u);
         const float inv = __uint_as_float((254u - min(b, 254u)) << 23);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= inv;
-        codes[c] = b == 255u ? 0u : e2m1x8(v);
+        for (int i = 0; i < 8; ++i) v[j][i] *= inv;
+        codes[c] = b == 255u ? 0u : e2m1x8(v[j]);
         if ((c & 3) == 0) scales[c >> 2] = static_cast<uint8_t>(b);
     }
 }
 
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, bool FLAT>
 __global__ void __launch_bounds__(kMxThreads) k_mx4_dequantize(const uint32_t* __restrict__ codes,
-                                                               const uint8_t* __restrict__ scales, int64_t rows,
-                                                               int64_t cols, int64_t ld, T* __restrict__ out) {
+                                                               const uint8_t* __restrict__ scales, int64_t chunks,
+                                                               int64_t per_row, int64_t ld, T* __restrict__ out) {
     griddep_wait();
     griddep_launch();
-    const int64_t per_row = cols / 8;
-    const int64_t chunks = rows * per_row;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kMxThreads;
-    for (int64_t c = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x; c < chunks; c += step) {
-        const int64_t row = c / per_row;
-        const float s = mx_scale(scales[c >> 2]);
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * (kMxThreads * kMxUnroll) + threadIdx.x;
+    uint32_t code[kMxUnroll], scale[kMxUnroll];
+#pragma unroll
+    for (int j = 0; j < kMxUnroll; ++j) {
+        const int64_t c = c0 + j * kMxThreads;
+        if (c < chunks) {
+            code[j] = __ldg(codes + c);
+            scale[j] = __ldg(scales + (c >> 2));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kMxUnroll; ++j) {
+        const int64_t c = c0 + j * kMxThreads;
+        if (c >= chunks) return;
+        const float s = mx_scale(scale[j]);
         float v[8];
-        e2m1x8_to_float(codes[c], v);
+        e2m1x8_to_float(code[j], v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= s;
-        store8<T, ALIGNED>(out + row * ld + (c - row * per_row) * 8, v);
+        store8<T, ALIGNED>(out + mx_at<FLAT>(c, per_row, ld), v);
     }
 }
 

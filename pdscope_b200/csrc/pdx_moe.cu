@@ -906,7 +906,8 @@ int check_mx4_matrix(int64_t rows, int64_t cols, int64_t ld, int32_t dtype) {
         return fail(PDX_ERR_INVALID, "MXFP4 needs rows of a positive multiple of 32 values (got %lld)",
                     static_cast<long long>(cols));
     if (ld < cols) return fail(PDX_ERR_INVALID, "row stride %lld shorter than a row", static_cast<long long>(ld));
-    if (rows > (int64_t(1) << 40) / cols) return fail(PDX_ERR_UNSUPPORTED, "matrix too large");
+    if (rows > (int64_t(1) << 40) / cols || ld > (int64_t(1) << 40) / std::max<int64_t>(rows, 1))
+        return fail(PDX_ERR_UNSUPPORTED, "matrix too large");
     return PDX_OK;
 }
 
@@ -916,15 +917,18 @@ bool mx4_aligned(const void* p, int64_t ld, int32_t dtype) {
 }
 
 template <typename F>
-cudaError_t with_mx4_type(int32_t dtype, bool aligned, F f) {
-    auto with_type = [&](auto type) { return aligned ? f(type, std::true_type{}) : f(type, std::false_type{}); };
+cudaError_t with_mx4_type(int32_t dtype, bool aligned, bool flat, F f) {
+    auto with_type = [&](auto type) {
+        if (flat) return aligned ? f(type, std::true_type{}, std::true_type{}) : f(type, std::false_type{}, std::true_type{});
+        return aligned ? f(type, std::true_type{}, std::false_type{}) : f(type, std::false_type{}, std::false_type{});
+    };
     if (dtype == PDX_DTYPE_BF16) return with_type(bf16{});
     if (dtype == PDX_DTYPE_FP16) return with_type(__half{});
     return with_type(float{});
 }
 
 dim3 mx4_grid(int64_t chunks) {
-    return dim3(static_cast<unsigned>(std::min<int64_t>((chunks + kMxThreads - 1) / kMxThreads, 16 * kPlanSMs)));
+    return dim3(static_cast<unsigned>((chunks + kMxThreads * kMxUnroll - 1) / (kMxThreads * kMxUnroll)));
 }
 
 int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool gathered,
@@ -958,6 +962,9 @@ int mx4_tile(int64_t rows, int64_t E) {
     const int64_t avg = (rows + est - 1) / est;
     return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 48 ? 64 : 112));
 }
+
+// Rows up to which the split takes four warps a row (all rows in flight at once).
+constexpr int64_t kMx4SplitFew = 4 * kPlanSMs;
 
 struct Mx4Bufs {
     int nt;
@@ -1054,11 +1061,13 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     if ((st = encode_mx4_weights(&tm_w, w->codes, (slots - 1) * tps + 3 * per))) return st;
     if ((st = encode_mx4_tokens(&tm_x, b.x, rows, Hp, b.nt))) return st;
     if ((st = encode_mx4_tokens(&tm_h, b.h, rows, Ip, b.nt))) return st;
-    const dim3 split_grid(static_cast<unsigned>(std::min<int64_t>((rows + kMx4SplitWarps - 1) / kMx4SplitWarps,
-                                                                  16 * kPlanSMs)));
-    PDX_PDL_TRY(launch_pdl(k_mx4_split, split_grid, dim3(kMx4SplitWarps * 32), 0, stream,
-                           static_cast<const uint16_t*>(x), tokens, static_cast<int>(T), n, static_cast<int>(H), Hp,
-                           b.x, b.row_scale, b.tickets, static_cast<int>(b.words1 + b.words2)));
+    const bool few = rows <= kMx4SplitFew;
+    const int64_t split_ctas = few ? rows : (rows + kMx4SplitWarps - 1) / kMx4SplitWarps;
+    PDX_PDL_TRY(launch_pdl(few ? k_mx4_split<kMx4SplitWarps> : k_mx4_split<1>,
+                           dim3(static_cast<unsigned>(std::min<int64_t>(split_ctas, 16 * kPlanSMs))),
+                           dim3(kMx4SplitWarps * 32), 0, stream, static_cast<const uint16_t*>(x), tokens,
+                           static_cast<int>(T), n, static_cast<int>(H), Hp, b.x, b.row_scale, b.tickets,
+                           static_cast<int>(b.words1 + b.words2)));
     const uint8_t* scales = static_cast<const uint8_t*>(w->scales);
     Mx4Args gu{offsets, active, w->slot_of_expert, slots, scales, ss, tps, 0, per, Hp, Ip, n, static_cast<int>(E),
                b.row_scale, b.sf, b.h, nullptr, 0, b.partials, b.tickets};
@@ -1106,18 +1115,6 @@ BlockNormArgs to_block_norm(const pdx_block_norm_args* p, const void* residual, 
     return a;
 }
 
-template <typename RES, bool COMBINE>
-cudaError_t launch_block_norm_typed(const BlockNormArgs& a, int64_t T, bool vec, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(T)), block(kBnThreads);
-    if (vec) {
-        if (a.H <= 8 * kBnThreads) return launch_pdl(k_block_norm<RES, COMBINE, 8, 1>, grid, block, 0, stream, a);
-        if (a.H <= 16 * kBnThreads) return launch_pdl(k_block_norm<RES, COMBINE, 8, 2>, grid, block, 0, stream, a);
-        return launch_pdl(k_block_norm<RES, COMBINE, 8, 4>, grid, block, 0, stream, a);
-    }
-    if (a.H <= 4 * kBnThreads) return launch_pdl(k_block_norm<RES, COMBINE, 1, 4>, grid, block, 0, stream, a);
-    return launch_pdl(k_block_norm<RES, COMBINE, 1, kBnMaxH / kBnThreads>, grid, block, 0, stream, a);
-}
-
 template <bool COMBINE>
 int launch_block_norm(const BlockNormArgs& a, int64_t T, bool fp32, cudaStream_t stream) {
     // 16-byte accesses: whole vectors per row and every row pointer aligned
@@ -1126,8 +1123,20 @@ int launch_block_norm(const BlockNormArgs& a, int64_t T, bool fp32, cudaStream_t
                      reinterpret_cast<uintptr_t>(a.stream) | reinterpret_cast<uintptr_t>(a.normed);
     if (a.gate && a.gate_col == 1) bits |= reinterpret_cast<uintptr_t>(a.gate) | static_cast<uintptr_t>(a.gate_row * 2);
     const bool vec = a.H % 8 == 0 && (bits & 15u) == 0;
-    PDX_PDL_TRY((fp32 ? launch_block_norm_typed<float, COMBINE>(a, T, vec, stream)
-                      : launch_block_norm_typed<uint16_t, COMBINE>(a, T, vec, stream)));
+    const dim3 grid(static_cast<unsigned>(T)), block(static_cast<unsigned>((a.H + 255) / 256 * 32));
+    const bool early = T <= 4 * kPlanSMs;   // every row resident at once
+    auto launch = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, stream, a); };
+    auto launch_as = [&](auto res) {
+        using RES = decltype(res);
+        if (!vec) return launch(k_block_norm<RES, COMBINE, false, 1024, true>);
+        if (a.H > 4096) return launch(k_block_norm<RES, COMBINE, true, 1024, true>);
+        if (a.H > 2048)
+            return early ? launch(k_block_norm<RES, COMBINE, true, 512, true>)
+                         : launch(k_block_norm<RES, COMBINE, true, 512, false>);
+        return early ? launch(k_block_norm<RES, COMBINE, true, 256, true>)
+                     : launch(k_block_norm<RES, COMBINE, true, 256, false>);
+    };
+    PDX_PDL_TRY(fp32 ? launch_as(float{}) : launch_as(uint16_t{}));
     return PDX_OK;
 }
 
@@ -1502,11 +1511,12 @@ int pdx_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols,
     if (rows == 0) return ok();
     if (!x || !codes || !scales) return fail(PDX_ERR_INVALID, "null quantisation argument");
     if (reinterpret_cast<uintptr_t>(codes) & 3u) return fail(PDX_ERR_INVALID, "codes must be 4-byte aligned");
-    PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(x, ld, dtype), [&](auto type, auto aligned) {
+    const int64_t chunks = rows * cols / 8;
+    PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(x, ld, dtype), ld == cols, [&](auto type, auto aligned, auto flat) {
         using T = decltype(type);
-        return launch_pdl(k_mx4_quantize<T, decltype(aligned)::value>, mx4_grid(rows * cols / 8), dim3(kMxThreads), 0,
-                          stream, static_cast<const T*>(x), rows, cols, ld, static_cast<uint32_t*>(codes),
-                          static_cast<uint8_t*>(scales));
+        return launch_pdl(k_mx4_quantize<T, decltype(aligned)::value, decltype(flat)::value>, mx4_grid(chunks),
+                          dim3(kMxThreads), 0, stream, static_cast<const T*>(x), chunks, cols / 8, ld,
+                          static_cast<uint32_t*>(codes), static_cast<uint8_t*>(scales));
     }));
     return ok();
 }
@@ -1518,11 +1528,12 @@ int pdx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, in
     if (rows == 0) return ok();
     if (!out || !codes || !scales) return fail(PDX_ERR_INVALID, "null quantisation argument");
     if (reinterpret_cast<uintptr_t>(codes) & 3u) return fail(PDX_ERR_INVALID, "codes must be 4-byte aligned");
-    PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(out, ld, dtype), [&](auto type, auto aligned) {
+    const int64_t chunks = rows * cols / 8;
+    PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(out, ld, dtype), ld == cols, [&](auto type, auto aligned, auto flat) {
         using T = decltype(type);
-        return launch_pdl(k_mx4_dequantize<T, decltype(aligned)::value>, mx4_grid(rows * cols / 8), dim3(kMxThreads),
-                          0, stream, static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(scales), rows,
-                          cols, ld, static_cast<T*>(out));
+        return launch_pdl(k_mx4_dequantize<T, decltype(aligned)::value, decltype(flat)::value>, mx4_grid(chunks),
+                          dim3(kMxThreads), 0, stream, static_cast<const uint32_t*>(codes),
+                          static_cast<const uint8_t*>(scales), chunks, cols / 8, ld, static_cast<T*>(out));
     }));
     return ok();
 }
