@@ -51,126 +51,131 @@ __device__ __forceinline__ float bn_block_sum(float v, float* red, int& turn) {
     return v;
 }
 
-// A thread's eight values of a row of H: VEC, the aligned eight from 8 * tid;
-// else every blockDim-th value from tid (any H and alignment).  Values past H
-// read as 0 and are not written.
-template <bool VEC>
+// A thread's 8 CH values of a row of H: VEC, the aligned eight from 8 (tid + c
+// blockDim) for every c < CH; else every blockDim-th value from tid (any H and
+// alignment).  Values past H read as 0 and are not written.
+template <bool VEC, int CH>
 struct BnPlace {
-    int H, first, step;
-    __device__ explicit BnPlace(int h)
-        : H(h), first(static_cast<int>(threadIdx.x) * (VEC ? 8 : 1)), step(VEC ? 1 : static_cast<int>(blockDim.x)) {}
-    __device__ __forceinline__ int col(int i) const { return first + i * step; }
-    __device__ __forceinline__ bool in(int i) const { return VEC ? first < H : col(i) < H; }
+    static constexpr int N = 8 * CH;
+    int H;
+    __device__ explicit BnPlace(int h) : H(h) {}
+    __device__ __forceinline__ int col(int i) const {
+        return VEC ? (static_cast<int>(threadIdx.x) + i / 8 * static_cast<int>(blockDim.x)) * 8 + i % 8
+                   : static_cast<int>(threadIdx.x) + i * static_cast<int>(blockDim.x);
+    }
+    __device__ __forceinline__ bool in(int i) const { return col(VEC ? i & ~7 : i) < H; }
+    __device__ __forceinline__ void clear(float (&v)[N]) const {   // values past H to 0
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!in(i)) v[i] = 0.f;
+    }
 };
 
 // Raw values, loaded early and converted where they are used.
-template <bool VEC, typename T>
-struct BnRaw;
-template <>
-struct BnRaw<true, uint16_t> {
-    uint4 q;
-    __device__ __forceinline__ void load(const BnPlace<true>& at, const uint16_t* p) {
-        q = make_uint4(0, 0, 0, 0);
-        if (at.in(0)) q = *reinterpret_cast<const uint4*>(p + at.first);
-    }
-    __device__ __forceinline__ float get(int i) const {
-        const uint32_t w = i < 2 ? q.x : (i < 4 ? q.y : (i < 6 ? q.z : q.w));
-        return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
-    }
-};
-template <>
-struct BnRaw<true, float> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const BnPlace<true>& at, const float* p) {
-        a = b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at.in(0)) {
-            a = reinterpret_cast<const float4*>(p + at.first)[0];
-            b = reinterpret_cast<const float4*>(p + at.first)[1];
+template <bool VEC, int CH, typename T>
+struct BnRaw {
+    static constexpr int kVecs = static_cast<int>(sizeof(T)) / 2;   // 16-byte pieces of eight values
+    uint4 q[VEC ? CH * kVecs : 1];
+    T one[VEC ? 1 : 8 * CH];
+    __device__ __forceinline__ void load(const BnPlace<VEC, CH>& at, const T* p) {
+        if (VEC) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int j = 0; j < kVecs; ++j)
+                    q[c * kVecs + j] = at.in(8 * c) ? reinterpret_cast<const uint4*>(p + at.col(8 * c))[j]
+                                                    : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8 * CH; ++i) one[i] = at.in(i) ? p[at.col(i)] : static_cast<T>(0);
         }
     }
     __device__ __forceinline__ float get(int i) const {
-        const float4& v = i < 4 ? a : b;
-        return (i & 3) == 0 ? v.x : ((i & 3) == 1 ? v.y : ((i & 3) == 2 ? v.z : v.w));
+        if (!VEC) return sizeof(T) == 4 ? static_cast<float>(one[i]) : bits2f(static_cast<uint16_t>(one[i]));
+        const int word = sizeof(T) == 4 ? i : i / 2;
+        const uint4& v = q[word / 4];
+        const uint32_t w = word % 4 == 0 ? v.x : (word % 4 == 1 ? v.y : (word % 4 == 2 ? v.z : v.w));
+        if (sizeof(T) == 4) return __uint_as_float(w);
+        return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
     }
-};
-template <>
-struct BnRaw<false, uint16_t> {
-    uint16_t v[8];
-    __device__ __forceinline__ void load(const BnPlace<false>& at, const uint16_t* p) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = at.in(i) ? p[at.col(i)] : static_cast<uint16_t>(0);
-    }
-    __device__ __forceinline__ float get(int i) const { return bits2f(v[i]); }
-};
-template <>
-struct BnRaw<false, float> {
-    float v[8];
-    __device__ __forceinline__ void load(const BnPlace<false>& at, const float* p) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = at.in(i) ? p[at.col(i)] : 0.f;
-    }
-    __device__ __forceinline__ float get(int i) const { return v[i]; }
 };
 
-template <bool VEC>
-__device__ __forceinline__ void bn_store(const BnPlace<VEC>& at, uint16_t* p, const float* v) {
+template <bool VEC, int CH>
+__device__ __forceinline__ void bn_store(const BnPlace<VEC, CH>& at, uint16_t* p, const float* v) {
     if (VEC) {
-        if (!at.in(0)) return;
-        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = static_cast<uint32_t>(f2bits(v[2 * i])) | (static_cast<uint32_t>(f2bits(v[2 * i + 1])) << 16);
-        *reinterpret_cast<uint4*>(p + at.first) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int c = 0; c < CH; ++c) {
+            if (!at.in(8 * c)) continue;
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(v[8 * c + 2 * i], v[8 * c + 2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&two);
+            }
+            *reinterpret_cast<uint4*>(p + at.col(8 * c)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8 * CH; ++i)
             if (at.in(i)) p[at.col(i)] = f2bits(v[i]);
     }
 }
-template <bool VEC>
-__device__ __forceinline__ void bn_store(const BnPlace<VEC>& at, float* p, const float* v) {
+template <bool VEC, int CH>
+__device__ __forceinline__ void bn_store(const BnPlace<VEC, CH>& at, float* p, const float* v) {
     if (VEC) {
-        if (!at.in(0)) return;
-        reinterpret_cast<float4*>(p + at.first)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p + at.first)[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (!at.in(8 * c)) continue;
+            float4* to = reinterpret_cast<float4*>(p + at.col(8 * c));
+            to[0] = make_float4(v[8 * c], v[8 * c + 1], v[8 * c + 2], v[8 * c + 3]);
+            to[1] = make_float4(v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8 * CH; ++i)
             if (at.in(i)) p[at.col(i)] = v[i];
     }
 }
 
 // Normalise the row held in v (values past H are 0 and stay so).
-template <bool VEC>
-__device__ __forceinline__ void bn_norm(float (&v)[8], int how, bool weighted, const BnRaw<VEC, uint16_t>& w,
-                                        const BnPlace<VEC>& at, float eps, float* red, int& turn) {
+template <bool VEC, int CH>
+__device__ __forceinline__ void bn_norm(float (&v)[8 * CH], int how, bool weighted, const BnRaw<VEC, CH, uint16_t>& w,
+                                        const BnPlace<VEC, CH>& at, float eps, float* red, int& turn) {
+    constexpr int N = 8 * CH;
     if (how == PDX_NORM_NONE) return;
     const float inv_h = 1.0f / static_cast<float>(at.H);
     if (how == PDX_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += v[i];
+        for (int i = 0; i < N; ++i) s += v[i];
         const float mean = bn_block_sum(s, red, turn) * inv_h;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (at.in(i)) v[i] -= mean;
+        for (int i = 0; i < N; ++i) v[i] -= mean;
+        at.clear(v);
     }
     float q = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q += v[i] * v[i];
+    for (int i = 0; i < N; ++i) q += v[i] * v[i];
     const float inv = rsqrtf(bn_block_sum(q, red, turn) * inv_h + eps);
+    if (weighted) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= weighted ? inv * w.get(i) : inv;
+        for (int i = 0; i < N; ++i) v[i] *= inv * w.get(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= inv;
+    }
 }
 
-// One CTA per row, eight values a thread, at most MAXT threads.  EARLY (few rows,
+// One CTA per row, 8 CH values a thread, at most MAXT threads.  EARLY (few rows,
 // where the latency of a row counts): every load that does not depend on a
 // reduction is issued before the first one, so a row costs one trip to memory
 // and up to four block reductions.  Otherwise rows hide each other's latency and
-// what counts is how many fit an SM: the weights (and beside expert rows the gate)
-// are loaded where they are used, at no more than 42 registers (48 warps an SM).
-template <typename RES, bool COMBINE, bool VEC, int MAXT, bool EARLY>
-__global__ void __launch_bounds__(MAXT, EARLY || MAXT == 1024 ? 1 : 1536 / MAXT) k_block_norm(BlockNormArgs a) {
+// issue slots count (a reduction and the set-up cost a warp as much as the
+// arithmetic of 8 values a lane, hence CH = 2), and how many rows fit an SM: the
+// weights (and beside expert rows the gate) are loaded where they are used.
+template <typename RES, bool COMBINE, bool VEC, int CH, int MAXT, bool EARLY>
+__global__ void __launch_bounds__(MAXT, EARLY || MAXT == 1024 ? 1 : 1024 / MAXT) k_block_norm(BlockNormArgs a) {
+    constexpr int N = 8 * CH;
     // expert rows loaded together; any-alignment rows take a register per value
     constexpr int kBatch = !VEC ? 2 : (EARLY && MAXT < 1024 ? 8 : 4);
     griddep_wait();
@@ -180,26 +185,21 @@ __global__ void __launch_bounds__(MAXT, EARLY || MAXT == 1024 ? 1 : 1536 / MAXT)
     __shared__ float s_w[32];
     const int64_t t = blockIdx.x;
     const int H = a.H;
-    const BnPlace<VEC> at(H);
+    const BnPlace<VEC, CH> at(H);
     int turn = 0;
-    BnRaw<VEC, RES> res;
-    BnRaw<VEC, uint16_t> yr, gate, post_w, pre_w;
+    BnRaw<VEC, CH, RES> res;
+    BnRaw<VEC, CH, uint16_t> yr, gate, post_w, pre_w;
     res.load(at, static_cast<const RES*>(a.residual) + t * H);
     if (!COMBINE && a.y) yr.load(at, a.y + t * H);
-    float gate_one = 1.f;
     const bool gate_rowwise = a.gate && a.gate_col == 1;
-    auto load_gate = [&]() {
-        if (gate_rowwise)
-            gate.load(at, a.gate + t * a.gate_row);
-        else if (a.gate && a.gate_col == 0)
-            gate_one = bits2f(a.gate[t * a.gate_row]);
-    };
-    if (EARLY || !COMBINE) load_gate();
+    if ((EARLY || !COMBINE) && gate_rowwise) gate.load(at, a.gate + t * a.gate_row);
     if (EARLY) {
         if (a.post_weight) post_w.load(at, a.post_weight);
         if (VEC && a.pre_weight) pre_w.load(at, a.pre_weight);
     }
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
     if (COMBINE) {
         if (threadIdx.x < static_cast<unsigned>(a.k)) {
             int row = a.inverse[t * a.k + threadIdx.x];
@@ -214,39 +214,51 @@ __global__ void __launch_bounds__(MAXT, EARLY || MAXT == 1024 ? 1 : 1536 / MAXT)
         __syncthreads();
         // FP32 sum in slot order
         for (int s0 = 0; s0 < a.k; s0 += kBatch) {
-            BnRaw<VEC, uint16_t> r[kBatch];
+            BnRaw<VEC, CH, uint16_t> r[kBatch];
 #pragma unroll
             for (int j = 0; j < kBatch; ++j)
                 if (s0 + j < a.k && s_row[s0 + j] >= 0) r[j].load(at, a.y + static_cast<int64_t>(s_row[s0 + j]) * H);
 #pragma unroll
             for (int j = 0; j < kBatch; ++j)
-                if (s0 + j < a.k && s_row[s0 + j] >= 0)
+                if (s0 + j < a.k && s_row[s0 + j] >= 0) {
+                    const float w = s_w[s0 + j];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] += r[j].get(i) * s_w[s0 + j];
+                    for (int i = 0; i < N; ++i) v[i] += r[j].get(i) * w;
+                }
         }
     } else if (a.y) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = yr.get(i);
+        for (int i = 0; i < N; ++i) v[i] = yr.get(i);
     }
-    if (!EARLY && a.post_weight) post_w.load(at, a.post_weight);
-    if (COMBINE || a.y) bn_norm<VEC>(v, a.post, a.post_weight != nullptr, post_w, at, a.eps, red, turn);
-    if (!EARLY && COMBINE) load_gate();
+    if (COMBINE || a.y) {
+        if (!EARLY && a.post_weight) post_w.load(at, a.post_weight);
+        bn_norm<VEC, CH>(v, a.post, a.post_weight != nullptr, post_w, at, a.eps, red, turn);
+    }
+    if (a.gate) {
+        float g[N];
+        if (gate_rowwise) {
+            if (!EARLY && COMBINE) gate.load(at, a.gate + t * a.gate_row);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float g = gate_one;
-        if (gate_rowwise)
-            g = gate.get(i);
-        else if (a.gate && a.gate_col > 1 && at.in(i))
-            g = bits2f(a.gate[t * a.gate_row + at.col(i) * a.gate_col]);
-        if (a.gate && a.gate_sigmoid) g = __fdividef(1.0f, 1.0f + expf(-g));   // approximate reciprocal: 1 ulp
-        v[i] = a.residual_scale * res.get(i) + a.block_scale * (a.gate ? g * v[i] : v[i]);
-        if (!at.in(i)) v[i] = 0.f;
+            for (int i = 0; i < N; ++i) g[i] = gate.get(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = at.in(i) ? bits2f(a.gate[t * a.gate_row + at.col(i) * a.gate_col]) : 0.f;
+        }
+        if (a.gate_sigmoid) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = __fdividef(1.0f, 1.0f + expf(-g[i]));   // 1 ulp reciprocal
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= g[i];
     }
-    if (a.stream) bn_store<VEC>(at, static_cast<RES*>(a.stream) + t * H, v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = a.residual_scale * res.get(i) + a.block_scale * v[i];
+    at.clear(v);
+    if (a.stream) bn_store(at, static_cast<RES*>(a.stream) + t * H, v);
     if (!a.normed) return;
     if (!(EARLY && VEC) && a.pre_weight) pre_w.load(at, a.pre_weight);
-    bn_norm<VEC>(v, a.pre, a.pre_weight != nullptr, pre_w, at, a.eps, red, turn);
-    bn_store<VEC>(at, a.normed + t * H, v);
+    bn_norm<VEC, CH>(v, a.pre, a.pre_weight != nullptr, pre_w, at, a.eps, red, turn);
+    bn_store(at, a.normed + t * H, v);
 }
 
 }  // namespace pdx
