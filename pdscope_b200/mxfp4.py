@@ -10,13 +10,14 @@ bytes, which is what a decode step streams.
 """
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
 from ._lib import Mxfp4Weights, check, lib
-from .runtime import (PROJECTIONS, Packed, _ptr, _require_cuda_bf16, _stream, ffn_workspace_bytes, grouped_ffn)
+from .runtime import PROJECTIONS, Packed, _on, _raw_stream, _require_cuda_bf16, ffn_workspace_bytes
 
 BLOCK = 32
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
@@ -48,28 +49,29 @@ def quantize_mxfp4(x):
     """MXFP4 of a BF16, FP16 or FP32 CUDA tensor along its last axis (a multiple
     of 32).  A matrix may have a row stride; a block holding an infinity or NaN
     reads back as NaN."""
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or x.dtype not in _DTYPES:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _DTYPES:
         raise ValueError("x must be a BF16, FP16 or FP32 CUDA tensor")
-    if x.ndim < 1 or x.shape[-1] < 1 or x.shape[-1] % BLOCK:
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1 or shape[-1] % BLOCK:
         raise ValueError("the last axis must be a positive multiple of 32")
     rows, cols, ld = _matrix(x)
-    q = Mxfp4(torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=x.device),
-              torch.empty((*x.shape[:-1], cols // BLOCK), dtype=torch.uint8, device=x.device))
-    with torch.cuda.device(x.device):
-        check(lib.pdx_mxfp4_quantize(_ptr(x), _DTYPES[x.dtype], rows, cols, ld, _ptr(q.codes), _ptr(q.scales),
-                                     _stream()))
-    return q
+    codes = x.new_empty((*shape[:-1], cols // 2), dtype=torch.uint8)
+    scales = x.new_empty((*shape[:-1], cols // BLOCK), dtype=torch.uint8)
+    with _on(x.device):
+        check(lib.pdx_mxfp4_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, cols, ld, codes.data_ptr(),
+                                     scales.data_ptr(), _raw_stream(x.device)))
+    return Mxfp4(codes, scales)
 
 
 def _require_mxfp4(name, q, ndim=None):
     if not isinstance(q, Mxfp4):
         raise ValueError(f"{name} must be an Mxfp4")
     for t in (q.codes, q.scales):
-        if t.device.type != "cuda" or t.dtype != torch.uint8 or not t.is_contiguous():
+        if not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous():
             raise ValueError(f"{name} must hold contiguous uint8 CUDA tensors")
-    if (q.codes.device != q.scales.device or q.codes.ndim < 1 or q.shape[-1] < 1 or q.shape[-1] % BLOCK
-            or q.scales.shape != (*q.codes.shape[:-1], q.shape[-1] // BLOCK)
-            or (ndim is not None and q.codes.ndim != ndim)):
+    shape = q.codes.shape
+    if (q.codes.device != q.scales.device or len(shape) < 1 or shape[-1] < 1 or shape[-1] % (BLOCK // 2)
+            or q.scales.shape != (*shape[:-1], shape[-1] * 2 // BLOCK) or (ndim is not None and len(shape) != ndim)):
         raise ValueError(f"{name}: codes must be [..., K/2] and scales [..., K/32], K a positive multiple of 32")
 
 
@@ -79,11 +81,12 @@ def dequantize_mxfp4(q, dtype=torch.bfloat16):
     _require_mxfp4("q", q)
     if dtype not in _DTYPES:
         raise ValueError("dtype must be BF16, FP16 or FP32")
-    out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
-    cols = q.shape[-1]
-    with torch.cuda.device(out.device):
-        check(lib.pdx_mxfp4_dequantize(_ptr(q.codes), _ptr(q.scales), out.numel() // cols, cols, cols,
-                                       _DTYPES[dtype], _ptr(out), _stream()))
+    shape = q.shape
+    out = q.codes.new_empty(shape, dtype=dtype)
+    cols = shape[-1]
+    with _on(out.device):
+        check(lib.pdx_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.numel() // cols, cols, cols,
+                                       _DTYPES[dtype], out.data_ptr(), _raw_stream(out.device)))
     return out
 
 
@@ -212,13 +215,16 @@ def moe_ffn_mxfp4(x, packed, slab, out=None):
     if t_count < 1 or rows % t_count:
         raise ValueError("the packing does not belong to this batch")
     if out is None:
-        out = torch.empty((rows, hidden), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((rows, hidden))
     else:
         _require_cuda_bf16("out", out, 2)
         if out.shape != (rows, hidden) or out.device != x.device:
             raise ValueError("out must be [T*k, H] on the device of x")
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         # from the stream-ordered allocator: calls on two streams or in two graphs share no scratch
-        ws = torch.empty(ffn_workspace_bytes(slab, rows, experts), dtype=torch.uint8, device=x.device)
-        grouped_ffn(x, t_count, packed.tokens, packed.offsets, packed.active, experts, rows, slab, out, ws)
+        nbytes = ffn_workspace_bytes(slab, rows, experts)
+        ws = x.new_empty((nbytes,), dtype=torch.uint8)
+        check(lib.pdx_mxfp4_ffn_grouped(x.data_ptr(), t_count, packed.tokens.data_ptr(), packed.offsets.data_ptr(),
+                                        packed.active.data_ptr(), experts, rows, ctypes.byref(slab.struct), hidden,
+                                        slab.inter, out.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(x.device)))
     return out

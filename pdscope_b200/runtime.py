@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import hashlib
 from collections import Counter
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -38,6 +39,16 @@ def _stream():
 
 def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def _raw_stream(device):
+    """Handle of ``device``'s current stream, as an int (``_stream`` of another device, without the Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _on(device):
+    """Context in which ``device`` is current."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 class _Workspace:
@@ -334,24 +345,15 @@ class BlockNorm:
 
     def args(self, t_count, hidden, residual_dtype, device):
         """Check against a [t_count, hidden] batch and form pdx_block_norm_args."""
-        if self.post not in _NORMS or self.pre not in _NORMS:
+        post, pre = _NORMS.get(self.post), _NORMS.get(self.pre)
+        if post is None or pre is None:
             raise ValueError("post and pre must be 'none', 'rms' or 'layer'")
         if self.gate_act not in ("none", "sigmoid"):
             raise ValueError("gate_act must be 'none' or 'sigmoid'")
-        for name, norm in (("post", self.post), ("pre", self.pre)):
-            w = getattr(self, name + "_weight")
-            if w is not None:
-                _require_cuda_bf16(name + "_weight", w, 1)
-                if norm == "none":
-                    raise ValueError(f"{name}_weight without a {name} norm")
-                if w.shape[0] != hidden or w.device != device:
-                    raise ValueError(f"{name}_weight must be [H] on the device of residual")
-        a = _lib.BlockNormArgs(post=_NORMS[self.post], pre=_NORMS[self.pre],
-                               post_weight=self.post_weight.data_ptr() if self.post_weight is not None else None,
-                               pre_weight=self.pre_weight.data_ptr() if self.pre_weight is not None else None,
-                               gate_sigmoid=int(self.gate_act == "sigmoid"),
-                               residual_fp32=int(residual_dtype == torch.float32),
-                               residual_scale=self.residual_scale, block_scale=self.block_scale, eps=self.eps)
+        a = _lib.BlockNormArgs(post, pre, _norm_weight("post", self.post_weight, post, hidden, device),
+                               _norm_weight("pre", self.pre_weight, pre, hidden, device), None, 0, 0,
+                               self.gate_act == "sigmoid", residual_dtype == torch.float32, self.residual_scale,
+                               self.block_scale, self.eps)
         g = self.gate
         if g is not None:
             if not isinstance(g, torch.Tensor) or g.device != device or g.dtype != torch.bfloat16:
@@ -359,35 +361,58 @@ class BlockNorm:
             if g.ndim > 2 or any(n not in (1, full) for n, full in zip(g.shape[::-1], (hidden, t_count))):
                 raise ValueError("gate does not broadcast against [T, H]")
             g = g.expand(t_count, hidden)
-            a.gate, a.gate_row, a.gate_col = g.data_ptr(), g.stride(0), g.stride(1)
+            a.gate = g.data_ptr()
+            a.gate_row, a.gate_col = g.stride()
         return a
 
 
-def _overlap(a, b):
-    """Whether two contiguous tensors share memory."""
-    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size()
-            and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+def _norm_weight(name, w, norm, hidden, device):
+    if w is None:
+        return None
+    _require_cuda_bf16(name + "_weight", w, 1)
+    if norm == _lib.NORM_NONE:
+        raise ValueError(f"{name}_weight without a {name} norm")
+    if w.shape[0] != hidden or w.device != device:
+        raise ValueError(f"{name}_weight must be [H] on the device of residual")
+    return w.data_ptr()
 
 
-def _block_norm_outputs(norm, residual, stream_out, out):
-    if not isinstance(residual, torch.Tensor) or residual.device.type != "cuda" or residual.ndim != 2 \
+def _span(t):
+    """First byte and end of a contiguous tensor."""
+    at = t.data_ptr()
+    return at, at + t.numel() * t.element_size()
+
+
+def _block_norm_outputs(norm, options, residual, stream_out, out, apart=None):
+    """Checked (arguments, stream_out, out) of a block norm; ``apart`` must not overlap the outputs."""
+    if norm is None:
+        norm = BlockNorm(**options)
+    elif options or not isinstance(norm, BlockNorm):
+        raise ValueError("pass either norm=BlockNorm(...) or its fields")
+    if not isinstance(residual, torch.Tensor) or not residual.is_cuda or residual.ndim != 2 \
             or residual.dtype not in (torch.bfloat16, torch.float32) or not residual.is_contiguous():
         raise ValueError("residual must be a contiguous [T, H] BF16 or FP32 CUDA tensor")
+    fresh = stream_out is None and out is None
     if stream_out is None:
         stream_out = torch.empty_like(residual)
     elif (stream_out.shape != residual.shape or stream_out.dtype != residual.dtype
           or stream_out.device != residual.device or not stream_out.is_contiguous()):
         raise ValueError("stream_out must be contiguous and like residual")
     if out is None:
-        out = torch.empty(residual.shape, dtype=torch.bfloat16, device=residual.device)
+        out = torch.empty_like(residual, dtype=torch.bfloat16)
     else:
         _require_cuda_bf16("out", out, 2)
         if out.shape != residual.shape or out.device != residual.device:
             raise ValueError("out must have residual's shape and device")
-    if _overlap(stream_out, out):
-        raise ValueError("stream_out and out must not overlap")
-    args = norm.args(*residual.shape, residual.dtype, residual.device)
-    return args, stream_out, out
+    if not fresh:
+        spans = [_span(stream_out), _span(out)]
+        if spans[0][0] < spans[1][1] and spans[1][0] < spans[0][1]:
+            raise ValueError("stream_out and out must not overlap")
+        if apart is not None:
+            first, end = _span(apart)
+            if any(a < end and first < b for a, b in spans):
+                raise ValueError("the outputs must not alias rows")
+    return norm.args(*residual.shape, residual.dtype, residual.device), stream_out, out
 
 
 def block_norm(y, residual, *, norm=None, stream_out=None, out=None, **options):
@@ -399,16 +424,16 @@ def block_norm(y, residual, *, norm=None, stream_out=None, out=None, **options):
     FP32.  The options are ``BlockNorm``'s fields, or ``norm=BlockNorm(...)``.
     ``stream`` has residual's type, ``normed`` is BF16; ``stream_out`` and
     ``out`` may be ``y`` or ``residual``."""
-    norm = _block_norm_of(norm, options)
-    args, stream_out, out = _block_norm_outputs(norm, residual, stream_out, out)
+    args, stream_out, out = _block_norm_outputs(norm, options, residual, stream_out, out)
     if y is not None:
         _require_cuda_bf16("y", y, 2)
         if y.shape != residual.shape or y.device != residual.device:
             raise ValueError("y and residual shapes differ")
     t_count, hidden = residual.shape
-    with torch.cuda.device(residual.device):
-        check(lib.pdx_block_norm(_ptr(y), _ptr(residual), t_count, hidden, ctypes.byref(args), _ptr(stream_out),
-                                 _ptr(out), _stream()))
+    with _on(residual.device):
+        check(lib.pdx_block_norm(y.data_ptr() if y is not None else None, residual.data_ptr(), t_count, hidden,
+                                 ctypes.byref(args), stream_out.data_ptr(), out.data_ptr(),
+                                 _raw_stream(residual.device)))
     return stream_out, out
 
 
@@ -416,32 +441,21 @@ def combine_block_norm(rows, weights, inverse, residual, *, norm=None, stream_ou
     """``block_norm`` of the weighted combine of the expert rows,
     ``y[t] = sum_s weights[t, s] * rows[inverse[t*k + s]]`` in FP32 (``combine``
     without its roundings in between); the arguments of both."""
-    norm = _block_norm_of(norm, options)
     _require_cuda_bf16("rows", rows, 2)
     _require_cuda_bf16("weights", weights, 2)
+    device = rows.device
     t_count, k = weights.shape
-    if not isinstance(inverse, torch.Tensor) or inverse.dtype != torch.int32 or inverse.device != rows.device \
+    if not isinstance(inverse, torch.Tensor) or inverse.dtype != torch.int32 or inverse.device != device \
             or inverse.numel() != t_count * k or not inverse.is_contiguous():
         raise ValueError("inverse must be a contiguous int32 tensor of T*k entries on the device of rows")
-    args, stream_out, out = _block_norm_outputs(norm, residual, stream_out, out)
-    if residual.shape != (t_count, rows.shape[1]) or residual.device != rows.device \
-            or weights.device != rows.device:
+    args, stream_out, out = _block_norm_outputs(norm, options, residual, stream_out, out, apart=rows)
+    if residual.shape != (t_count, rows.shape[1]) or residual.device != device or weights.device != device:
         raise ValueError("residual must be [T, H] on the device of rows")
-    if _overlap(stream_out, rows) or _overlap(out, rows):
-        raise ValueError("the outputs must not alias rows")
-    with torch.cuda.device(rows.device):
-        check(lib.pdx_combine_block_norm(_ptr(rows), rows.shape[0], _ptr(weights), _ptr(inverse), t_count, k,
-                                         rows.shape[1], _ptr(residual), ctypes.byref(args), _ptr(stream_out),
-                                         _ptr(out), _stream()))
+    with _on(device):
+        check(lib.pdx_combine_block_norm(rows.data_ptr(), rows.shape[0], weights.data_ptr(), inverse.data_ptr(),
+                                         t_count, k, rows.shape[1], residual.data_ptr(), ctypes.byref(args),
+                                         stream_out.data_ptr(), out.data_ptr(), _raw_stream(device)))
     return stream_out, out
-
-
-def _block_norm_of(norm, options):
-    if norm is None:
-        return BlockNorm(**options)
-    if options or not isinstance(norm, BlockNorm):
-        raise ValueError("pass either norm=BlockNorm(...) or its fields")
-    return norm
 
 
 # ---------------------------------------------------------------------------
