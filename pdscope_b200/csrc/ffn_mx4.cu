@@ -48,6 +48,7 @@ constexpr uint32_t kMx4ABytes = 128 * kMx4BK;       // one weight tile, a byte p
 constexpr int kMx4TileBytes = 128 * kMx4BK / 2;     // its codes in memory
 constexpr uint32_t kMx4SfBytes = 512;               // scales of 128 rows x 128 columns
 constexpr int kMx4MaxActive = 1024;
+constexpr int kMx4MinPart = 4;                      // K steps of a part of a tile, at least
 constexpr uint32_t kMx4TmemCols = 512;
 constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of (gate | up | token) scales, 4 columns each
 constexpr uint32_t kMx4OneCol = 496;                // token scales of 1 (x is scaled by its row factor)
@@ -80,7 +81,8 @@ __device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint
 // values a lane at a time; up to kMx4SplitHeld of those stay in registers
 // between finding the row's largest value and splitting, longer rows are read
 // again.  One warp a row for many rows, four for few, where the trip to memory
-// is what a row costs.  CTA 0 clears the tickets of the two products that follow.
+// is what a row costs.  The kernel also clears the tickets of the two products
+// that follow.
 constexpr int kMx4SplitWarps = 4;     // warps per CTA
 constexpr int kMx4SplitHeld = 8;
 template <int WARPS>
@@ -91,8 +93,9 @@ __global__ void __launch_bounds__(kMx4SplitWarps * 32, 8)
     griddep_wait();
     griddep_launch();
     __shared__ uint32_t s_top[kMx4SplitWarps];
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < zero_words; i += blockDim.x) zero_ptr[i] = 0u;
+    for (int i = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x); i < zero_words;
+         i += static_cast<int>(gridDim.x * blockDim.x))
+        zero_ptr[i] = 0u;
     constexpr int kGroups = kMx4SplitWarps / WARPS, kLanes = 32 * WARPS;
     const int group = static_cast<int>(threadIdx.x) / kLanes, lane = static_cast<int>(threadIdx.x) % kLanes;
     const int chunks = H / 8, chunks_p = Hp / 8;
@@ -169,6 +172,14 @@ struct Mx4Args {
     float* partials;                // [gridDim.x][2][columns][128]
     unsigned int* tickets;          // [tiles * kMx4EpiWarps], zero on entry
 };
+
+// One more of the parts of a tile is stored: the parts written before it (by the
+// lanes of this warp, behind __syncwarp) are visible to whoever sees the count.
+__device__ __forceinline__ unsigned int ticket_acq_rel(unsigned int* p) {
+    unsigned int v;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -315,11 +326,16 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     // CTA c takes the whole tiles c, c + G, ... of the full waves of G tiles, and
     // before them its share [w0, w1) of the (tile, K step) sequence of the rest
     // (`work` steps), at least one step per sharing CTA, so every CTA between two
-    // sharers of a tile shares it too.
+    // sharers of a tile shares it too.  Without a full wave (a few tokens) joining
+    // the parts is what a shared tile costs, so a tile is cut into equal parts of
+    // at least kMx4MinPart steps or not at all: one token at H = 2048, I = 768, 8
+    // experts takes 48 gate/up tiles of 16 steps in 3 parts, 64 down tiles of 6 whole.
     const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
     const int waves = s_misc[0] / grid, whole_tiles = waves * grid;
-    const int64_t work = static_cast<int64_t>(s_misc[0] - whole_tiles) * nkb;
-    const int64_t shares = max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), work));
+    const int rest = s_misc[0] - whole_tiles;
+    const int64_t work = static_cast<int64_t>(rest) * nkb;
+    const int64_t shares = waves > 0 ? max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), work))
+                                     : rest * max(1, min(grid / max(rest, 1), nkb / kMx4MinPart));
     const int64_t w0 = cta < shares ? work * cta / shares : 0;
     const int64_t w1 = cta < shares ? work * (cta + 1) / shares : 0;
 
@@ -457,21 +473,22 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         const int q = warp & 3;                                  // TMEM lane quadrant
         const int half = (warp - 2) >> 2;                        // this warp's chunks: half, half + 2, ...
         const int i_row = q * 32 + static_cast<int>(lane);
-        // Token columns [c0, c0 + 8) of a tile: the sums g of the first, u of the second 128 weight rows.
-        auto finish = [&](const Tile& t, int c0, float (&g)[kMx4Chunk], float (&u)[kMx4Chunk]) {
-            const int r0 = t.nb * NT + c0;                       // row of the expert's segment
-            const int n = min(kMx4Chunk, t_rows[t.a] - r0);
-            if (n <= 0) return;
-            const int64_t p0 = static_cast<int64_t>(t_seg0[t.a]) + r0;
+        float rs[(NT + 31) / 32];                                // factor of the tile's row 32 i + lane (SWIGLU)
+        // Token columns [c0, c0 + n), n <= 8, of a tile: the sums g of the first, u of the second 128 weight rows.
+        auto finish = [&](const Tile& t, int c0, int n, float (&g)[kMx4Chunk], float (&u)[kMx4Chunk]) {
+            const int64_t p0 = static_cast<int64_t>(t_seg0[t.a]) + t.nb * NT + c0;
             if (SWIGLU) {
-                const float rs = static_cast<int>(lane) < n ? __ldcg(args.row_scale + p0 + lane) : 0.f;
+                float factor = 0.f;                              // of row 32 (c0 / 32) + lane
+#pragma unroll
+                for (int i = 0; i < (NT + 31) / 32; ++i)
+                    if (c0 / 32 == i) factor = rs[i];
                 uint32_t byte = 0;                               // lane j: scale byte of column j
                 uint8_t* at = args.h + p0 * args.M + t.mt * 128 + i_row;
                 const int64_t lo_at = static_cast<int64_t>(args.rows) * args.M;
                 uint32_t top[kMx4Chunk];
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) {
-                    const float s = __shfl_sync(0xffffffffu, rs, j);
+                    const float s = __shfl_sync(0xffffffffu, factor, c0 % 32 + j);
                     const float gs = g[j] * s;
                     g[j] = __fdividef(gs, 1.0f + __expf(-gs)) * (u[j] * s);
                     // the 32 lanes are one scale block of h
@@ -518,6 +535,13 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         for (Tile t = begin(); next(t); ++lt) {
             const int b = lt & 1;
             const uint32_t acc_phase = static_cast<uint32_t>(lt >> 1) & 1u;
+            const int ne = min(NT, t_rows[t.a] - t.nb * NT);     // rows of the tile
+            if (SWIGLU) {
+                const float* row_scale = args.row_scale + t_seg0[t.a] + t.nb * NT;
+#pragma unroll
+                for (int i = 0; i < (NT + 31) / 32; ++i)
+                    rs[i] = 32 * i + static_cast<int>(lane) < ne ? __ldcg(row_scale + 32 * i + lane) : 0.f;
+            }
             if (!mbar_wait(&tmem_full[b], acc_phase, abort_flag)) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(b * S::kAcc);
@@ -526,63 +550,74 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             // last tile (slot 1), every other part its CTA's first (slot 0)
             float* mine = args.partials +
                           (static_cast<int64_t>(cta) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
-            for (int c0 = half * kMx4Chunk; c0 < NT; c0 += 2 * kMx4Chunk) {
+            for (int c = half * kMx4Chunk; c < ne; c += 2 * kMx4Chunk) {
+                const int n = min(kMx4Chunk, ne - c);
                 uint32_t r[4][kMx4Chunk];
-                tmem_ld8(taddr + c0, r[0]);
-                tmem_ld8(taddr + S::kN + c0, r[1]);
+                tmem_ld8(taddr + c, r[0]);
+                tmem_ld8(taddr + S::kN + c, r[1]);
                 if (S::kStack) {
-                    tmem_ld8(taddr + NT + c0, r[2]);
-                    tmem_ld8(taddr + S::kN + NT + c0, r[3]);
+                    tmem_ld8(taddr + NT + c, r[2]);
+                    tmem_ld8(taddr + S::kN + NT + c, r[3]);
                 }
                 tmem_wait_ld();
+                if (c + 2 * kMx4Chunk >= ne) {                   // this warp's last columns are read
+                    tc_fence_before();
+                    mbar_arrive(&tmem_empty[b]);
+                }
                 float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) {
                     g[j] = __uint_as_float(r[0][j]) + (S::kStack ? __uint_as_float(r[2][j]) : 0.f);
                     u[j] = __uint_as_float(r[1][j]) + (S::kStack ? __uint_as_float(r[3][j]) : 0.f);
                 }
-                if (c0 + 2 * kMx4Chunk >= NT) {
-                    tc_fence_before();
-                    mbar_arrive(&tmem_empty[b]);
-                }
                 if (whole) {
-                    finish(t, c0, g, u);
+                    finish(t, c, n, g, u);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < kMx4Chunk; ++j) {
-                        mine[(c0 + j) * 128] = g[j];
-                        mine[(NT + c0 + j) * 128] = u[j];
-                    }
+                    for (int j = 0; j < kMx4Chunk; ++j)
+                        if (j < n) {
+                            mine[(c + j) * 128] = g[j];
+                            mine[(NT + c + j) * 128] = u[j];
+                        }
                 }
+            }
+            if (half * kMx4Chunk >= ne) {
+                tc_fence_before();
+                mbar_arrive(&tmem_empty[b]);
             }
             if (whole) continue;
             // the CTAs that share the tile: step w belongs to CTA floor(((w + 1) shares - 1) / work)
             const int64_t first = static_cast<int64_t>(t.index - whole_tiles) * nkb, last = first + nkb - 1;
             const int c_first = static_cast<int>(((first + 1) * shares - 1) / work);
             const int c_last = static_cast<int>(((last + 1) * shares - 1) / work);
-            __threadfence();
             __syncwarp();
             unsigned int prev = 0;
-            if (lane == 0) prev = atomicAdd(&args.tickets[t.index * kMx4EpiWarps + warp - 2], 1u);
+            if (lane == 0) prev = ticket_acq_rel(&args.tickets[t.index * kMx4EpiWarps + warp - 2]);
             prev = __shfl_sync(0xffffffffu, prev, 0);
             if (prev != static_cast<unsigned int>(c_last - c_first)) continue;
-            __threadfence();
-            for (int c0 = half * kMx4Chunk; c0 < NT; c0 += 2 * kMx4Chunk) {
+            for (int col = half * kMx4Chunk; col < ne; col += 2 * kMx4Chunk) {
+                const int n = min(kMx4Chunk, ne - col);
                 float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) g[j] = u[j] = 0.f;
-#pragma unroll 4
+#pragma unroll 2
                 for (int c = c_first; c <= c_last; ++c) {
                     // c_first holds the tile's first K step
                     const float* p = args.partials +
                                      (static_cast<int64_t>(c) * 2 + (c == c_first ? 1 : 0)) * S::kCols * 128 + i_row;
+                    float pg[kMx4Chunk], pu[kMx4Chunk];
 #pragma unroll
                     for (int j = 0; j < kMx4Chunk; ++j) {
-                        g[j] += __ldcg(p + (c0 + j) * 128);
-                        u[j] += __ldcg(p + (NT + c0 + j) * 128);
+                        pg[j] = j < n ? __ldcg(p + (col + j) * 128) : 0.f;
+                        pu[j] = j < n ? __ldcg(p + (NT + col + j) * 128) : 0.f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < kMx4Chunk; ++j) {
+                        g[j] += pg[j];
+                        u[j] += pu[j];
                     }
                 }
-                finish(t, c0, g, u);
+                finish(t, col, n, g, u);
             }
         }
     }
