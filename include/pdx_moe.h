@@ -334,7 +334,7 @@ int pdx_mxfp4_dequantize(const void *codes, const void *scales, int64_t rows, in
  * row r and columns c .. c + 31.  Slot s holds the tiles of gate [I, H], up
  * [I, H] and down [H, I] back to back from codes + s*code_stride, and their
  * scales from scales + s*scale_stride (strides in bytes).  codes 128-byte,
- * scales 16-byte aligned; code_stride a multiple of 8192, scale_stride of 16. */
+ * scales 16-byte aligned; code_stride a multiple of 8192, scale_stride of 512. */
 typedef struct pdx_mxfp4_weights {
     const void *codes;
     const void *scales;

@@ -192,23 +192,38 @@ __device__ __forceinline__ uint64_t mx4_sf_desc(uint32_t smem_addr) {  // 32 x 1
            (static_cast<uint64_t>(1) << 46);
 }
 
-// A = E2M1 (5), B = E4M3 (0), E8M0 scales, M = 128; the scale byte of the K step is or'ed in.
-__host__ __device__ constexpr uint32_t mx4_idesc(int n) {
-    return (5u << 7) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (1u << 27);
+// A = E2M1 (5), B = E4M3 (0), E8M0 scales; the scale byte of the K step is or'ed in.
+__host__ __device__ constexpr uint32_t mx4_idesc(int m, int n) {
+    return (5u << 7) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27);
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void umma_mx4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                          uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::
+                "r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::
+                "r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
 }
 
+// 512 bytes of scales from shared memory to four TMEM columns (PAIR: in both
+// CTAs, each from its own shared memory).
+template <bool PAIR>
 __device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    if (PAIR)
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -216,6 +231,15 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
             smem_u32(smem_dst)),
         "l"(src), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, int32_t x,
+                                                 int32_t y, int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+        "%5}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 
@@ -228,27 +252,38 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, ui
         : "memory");
 }
 
-template <int NT>
+template <int NT, bool PAIR>
 struct Mx4Shape {
     static constexpr bool kStack = NT <= 32;                        // pieces side by side along N
     static constexpr int kN = kStack ? 2 * NT : NT;                 // N of one MMA
     static constexpr int kAcc = 2 * kN;                             // accumulator columns of a tile
     static constexpr int kCols = 2 * NT;                            // FP32 columns of a partial tile
+    static constexpr int kBRows = PAIR ? NT / 2 : NT;               // token rows a CTA stages
     static constexpr uint32_t kA = 2 * kMx4ABytes;
     static constexpr uint32_t kATx = kA / 2;                        // the copy counts the packed bytes it reads
-    static constexpr uint32_t kB = 2 * NT * kMx4BK;
+    static constexpr uint32_t kB = 2 * kBRows * kMx4BK;
     static constexpr uint32_t kStage = kA + kB;                     // multiple of 1024
     static constexpr uint32_t kSf = 3 * kMx4SfBytes;                // both weight halves | tokens
     static constexpr uint32_t kTables = 4 * (kMx4MaxActive + 1) * 4;
     static constexpr int kStages = static_cast<int>((kMx4SmemLimit - 1024 - 512 - 512 - kTables) / (kStage + kSf));
     static constexpr size_t kSmem = 1024 + kStages * (kStage + kSf) + 512 + 512 + kTables;
-    static_assert(NT % 16 == 0 && kStages >= 2 && 2 * kAcc <= static_cast<int>(kMx4SfCol), "token tile");
+    static_assert(NT % 16 == 0 && kBRows % 8 == 0 && !(PAIR && kStack) && kStages >= 2 &&
+                      2 * kAcc <= static_cast<int>(kMx4SfCol),
+                  "token tile");
 };
 
-template <int NT, bool SWIGLU>
+// PAIR: a cluster of two CTAs shares a tile of 512 weight rows (tcgen05
+// cta_group::2): each CTA stages its own 256 weight rows and half of the token
+// rows, rank 0 issues the MMAs for both, each CTA's TMEM holds the sums of its own
+// weight rows.  Token bytes from L2 and their shared memory are halved, which
+// leaves room for a fourth stage at NT = 112.  Rank 0's full barriers count the
+// bytes of both CTAs; rank 0 commits to the empty and TMEM barriers of both.
+template <int NT, bool SWIGLU, bool PAIR>
 __global__ void __launch_bounds__(kMx4Threads, 1)
-    k_mx4_gemm(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, Mx4Args args) {
-    using S = Mx4Shape<NT>;
+    k_mx4_gemm(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+               const __grid_constant__ CUtensorMap tm_ws, const __grid_constant__ CUtensorMap tm_xs, Mx4Args args) {
+    using S = Mx4Shape<NT, PAIR>;
+    constexpr int kCtas = PAIR ? 2 : 1;
     extern __shared__ __align__(1024) unsigned char smem_mx4[];
     unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
     unsigned char* s_sf = smem + S::kStages * S::kStage;             // kStages x kSf
@@ -270,7 +305,17 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     const int warp = static_cast<int>(threadIdx.x >> 5);
     const uint32_t lane = lane_id();
     const int m_blocks = args.M / 128, nkb = args.K / kMx4BK;
-    const int m_tiles = SWIGLU ? m_blocks : (m_blocks + 1) / 2;
+    constexpr int kTileBlocks = (SWIGLU ? 1 : 2) * kCtas;    // 128-row blocks of M a tile covers
+    const int m_tiles = (m_blocks + kTileBlocks - 1) / kTileBlocks;
+    const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
+    const uint32_t peer_abort =
+        PAIR ? mapa_shared(smem_u32(const_cast<int*>(abort_flag)), static_cast<uint32_t>(rank ^ 1)) : 0u;
+    // Bounded wait; running out releases the other roles, and the other CTA.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_wait(bar, parity, abort_flag)) return true;
+        if (PAIR) st_shared_remote_u32(peer_abort, 1u);
+        return false;
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -279,7 +324,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tmem_full[b], 1);
-            mbar_init(&tmem_empty[b], kMx4EpiWarps * 32);
+            mbar_init(&tmem_empty[b], kCtas * kMx4EpiWarps);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -288,10 +333,19 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         tma_prefetch_desc(&tm_x);
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(kMx4TmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile(
+                "tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                "r"(kMx4TmemCols)
+                : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile(
+                "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                "r"(kMx4TmemCols)
+                : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     if (warp >= 3)
         for (int i = static_cast<int>(threadIdx.x) - 96; i < 128; i += kMx4Threads - 96)
@@ -321,16 +375,22 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                                            [&](int a) { return m_tiles * ((t_rows[a] + NT - 1) / NT); });
         if (lane == 0) s_misc[0] = total;
     }
-    __syncthreads();
+    __syncwarp();
+    if (PAIR)
+        cluster_sync_all();   // both CTAs' barriers are initialised before any remote arrival
+    else
+        __syncthreads();
+    const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full_bar), 0) : 0u;          // rank 0's barriers
+    const uint32_t tmem_empty0 = PAIR ? mapa_shared(smem_u32(tmem_empty), 0) : 0u;
     const uint32_t tmem_base = *tmem_slot;
-    // CTA c takes the whole tiles c, c + G, ... of the full waves of G tiles, and
+    // CTA (or pair) c takes the whole tiles c, c + G, ... of the full waves of G tiles, and
     // before them its share [w0, w1) of the (tile, K step) sequence of the rest
     // (`work` steps), at least one step per sharing CTA, so every CTA between two
     // sharers of a tile shares it too.  Without a full wave (a few tokens) joining
     // the parts is what a shared tile costs, so a tile is cut into equal parts of
     // at least kMx4MinPart steps or not at all: one token at H = 2048, I = 768, 8
     // experts takes 48 gate/up tiles of 16 steps in 3 parts, 64 down tiles of 6 whole.
-    const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+    const int grid = static_cast<int>(gridDim.x) / kCtas, cta = static_cast<int>(blockIdx.x) / kCtas;
     const int waves = s_misc[0] / grid, whole_tiles = waves * grid;
     const int rest = s_misc[0] - whole_tiles;
     const int64_t work = static_cast<int64_t>(rest) * nkb;
@@ -379,24 +439,42 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             bool ok = true;
             for (Tile t = begin(); ok && next(t);) {
                 const int64_t slot = t_slot[t.a];
-                // weight tiles of both halves; down's odd last block is loaded twice, its second half unused
-                const int b0 = SWIGLU ? args.tile0 + t.mt * nkb : args.tile0 + 2 * t.mt * nkb;
-                const int b1 = SWIGLU ? args.tile1 + t.mt * nkb : args.tile0 + min(2 * t.mt + 1, m_blocks - 1) * nkb;
-                const int row = static_cast<int>(slot * args.tiles_per_slot) * 128;
+                // weight tiles of both halves; blocks past the last are loaded again and not used
+                const int blk = t.mt * kTileBlocks + rank * (SWIGLU ? 1 : 2), end = m_blocks - 1;
+                const int b0 = args.tile0 + min(blk, end) * nkb;
+                const int b1 = SWIGLU ? args.tile1 + min(blk, end) * nkb : args.tile0 + min(blk + 1, end) * nkb;
+                const int64_t tile0 = slot * args.tiles_per_slot;
                 const uint8_t* sf = args.scales + slot * args.scale_stride;
+                const int sf_row = static_cast<int>(slot * (args.scale_stride / kMx4SfBytes));
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                    if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+                    if (!wait(&empty_bar[stage], phase ^ 1u)) { ok = false; break; }
                     unsigned char* sa = smem + stage * S::kStage;
                     unsigned char* ss = s_sf + stage * S::kSf;
-                    mbar_arrive_expect_tx(&full_bar[stage],
-                                          S::kATx + S::kB + (SWIGLU ? 2 : 3) * kMx4SfBytes);
-                    tma_load_2d(sa, &tm_w, &full_bar[stage], 0, row + (b0 + kb) * 128);
-                    tma_load_2d(sa + kMx4ABytes, &tm_w, &full_bar[stage], 0, row + (b1 + kb) * 128);
-                    bulk_load(ss, sf + static_cast<int64_t>(b0 + kb) * kMx4SfBytes, kMx4SfBytes, &full_bar[stage]);
-                    bulk_load(ss + kMx4SfBytes, sf + static_cast<int64_t>(b1 + kb) * kMx4SfBytes, kMx4SfBytes,
-                              &full_bar[stage]);
+                    const int y0 = static_cast<int>(tile0 + b0 + kb) * 128, y1 = static_cast<int>(tile0 + b1 + kb) * 128;
+                    if (rank == 0)
+                        mbar_arrive_expect_tx(&full_bar[stage],
+                                              kCtas * (S::kATx + S::kB + (SWIGLU ? 2 : 3) * kMx4SfBytes));
+                    if (PAIR) {
+                        const uint32_t fb = full0 + static_cast<uint32_t>(stage) * 8u;
+                        tma_load_2d_pair(sa, &tm_w, fb, 0, y0);
+                        tma_load_2d_pair(sa + kMx4ABytes, &tm_w, fb, 0, y1);
+                        tma_load_2d_pair(ss, &tm_ws, fb, 0, sf_row + b0 + kb);
+                        tma_load_2d_pair(ss + kMx4SfBytes, &tm_ws, fb, 0, sf_row + b1 + kb);
+                    } else {
+                        tma_load_2d(sa, &tm_w, &full_bar[stage], 0, y0);
+                        tma_load_2d(sa + kMx4ABytes, &tm_w, &full_bar[stage], 0, y1);
+                        bulk_load(ss, sf + static_cast<int64_t>(b0 + kb) * kMx4SfBytes, kMx4SfBytes, &full_bar[stage]);
+                        bulk_load(ss + kMx4SfBytes, sf + static_cast<int64_t>(b1 + kb) * kMx4SfBytes, kMx4SfBytes,
+                                  &full_bar[stage]);
+                    }
                     if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
                 }
+            }
+            // PAIR: every stage's last release (a commit of rank 0) has landed before
+            // this CTA's shared memory can go away
+            for (int i = 0; PAIR && i < S::kStages && ok; ++i) {
+                ok = wait(&empty_bar[stage], phase ^ 1u);
+                if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
             }
         }
         __syncwarp();
@@ -409,10 +487,19 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             uint32_t phase = 0;
             bool ok = true;
             for (Tile t = begin(); ok && next(t);) {
-                const int row = t_seg0[t.a] + t.nb * NT;
+                const int row = t_seg0[t.a] + t.nb * NT + rank * S::kBRows;
                 const int64_t tt = prefix[t.a] / m_tiles + t.nb;
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                    if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+                    if (!wait(&empty_bar[stage], phase ^ 1u)) { ok = false; break; }
+                    if (PAIR) {
+                        const uint32_t fb = full0 + static_cast<uint32_t>(stage) * 8u;
+                        tma_load_3d_pair(smem + stage * S::kStage + S::kA, &tm_x, fb, kb * kMx4BK, row, 0);
+                        if (!SWIGLU)
+                            tma_load_2d_pair(s_sf + stage * S::kSf + 2 * kMx4SfBytes, &tm_xs, fb, 0,
+                                             static_cast<int>(tt * nkb + kb));
+                        if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                        continue;
+                    }
                     tma_load_3d(smem + stage * S::kStage + S::kA, &tm_x, &full_bar[stage], kb * kMx4BK, row, 0);
                     if (!SWIGLU)
                         bulk_load(s_sf + stage * S::kSf + 2 * kMx4SfBytes, args.sf + (tt * nkb + kb) * kMx4SfBytes,
@@ -422,52 +509,60 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        constexpr uint32_t idesc = mx4_idesc(S::kN);
-        if (elect_one()) tmem_cp_sf(tmem_base + kMx4OneCol, mx4_sf_desc(smem_u32(s_one)));
+    } else if (warp == 1 && rank == 0) {
+        // ---------------- MMA issuer (of the pair: rank 0) ----------------
+        constexpr uint32_t idesc = mx4_idesc(128 * kCtas, S::kN);
+        if (elect_one()) tmem_cp_sf<PAIR>(tmem_base + kMx4OneCol, mx4_sf_desc(smem_u32(s_one)));
         __syncwarp();
+        auto commit = [&](uint64_t* bar) {   // to this barrier of every CTA of the tile
+            if (PAIR) {
+                umma_commit_pair(smem_u32(bar));
+                umma_commit_pair(mapa_shared(smem_u32(bar), 1));
+            } else {
+                umma_commit(bar);
+            }
+        };
         int stage = 0, lt = 0, step = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (Tile t = begin(); ok && next(t); ++lt) {
             const int b = lt & 1;
             const uint32_t acc_phase = static_cast<uint32_t>(lt >> 1) & 1u;
-            if (!mbar_wait(&tmem_empty[b], acc_phase ^ 1u, abort_flag)) { ok = false; break; }
+            if (!wait(&tmem_empty[b], acc_phase ^ 1u)) { ok = false; break; }
             tc_fence_after();
             const uint32_t d = tmem_base + static_cast<uint32_t>(b * S::kAcc);
             for (int kb = t.kb0; kb < t.kb1; ++kb, ++step) {
-                if (!mbar_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
+                if (!wait(&full_bar[stage], phase)) { ok = false; break; }
                 tc_fence_after();
                 if (elect_one()) {
                     const uint32_t sa = smem_u32(smem + stage * S::kStage);
                     const uint32_t ss = smem_u32(s_sf + stage * S::kSf);
                     const uint32_t sf = tmem_base + kMx4SfCol + static_cast<uint32_t>(step & 3) * 12;
-                    tmem_cp_sf(sf, mx4_sf_desc(ss));
-                    tmem_cp_sf(sf + 4, mx4_sf_desc(ss + kMx4SfBytes));
-                    if (!SWIGLU) tmem_cp_sf(sf + 8, mx4_sf_desc(ss + 2 * kMx4SfBytes));
+                    tmem_cp_sf<PAIR>(sf, mx4_sf_desc(ss));
+                    tmem_cp_sf<PAIR>(sf + 4, mx4_sf_desc(ss + kMx4SfBytes));
+                    if (!SWIGLU) tmem_cp_sf<PAIR>(sf + 8, mx4_sf_desc(ss + 2 * kMx4SfBytes));
                     const uint32_t sfb = SWIGLU ? tmem_base + kMx4OneCol : sf + 8;
                     const uint64_t a0 = sw128_desc(sa), a1 = sw128_desc(sa + kMx4ABytes);
-                    const uint64_t hi = sw128_desc(sa + S::kA), lo = sw128_desc(sa + S::kA + NT * kMx4BK);
+                    const uint64_t hi = sw128_desc(sa + S::kA), lo = sw128_desc(sa + S::kA + S::kBRows * kMx4BK);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint32_t acc = (kb > t.kb0 || kk > 0) ? 1u : 0u;
                         const uint32_t id = idesc | (static_cast<uint32_t>(kk) << 29) | (static_cast<uint32_t>(kk) << 4);
-                        umma_mx4(d, a0 + 2u * kk, hi + 2u * kk, id, sf, sfb, acc);
-                        if (!S::kStack) umma_mx4(d, a0 + 2u * kk, lo + 2u * kk, id, sf, sfb, 1u);
-                        umma_mx4(d + S::kN, a1 + 2u * kk, hi + 2u * kk, id, sf + 4, sfb, acc);
-                        if (!S::kStack) umma_mx4(d + S::kN, a1 + 2u * kk, lo + 2u * kk, id, sf + 4, sfb, 1u);
+                        umma_mx4<PAIR>(d, a0 + 2u * kk, hi + 2u * kk, id, sf, sfb, acc);
+                        if (!S::kStack) umma_mx4<PAIR>(d, a0 + 2u * kk, lo + 2u * kk, id, sf, sfb, 1u);
+                        umma_mx4<PAIR>(d + S::kN, a1 + 2u * kk, hi + 2u * kk, id, sf + 4, sfb, acc);
+                        if (!S::kStack) umma_mx4<PAIR>(d + S::kN, a1 + 2u * kk, lo + 2u * kk, id, sf + 4, sfb, 1u);
                     }
-                    umma_commit(&empty_bar[stage]);
+                    commit(&empty_bar[stage]);
                 }
                 __syncwarp();
                 if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
             }
             if (!ok) break;
-            if (elect_one()) umma_commit(&tmem_full[b]);
+            if (elect_one()) commit(&tmem_full[b]);
             __syncwarp();
         }
-    } else {
+    } else if (warp >= 2) {
         // ---------------- epilogue (warps 2..9) ----------------
         griddep_wait();
         const int q = warp & 3;                                  // TMEM lane quadrant
@@ -477,13 +572,15 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         // Token columns [c0, c0 + n), n <= 8, of a tile: the sums g of the first, u of the second 128 weight rows.
         auto finish = [&](const Tile& t, int c0, int n, float (&g)[kMx4Chunk], float (&u)[kMx4Chunk]) {
             const int64_t p0 = static_cast<int64_t>(t_seg0[t.a]) + t.nb * NT + c0;
+            const int part = t.mt * kCtas + rank;                // of the tiles of 256 weight rows
             if (SWIGLU) {
+                if (part >= m_blocks) return;
                 float factor = 0.f;                              // of row 32 (c0 / 32) + lane
 #pragma unroll
                 for (int i = 0; i < (NT + 31) / 32; ++i)
                     if (c0 / 32 == i) factor = rs[i];
                 uint32_t byte = 0;                               // lane j: scale byte of column j
-                uint8_t* at = args.h + p0 * args.M + t.mt * 128 + i_row;
+                uint8_t* at = args.h + p0 * args.M + part * 128 + i_row;
                 const int64_t lo_at = static_cast<int64_t>(args.rows) * args.M;
                 uint32_t top[kMx4Chunk];
 #pragma unroll
@@ -516,12 +613,12 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 if (lane < kMx4Chunk) {
                     const int r = c0 + static_cast<int>(lane);   // row of the token tile
                     const int64_t tt = prefix[t.a] / m_tiles + t.nb;
-                    uint8_t* sf = args.sf + (tt * m_blocks + t.mt) * kMx4SfBytes + q;
+                    uint8_t* sf = args.sf + (tt * m_blocks + part) * kMx4SfBytes + q;
                     sf[(r & 31) * 16 + (r >> 5) * 4] = static_cast<uint8_t>(byte);
                     if (S::kStack) sf[((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4] = static_cast<uint8_t>(byte);
                 }
             } else {
-                const int col = t.mt * 256 + i_row;
+                const int col = part * 256 + i_row;
                 uint16_t* at = args.y + p0 * args.ldy + col;
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) {
@@ -530,6 +627,15 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     at += args.ldy;
                 }
             }
+        };
+        auto release = [&](int b) {                              // this warp has read accumulator b
+            tc_fence_before();
+            __syncwarp();
+            if (lane != 0) return;
+            if (PAIR)
+                mbar_arrive_remote(tmem_empty0 + static_cast<uint32_t>(b) * 8u);
+            else
+                mbar_arrive(&tmem_empty[b]);
         };
         int lt = 0;
         for (Tile t = begin(); next(t); ++lt) {
@@ -542,14 +648,14 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 for (int i = 0; i < (NT + 31) / 32; ++i)
                     rs[i] = 32 * i + static_cast<int>(lane) < ne ? __ldcg(row_scale + 32 * i + lane) : 0.f;
             }
-            if (!mbar_wait(&tmem_full[b], acc_phase, abort_flag)) break;
+            if (!wait(&tmem_full[b], acc_phase)) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(b * S::kAcc);
             const bool whole = t.kb0 == 0 && t.kb1 == nkb;
             // a share of a tile: the part with the tile's first K step is its CTA's
             // last tile (slot 1), every other part its CTA's first (slot 0)
             float* mine = args.partials +
-                          (static_cast<int64_t>(cta) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
+                          (static_cast<int64_t>(blockIdx.x) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
             for (int c = half * kMx4Chunk; c < ne; c += 2 * kMx4Chunk) {
                 const int n = min(kMx4Chunk, ne - c);
                 uint32_t r[4][kMx4Chunk];
@@ -561,8 +667,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 }
                 tmem_wait_ld();
                 if (c + 2 * kMx4Chunk >= ne) {                   // this warp's last columns are read
-                    tc_fence_before();
-                    mbar_arrive(&tmem_empty[b]);
+                    release(b);
                 }
                 float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll
@@ -582,8 +687,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 }
             }
             if (half * kMx4Chunk >= ne) {
-                tc_fence_before();
-                mbar_arrive(&tmem_empty[b]);
+                release(b);
             }
             if (whole) continue;
             // the CTAs that share the tile: step w belongs to CTA floor(((w + 1) shares - 1) / work)
@@ -592,7 +696,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             const int c_last = static_cast<int>(((last + 1) * shares - 1) / work);
             __syncwarp();
             unsigned int prev = 0;
-            if (lane == 0) prev = ticket_acq_rel(&args.tickets[t.index * kMx4EpiWarps + warp - 2]);
+            if (lane == 0) prev = ticket_acq_rel(&args.tickets[(t.index * kCtas + rank) * kMx4EpiWarps + warp - 2]);
             prev = __shfl_sync(0xffffffffu, prev, 0);
             if (prev != static_cast<unsigned int>(c_last - c_first)) continue;
             for (int col = half * kMx4Chunk; col < ne; col += 2 * kMx4Chunk) {
@@ -604,7 +708,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 for (int c = c_first; c <= c_last; ++c) {
                     // c_first holds the tile's first K step
                     const float* p = args.partials +
-                                     (static_cast<int64_t>(c) * 2 + (c == c_first ? 1 : 0)) * S::kCols * 128 + i_row;
+                                     (static_cast<int64_t>(c * kCtas + rank) * 2 + (c == c_first ? 1 : 0)) * S::kCols * 128 + i_row;
                     float pg[kMx4Chunk], pu[kMx4Chunk];
 #pragma unroll
                     for (int j = 0; j < kMx4Chunk; ++j) {
@@ -622,6 +726,32 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         }
     }
 
+    if (PAIR) {
+        // The other CTA may raise this one's abort flag at any time, so every thread
+        // acts on one snapshot taken after the roles have finished.
+        __syncthreads();
+        if (threadIdx.x == 0) s_misc[1] = *abort_flag;
+        if (warp == 1 && rank == 0) {
+            if (elect_one()) umma_commit_pair(smem_u32(drain_bar));   // every MMA has completed
+            __syncwarp();
+            volatile int never = 0;
+            mbar_wait(drain_bar, 0, &never);
+        }
+        __syncthreads();
+        if (s_misc[1]) {
+            // let this CTA's copies in flight land before its shared memory is released
+            const unsigned long long t0 = global_timer_ns();
+            while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+        }
+        tc_fence_before();
+        cluster_sync_all();   // nothing of the other CTA still reaches into this one
+        if (warp == 1) {
+            tc_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kMx4TmemCols)
+                         : "memory");
+        }
+        return;
+    }
     __syncthreads();
     if (*abort_flag) {
         if (warp == 1) {

@@ -202,12 +202,12 @@ int device_setup(int* sms_out) {
         PDX_DEC_ATTR(true, 64, 16); PDX_DEC_ATTR(true, 64, 32); PDX_DEC_ATTR(true, 64, 64);
         PDX_DEC_ATTR(false, 16, 16); PDX_DEC_ATTR(false, 32, 32); PDX_DEC_ATTR(false, 64, 64);
 #undef PDX_DEC_ATTR
-#define PDX_MX4_ATTR(NT)                                                                                           \
-    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,           \
-                                      static_cast<int>(Mx4Shape<NT>::kSmem)));                               \
-    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,          \
-                                      static_cast<int>(Mx4Shape<NT>::kSmem)))
-        PDX_MX4_ATTR(16); PDX_MX4_ATTR(32); PDX_MX4_ATTR(64); PDX_MX4_ATTR(112);
+#define PDX_MX4_ATTR(NT, PAIR)                                                                                     \
+    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, true, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,     \
+                                      static_cast<int>(Mx4Shape<NT, PAIR>::kSmem)));                               \
+    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, false, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,    \
+                                      static_cast<int>(Mx4Shape<NT, PAIR>::kSmem)))
+        PDX_MX4_ATTR(16, false); PDX_MX4_ATTR(32, false); PDX_MX4_ATTR(64, false); PDX_MX4_ATTR(112, true);
 #undef PDX_MX4_ATTR
         g_num_sms[dev] = sms;
         g_attrs_set[dev] = true;
@@ -947,7 +947,7 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
     if ((reinterpret_cast<uintptr_t>(w->codes) & 127u) || (reinterpret_cast<uintptr_t>(w->scales) & 15u))
         return fail(PDX_ERR_INVALID, "codes must be 128-byte and scales 16-byte aligned");
     if (w->num_slots > 1 && (w->code_stride < 3 * Hp * Ip / 2 || w->scale_stride < 3 * Hp * Ip / 32 ||
-                             w->code_stride % kMx4TileBytes || w->scale_stride % 16))
+                             w->code_stride % kMx4TileBytes || w->scale_stride % kMx4SfBytes))
         return fail(PDX_ERR_INVALID, "slot strides must cover one expert and be whole tiles");
     if (w->num_slots * (std::max(w->code_stride, 3 * Hp * Ip / 2) / (kMx4BK / 2)) >= (int64_t(1) << 31))
         return fail(PDX_ERR_UNSUPPORTED, "expert slab too large for 32-bit TMA row coordinates");
@@ -957,10 +957,11 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
 // Token tile of the MXFP4 path: the smallest that holds an expert's average
 // rows with room to spare (a tile's MMAs cost its full width), 112 at most (two
 // gate/up accumulators of 2 x 112 columns and the scales fill TMEM).
+constexpr int kMx4PairTile = 112;
 int mx4_tile(int64_t rows, int64_t E) {
     const int64_t est = std::max<int64_t>(1, std::min(E, rows));
     const int64_t avg = (rows + est - 1) / est;
-    return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 48 ? 64 : 112));
+    return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 48 ? 64 : kMx4PairTile));
 }
 
 // Rows up to which the split takes four warps a row (all rows in flight at once).
@@ -988,8 +989,9 @@ Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
     b.h = static_cast<uint8_t*>(c.take(2 * rows * Ip));
     b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * kMx4SfBytes));
     b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * 2 * b.nt * 128 * 4));
-    b.words1 = b.tiles * (Ip / 128) * kMx4EpiWarps;
-    b.words2 = b.tiles * ((Hp + 255) / 256) * kMx4EpiWarps;
+    // a ticket per tile, CTA of a pair and epilogue warp; pairs round the tiles of 256 rows up to even
+    b.words1 = b.tiles * ((Ip / 128 + 1) / 2 * 2) * kMx4EpiWarps;
+    b.words2 = b.tiles * ((Hp + 511) / 512 * 2) * kMx4EpiWarps;
     b.tickets = static_cast<unsigned int*>(c.take((b.words1 + b.words2) * 4));
     return b;
 }
@@ -1016,6 +1018,21 @@ int encode_mx4_weights(CUtensorMap* map, const void* base, uint64_t tiles) {
     return PDX_OK;
 }
 
+// Scale tiles of 512 bytes, one box a tile (the pair form; its bulk copies could not count on the other CTA).
+int encode_mx4_scales(CUtensorMap* map, const void* base, uint64_t tiles) {
+    int st = load_encode();
+    if (st) return st;
+    const cuuint64_t dims[2] = {kMx4SfBytes / 4, tiles};
+    const cuuint64_t strides[1] = {kMx4SfBytes};
+    const cuuint32_t box[2] = {kMx4SfBytes / 4, 1};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(PDX_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return PDX_OK;
+}
+
 // E4M3 pieces [2][rows][cols]; boxes of 128 columns x box_rows of both pieces.
 int encode_mx4_tokens(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
     int st = load_encode();
@@ -1031,17 +1048,37 @@ int encode_mx4_tokens(CUtensorMap* map, const void* base, uint64_t rows, uint64_
     return PDX_OK;
 }
 
-template <int NT>
-int launch_mx4_pair(const CUtensorMap& tm_w, const CUtensorMap& tm_x, const Mx4Args& gu, const CUtensorMap& tm_h,
-                    const Mx4Args& down, int64_t tiles, int sms, cudaStream_t stream) {
-    const int64_t most = std::min(sms, kPlanSMs);   // the partial sums are sized for kPlanSMs CTAs
-    const int64_t work1 = tiles * (gu.M / 128) * (gu.K / kMx4BK);
-    const int64_t work2 = tiles * ((down.M + 255) / 256) * (down.K / kMx4BK);
-    constexpr size_t smem = Mx4Shape<NT>::kSmem;
-    PDX_PDL_TRY(launch_pdl(k_mx4_gemm<NT, true>, dim3(static_cast<unsigned>(std::min(most, work1))), dim3(kMx4Threads),
-                           smem, stream, tm_w, tm_x, gu));
-    PDX_PDL_TRY(launch_pdl(k_mx4_gemm<NT, false>, dim3(static_cast<unsigned>(std::min(most, work2))), dim3(kMx4Threads),
-                           smem, stream, tm_w, tm_h, down));
+struct Mx4Maps {
+    CUtensorMap w, ws;      // weight codes and scales
+    CUtensorMap x, h, hs;   // token pieces of both products, scales of h
+};
+
+// The two products on tiles of NT tokens; PAIR: as clusters of two CTAs.
+template <int NT, bool PAIR>
+int launch_mx4_products(const Mx4Maps& m, const Mx4Args& gu, const Mx4Args& down, int64_t tiles, int sms,
+                        cudaStream_t stream) {
+    constexpr int64_t ctas = PAIR ? 2 : 1;
+    const int64_t most = std::min(sms, kPlanSMs) / ctas;   // the partial sums are sized for kPlanSMs CTAs
+    const int64_t work1 = tiles * ((gu.M / 128 + ctas - 1) / ctas) * (gu.K / kMx4BK);
+    const int64_t work2 = tiles * ((down.M / 128 + 2 * ctas - 1) / (2 * ctas)) * (down.K / kMx4BK);
+    auto launch = [&](auto kernel, int64_t work, const CUtensorMap& tokens, const Mx4Args& a) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(ctas * std::min(most, work)));
+        cfg.blockDim = dim3(kMx4Threads);
+        cfg.dynamicSmemBytes = Mx4Shape<NT, PAIR>::kSmem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = PAIR ? 2 : 1;
+        return cudaLaunchKernelEx(&cfg, kernel, m.w, tokens, m.ws, m.hs, a);
+    };
+    PDX_PDL_TRY(launch(k_mx4_gemm<NT, true, PAIR>, work1, m.x, gu));
+    PDX_PDL_TRY(launch(k_mx4_gemm<NT, false, PAIR>, work2, m.h, down));
     return PDX_OK;
 }
 
@@ -1057,10 +1094,14 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     const int per = (Hp / 128) * (Ip / 128);        // weight tiles of a projection
     const int64_t slots = w->num_slots, ss = slots > 1 ? w->scale_stride : 0;
     const int64_t tps = slots > 1 ? w->code_stride / kMx4TileBytes : 0;
-    CUtensorMap tm_w, tm_x, tm_h;
-    if ((st = encode_mx4_weights(&tm_w, w->codes, (slots - 1) * tps + 3 * per))) return st;
-    if ((st = encode_mx4_tokens(&tm_x, b.x, rows, Hp, b.nt))) return st;
-    if ((st = encode_mx4_tokens(&tm_h, b.h, rows, Ip, b.nt))) return st;
+    const bool pair = b.nt == kMx4PairTile;
+    const int box = pair ? b.nt / 2 : b.nt;
+    Mx4Maps m;
+    if ((st = encode_mx4_weights(&m.w, w->codes, (slots - 1) * tps + 3 * per))) return st;
+    if ((st = encode_mx4_tokens(&m.x, b.x, rows, Hp, box))) return st;
+    if ((st = encode_mx4_tokens(&m.h, b.h, rows, Ip, box))) return st;
+    if ((st = encode_mx4_scales(&m.ws, w->scales, (slots - 1) * (ss / kMx4SfBytes) + 3 * per))) return st;
+    if ((st = encode_mx4_scales(&m.hs, b.sf, b.tiles * (Ip / 128)))) return st;
     const bool few = rows <= kMx4SplitFew;
     const int64_t split_ctas = few ? rows : (rows + kMx4SplitWarps - 1) / kMx4SplitWarps;
     PDX_PDL_TRY(launch_pdl(few ? k_mx4_split<kMx4SplitWarps> : k_mx4_split<1>,
@@ -1074,10 +1115,10 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     Mx4Args down{offsets, active, w->slot_of_expert, slots, scales, ss, tps, 2 * per, 0, Ip, Hp, n,
                  static_cast<int>(E), nullptr, b.sf, nullptr, static_cast<uint16_t*>(y), static_cast<int>(H),
                  b.partials, b.tickets + b.words1};
-    if (b.nt == 16) return launch_mx4_pair<16>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
-    if (b.nt == 32) return launch_mx4_pair<32>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
-    if (b.nt == 64) return launch_mx4_pair<64>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
-    return launch_mx4_pair<112>(tm_w, tm_x, gu, tm_h, down, b.tiles, sms, stream);
+    if (b.nt == 16) return launch_mx4_products<16, false>(m, gu, down, b.tiles, sms, stream);
+    if (b.nt == 32) return launch_mx4_products<32, false>(m, gu, down, b.tiles, sms, stream);
+    if (b.nt == 64) return launch_mx4_products<64, false>(m, gu, down, b.tiles, sms, stream);
+    return launch_mx4_products<kMx4PairTile, true>(m, gu, down, b.tiles, sms, stream);
 }
 
 // ---- block norms ---------------------------------------------------------------------
