@@ -49,6 +49,7 @@ constexpr int kMx4TileBytes = 128 * kMx4BK / 2;     // its codes in memory
 constexpr uint32_t kMx4SfBytes = 512;               // scales of 128 rows x 128 columns
 constexpr int kMx4MaxActive = 1024;
 constexpr int kMx4MinPart = 4;                      // K steps of a part of a tile, at least
+constexpr uint32_t kMx4StageOut = 1024;             // 8 token columns x 64 weight rows on their way out
 constexpr uint32_t kMx4TmemCols = 512;
 constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of (gate | up | token) scales, 4 columns each
 constexpr uint32_t kMx4OneCol = 496;                // token scales of 1 (x is scaled by its row factor)
@@ -77,16 +78,16 @@ __device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint
 
 // Token rows in packed order as E4M3 pieces: out [2][rows][Hp] (hi rows, then lo
 // rows, zero past H) and the row's factor 2^(b - 127).  HBM-bound (the pieces
-// are written once, x comes from L2).  A group of WARPS warps takes a row, eight
+// are written once, x comes from L2).  A group of WARPS warps takes a row, 16
 // values a lane at a time; up to kMx4SplitHeld of those stay in registers
 // between finding the row's largest value and splitting, longer rows are read
 // again.  One warp a row for many rows, four for few, where the trip to memory
 // is what a row costs.  The kernel also clears the tickets of the two products
 // that follow.
 constexpr int kMx4SplitWarps = 4;     // warps per CTA
-constexpr int kMx4SplitHeld = 8;
+constexpr int kMx4SplitHeld = 4;
 template <int WARPS>
-__global__ void __launch_bounds__(kMx4SplitWarps * 32, 8)
+__global__ void __launch_bounds__(kMx4SplitWarps * 32, 7)
     k_mx4_split(const uint16_t* __restrict__ x, const int32_t* __restrict__ tokens, int T, int rows, int H, int Hp,
                 uint8_t* __restrict__ out, float* __restrict__ row_scale, unsigned int* __restrict__ zero_ptr,
                 int zero_words) {
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kMx4SplitWarps * 32, 8)
         zero_ptr[i] = 0u;
     constexpr int kGroups = kMx4SplitWarps / WARPS, kLanes = 32 * WARPS;
     const int group = static_cast<int>(threadIdx.x) / kLanes, lane = static_cast<int>(threadIdx.x) % kLanes;
-    const int chunks = H / 8, chunks_p = Hp / 8;
+    const int chunks = H / 16, chunks_p = Hp / 16;
     // WARPS > 1: one group per CTA, so the loop below is uniform over the CTA
     static_assert(WARPS == 1 || kGroups == 1, "the barriers need whole CTAs");
     for (int p = static_cast<int>(blockIdx.x) * kGroups + group; p < rows; p += static_cast<int>(gridDim.x) * kGroups) {
@@ -108,21 +109,26 @@ __global__ void __launch_bounds__(kMx4SplitWarps * 32, 8)
             t = 0;
         }
         const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t) * H);
-        uint4 held[kMx4SplitHeld];
+        struct Sixteen {
+            uint4 a, b;
+        };
+        auto load = [&](int c) {
+            Sixteen v{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+            if (c < chunks) v = Sixteen{__ldg(src + 2 * c), __ldg(src + 2 * c + 1)};
+            return v;
+        };
+        Sixteen held[kMx4SplitHeld];
         uint32_t top = 0;
-        auto widen = [&](const uint4& v) {
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        auto widen = [&](const Sixteen& v) {
+            const uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
+            for (int i = 0; i < 8; ++i) top = max(top, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
         };
 #pragma unroll
-        for (int j = 0; j < kMx4SplitHeld; ++j) {
-            const int c = j * kLanes + lane;
-            held[j] = c < chunks ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-        }
+        for (int j = 0; j < kMx4SplitHeld; ++j) held[j] = load(j * kLanes + lane);
 #pragma unroll
         for (int j = 0; j < kMx4SplitHeld; ++j) widen(held[j]);
-        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks; c += kLanes) widen(__ldg(src + c));
+        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks; c += kLanes) widen(load(c));
         top = __reduce_max_sync(0xffffffffu, top);
         if (WARPS > 1) {
             __syncthreads();   // s_top free from the previous row
@@ -133,22 +139,27 @@ __global__ void __launch_bounds__(kMx4SplitWarps * 32, 8)
         }
         const uint32_t byte = mx4_group_byte(top);
         const float inv = mx4_inverse(byte);
-        uint2* hi_row = reinterpret_cast<uint2*>(out + static_cast<int64_t>(p) * Hp);
-        uint2* lo_row = reinterpret_cast<uint2*>(out + (static_cast<int64_t>(rows) + p) * Hp);
-        auto split = [&](const uint4& v, int c) {
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            uint16_t h[4], l[4];
+        uint4* hi_row = reinterpret_cast<uint4*>(out + static_cast<int64_t>(p) * Hp);
+        uint4* lo_row = reinterpret_cast<uint4*>(out + (static_cast<int64_t>(rows) + p) * Hp);
+        auto split = [&](const Sixteen& v, int c) {
+            const uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
+            uint32_t h[4], l[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                e4m3_split2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xFFFF0000u) * inv, h[i], l[i]);
-            hi_row[c] = make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
-            lo_row[c] = make_uint2(l[0] | (static_cast<uint32_t>(l[1]) << 16), l[2] | (static_cast<uint32_t>(l[3]) << 16));
+            for (int i = 0; i < 4; ++i) {
+                uint16_t h0, h1, l0, l1;
+                e4m3_split2(__uint_as_float(w[2 * i] << 16) * inv, __uint_as_float(w[2 * i] & 0xFFFF0000u) * inv, h0, l0);
+                e4m3_split2(__uint_as_float(w[2 * i + 1] << 16) * inv, __uint_as_float(w[2 * i + 1] & 0xFFFF0000u) * inv,
+                            h1, l1);
+                h[i] = h0 | (static_cast<uint32_t>(h1) << 16);
+                l[i] = l0 | (static_cast<uint32_t>(l1) << 16);
+            }
+            hi_row[c] = make_uint4(h[0], h[1], h[2], h[3]);
+            lo_row[c] = make_uint4(l[0], l[1], l[2], l[3]);
         };
 #pragma unroll
         for (int j = 0; j < kMx4SplitHeld; ++j)
             if (j * kLanes + lane < chunks_p) split(held[j], j * kLanes + lane);
-        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks_p; c += kLanes)
-            split(c < chunks ? __ldg(src + c) : make_uint4(0, 0, 0, 0), c);
+        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks_p; c += kLanes) split(load(c), c);
         if (lane == 0) row_scale[p] = mx_scale(byte);
     }
 }
@@ -163,12 +174,13 @@ struct Mx4Args {
     int64_t tiles_per_slot;         // weight tiles between slots
     int tile0, tile1;               // first weight tile of gate and up, or of down (tile0)
     int K, M;                       // multiples of 128: reduction length, weight rows
-    int rows, experts;
+    int rows;
     const float* row_scale;         // [rows] factor of a packed row of x (SWIGLU)
     uint8_t* sf;                    // h scales: [token tile][Ip / 128] tiles of 512 bytes (out of SWIGLU, else in)
     uint8_t* h;                     // [2][rows][M] pieces (SWIGLU)
     uint16_t* y;                    // [rows, ldy] (down)
     int ldy;                        // H
+    int stages, table;              // ring stages, entries of the expert tables (mx4_layout)
     float* partials;                // [gridDim.x][2][columns][128]
     unsigned int* tickets;          // [tiles * kMx4EpiWarps], zero on entry
 };
@@ -264,10 +276,14 @@ struct Mx4Shape {
     static constexpr uint32_t kB = 2 * kBRows * kMx4BK;
     static constexpr uint32_t kStage = kA + kB;                     // multiple of 1024
     static constexpr uint32_t kSf = 3 * kMx4SfBytes;                // both weight halves | tokens
-    static constexpr uint32_t kTables = 4 * (kMx4MaxActive + 1) * 4;
-    static constexpr int kStages = static_cast<int>((kMx4SmemLimit - 1024 - 512 - 512 - kTables) / (kStage + kSf));
-    static constexpr size_t kSmem = 1024 + kStages * (kStage + kSf) + 512 + 512 + kTables;
-    static_assert(NT % 16 == 0 && kBRows % 8 == 0 && !(PAIR && kStack) && kStages >= 2 &&
+    static constexpr uint32_t kFixed = 1024 + 512 + 512 + kMx4EpiWarps * kMx4StageOut;   // alignment, ones, barriers, staging
+    // Ring stages beside tables of `entries` experts, and the shared memory of both.
+    static constexpr int stages(int entries) {
+        return static_cast<int>((kMx4SmemLimit - kFixed - 16u * entries) / (kStage + kSf));
+    }
+    static constexpr size_t smem(int entries) { return kFixed + 16u * entries + stages(entries) * (kStage + kSf); }
+    static constexpr int kMaxStages = stages(1);
+    static_assert(NT % 16 == 0 && kBRows % 8 == 0 && !(PAIR && kStack) && stages(kMx4MaxActive) >= 3 && 2 * kMaxStages + 5 <= 56 &&
                       2 * kAcc <= static_cast<int>(kMx4SfCol),
                   "token tile");
 };
@@ -286,21 +302,22 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     constexpr int kCtas = PAIR ? 2 : 1;
     extern __shared__ __align__(1024) unsigned char smem_mx4[];
     unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
-    unsigned char* s_sf = smem + S::kStages * S::kStage;             // kStages x kSf
-    unsigned char* s_one = s_sf + S::kStages * S::kSf;               // 512 bytes of scale 1
+    const int stages = args.stages;
+    unsigned char* s_sf = smem + stages * S::kStage;                 // stages x kSf
+    unsigned char* s_one = s_sf + stages * S::kSf;                   // 512 bytes of scale 1
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_one + 512);
-    uint64_t* empty_bar = full_bar + S::kStages;
-    uint64_t* tmem_full = empty_bar + S::kStages;
+    uint64_t* empty_bar = full_bar + stages;
+    uint64_t* tmem_full = empty_bar + stages;
     uint64_t* tmem_empty = tmem_full + 2;
     uint64_t* drain_bar = tmem_empty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_misc = reinterpret_cast<int*>(tmem_slot + 2);
-    int* prefix = reinterpret_cast<int*>(s_one + 1024);              // tiles before an active expert
-    int* t_seg0 = prefix + (kMx4MaxActive + 1);
-    int* t_rows = t_seg0 + (kMx4MaxActive + 1);
-    int* t_slot = t_rows + (kMx4MaxActive + 1);
-    static_assert(2 * S::kStages + 5 <= 56, "barriers and words fit 512 bytes");
+    unsigned char* s_out = s_one + 1024;                             // an epilogue warp's staging: kMx4StageOut
+    int* prefix = reinterpret_cast<int*>(s_out + kMx4EpiWarps * kMx4StageOut);   // tiles before an active expert
+    int* t_seg0 = prefix + args.table;
+    int* t_rows = t_seg0 + args.table;
+    int* t_slot = t_rows + args.table;
 
     const int warp = static_cast<int>(threadIdx.x >> 5);
     const uint32_t lane = lane_id();
@@ -318,7 +335,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     };
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
         }
@@ -354,7 +371,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     // The routing tables are older than the launch before this one, which has
     // passed its own wait by the time this one starts; only that launch's
     // output (the token pieces) has to be waited for, by the warps that read it.
-    const int n_active = max(0, min(__ldcg(args.active), min(args.experts, kMx4MaxActive)));
+    const int n_active = max(0, min(__ldcg(args.active), args.table));
     for (int i = static_cast<int>(threadIdx.x); i < n_active; i += kMx4Threads) {
         const int e = __ldcg(args.active + 1 + i);
         const int seg0 = __ldcg(args.offsets + e);
@@ -467,14 +484,14 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                         bulk_load(ss + kMx4SfBytes, sf + static_cast<int64_t>(b1 + kb) * kMx4SfBytes, kMx4SfBytes,
                                   &full_bar[stage]);
                     }
-                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                    if (++stage == stages) { stage = 0; phase ^= 1u; }
                 }
             }
             // PAIR: every stage's last release (a commit of rank 0) has landed before
             // this CTA's shared memory can go away
-            for (int i = 0; PAIR && i < S::kStages && ok; ++i) {
+            for (int i = 0; PAIR && i < stages && ok; ++i) {
                 ok = wait(&empty_bar[stage], phase ^ 1u);
-                if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                if (++stage == stages) { stage = 0; phase ^= 1u; }
             }
         }
         __syncwarp();
@@ -497,14 +514,14 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                         if (!SWIGLU)
                             tma_load_2d_pair(s_sf + stage * S::kSf + 2 * kMx4SfBytes, &tm_xs, fb, 0,
                                              static_cast<int>(tt * nkb + kb));
-                        if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                        if (++stage == stages) { stage = 0; phase ^= 1u; }
                         continue;
                     }
                     tma_load_3d(smem + stage * S::kStage + S::kA, &tm_x, &full_bar[stage], kb * kMx4BK, row, 0);
                     if (!SWIGLU)
                         bulk_load(s_sf + stage * S::kSf + 2 * kMx4SfBytes, args.sf + (tt * nkb + kb) * kMx4SfBytes,
                                   kMx4SfBytes, &full_bar[stage]);
-                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                    if (++stage == stages) { stage = 0; phase ^= 1u; }
                 }
             }
         }
@@ -556,7 +573,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     commit(&empty_bar[stage]);
                 }
                 __syncwarp();
-                if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                if (++stage == stages) { stage = 0; phase ^= 1u; }
             }
             if (!ok) break;
             if (elect_one()) commit(&tmem_full[b]);
@@ -568,6 +585,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         const int q = warp & 3;                                  // TMEM lane quadrant
         const int half = (warp - 2) >> 2;                        // this warp's chunks: half, half + 2, ...
         const int i_row = q * 32 + static_cast<int>(lane);
+        unsigned char* out = s_out + (warp - 2) * kMx4StageOut;
         float rs[(NT + 31) / 32];                                // factor of the tile's row 32 i + lane (SWIGLU)
         // Token columns [c0, c0 + n), n <= 8, of a tile: the sums g of the first, u of the second 128 weight rows.
         auto finish = [&](const Tile& t, int c0, int n, float (&g)[kMx4Chunk], float (&u)[kMx4Chunk]) {
@@ -580,8 +598,6 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                 for (int i = 0; i < (NT + 31) / 32; ++i)
                     if (c0 / 32 == i) factor = rs[i];
                 uint32_t byte = 0;                               // lane j: scale byte of column j
-                uint8_t* at = args.h + p0 * args.M + part * 128 + i_row;
-                const int64_t lo_at = static_cast<int64_t>(args.rows) * args.M;
                 uint32_t top[kMx4Chunk];
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) {
@@ -597,19 +613,23 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     g[j] *= mx4_inverse(by);
                     if (static_cast<int>(lane) == j) byte = by;
                 }
+                // [column][piece][32 rows] bytes in shared memory, out as 16 bytes a lane
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; j += 2) {
                     uint16_t hi, lo;
                     e4m3_split2(g[j], g[j + 1], hi, lo);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (j + i < n) {
-                            at[0] = static_cast<uint8_t>(hi >> (8 * i));
-                            at[lo_at] = static_cast<uint8_t>(lo >> (8 * i));
-                        }
-                        at += args.M;
-                    }
+                    out[64 * j + lane] = static_cast<uint8_t>(hi);
+                    out[64 * j + 32 + lane] = static_cast<uint8_t>(lo);
+                    out[64 * j + 64 + lane] = static_cast<uint8_t>(hi >> 8);
+                    out[64 * j + 96 + lane] = static_cast<uint8_t>(lo >> 8);
                 }
+                __syncwarp();
+                const int j = static_cast<int>(lane) >> 2, piece = (static_cast<int>(lane) >> 1) & 1;
+                if (j < n)
+                    *reinterpret_cast<uint4*>(args.h + (piece * static_cast<int64_t>(args.rows) + p0 + j) * args.M +
+                                              part * 128 + q * 32 + (lane & 1) * 16) =
+                        *reinterpret_cast<const uint4*>(out + 16 * lane);
+                __syncwarp();
                 if (lane < kMx4Chunk) {
                     const int r = c0 + static_cast<int>(lane);   // row of the token tile
                     const int64_t tt = prefix[t.a] / m_tiles + t.nb;
@@ -618,14 +638,21 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     if (S::kStack) sf[((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4] = static_cast<uint8_t>(byte);
                 }
             } else {
-                const int col = part * 256 + i_row;
-                uint16_t* at = args.y + p0 * args.ldy + col;
+                // [column][32 rows] BF16 in shared memory, out as 16 bytes a lane
+                const int col = part * 256 + q * 32;             // H is a multiple of 32: all lanes in or out
+                uint16_t* out16 = reinterpret_cast<uint16_t*>(out);
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) {
-                    if (j < n && col < args.ldy) at[0] = f2bits(g[j]);
-                    if (j < n && col + 128 < args.ldy) at[128] = f2bits(u[j]);
-                    at += args.ldy;
+                    out16[32 * j + lane] = f2bits(g[j]);
+                    out16[256 + 32 * j + lane] = f2bits(u[j]);
                 }
+                __syncwarp();
+                const int j = static_cast<int>(lane) >> 2;
+                uint16_t* at = args.y + (p0 + j) * args.ldy + col + (lane & 3) * 8;
+                if (j < n && col < args.ldy) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(out + 16 * lane);
+                if (j < n && col + 128 < args.ldy)
+                    *reinterpret_cast<uint4*>(at + 128) = *reinterpret_cast<const uint4*>(out + 512 + 16 * lane);
+                __syncwarp();
             }
         };
         auto release = [&](int b) {                              // this warp has read accumulator b

@@ -204,9 +204,9 @@ int device_setup(int* sms_out) {
 #undef PDX_DEC_ATTR
 #define PDX_MX4_ATTR(NT, PAIR)                                                                                     \
     PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, true, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,     \
-                                      static_cast<int>(Mx4Shape<NT, PAIR>::kSmem)));                               \
+                                      kMx4SmemLimit));                                                             \
     PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, false, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,    \
-                                      static_cast<int>(Mx4Shape<NT, PAIR>::kSmem)))
+                                      kMx4SmemLimit))
         PDX_MX4_ATTR(16, false); PDX_MX4_ATTR(32, false); PDX_MX4_ATTR(64, false); PDX_MX4_ATTR(112, true);
 #undef PDX_MX4_ATTR
         g_num_sms[dev] = sms;
@@ -1055,9 +1055,11 @@ struct Mx4Maps {
 
 // The two products on tiles of NT tokens; PAIR: as clusters of two CTAs.
 template <int NT, bool PAIR>
-int launch_mx4_products(const Mx4Maps& m, const Mx4Args& gu, const Mx4Args& down, int64_t tiles, int sms,
+int launch_mx4_products(const Mx4Maps& m, Mx4Args gu, Mx4Args down, int64_t tiles, int sms,
                         cudaStream_t stream) {
+    using S = Mx4Shape<NT, PAIR>;
     constexpr int64_t ctas = PAIR ? 2 : 1;
+    gu.stages = down.stages = S::stages(gu.table);
     const int64_t most = std::min(sms, kPlanSMs) / ctas;   // the partial sums are sized for kPlanSMs CTAs
     const int64_t work1 = tiles * ((gu.M / 128 + ctas - 1) / ctas) * (gu.K / kMx4BK);
     const int64_t work2 = tiles * ((down.M / 128 + 2 * ctas - 1) / (2 * ctas)) * (down.K / kMx4BK);
@@ -1065,7 +1067,7 @@ int launch_mx4_products(const Mx4Maps& m, const Mx4Args& gu, const Mx4Args& down
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(ctas * std::min(most, work)));
         cfg.blockDim = dim3(kMx4Threads);
-        cfg.dynamicSmemBytes = Mx4Shape<NT, PAIR>::kSmem;
+        cfg.dynamicSmemBytes = S::smem(a.table);
         cfg.stream = stream;
         cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1109,12 +1111,32 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
                            dim3(kMx4SplitWarps * 32), 0, stream, static_cast<const uint16_t*>(x), tokens,
                            static_cast<int>(T), n, static_cast<int>(H), Hp, b.x, b.row_scale, b.tickets,
                            static_cast<int>(b.words1 + b.words2)));
-    const uint8_t* scales = static_cast<const uint8_t*>(w->scales);
-    Mx4Args gu{offsets, active, w->slot_of_expert, slots, scales, ss, tps, 0, per, Hp, Ip, n, static_cast<int>(E),
-               b.row_scale, b.sf, b.h, nullptr, 0, b.partials, b.tickets};
-    Mx4Args down{offsets, active, w->slot_of_expert, slots, scales, ss, tps, 2 * per, 0, Ip, Hp, n,
-                 static_cast<int>(E), nullptr, b.sf, nullptr, static_cast<uint16_t*>(y), static_cast<int>(H),
-                 b.partials, b.tickets + b.words1};
+    Mx4Args gu{};
+    gu.offsets = offsets;
+    gu.active = active;
+    gu.slot_of_expert = w->slot_of_expert;
+    gu.num_slots = slots;
+    gu.scales = static_cast<const uint8_t*>(w->scales);
+    gu.scale_stride = ss;
+    gu.tiles_per_slot = tps;
+    gu.rows = n;
+    gu.table = static_cast<int>(std::min(E, rows));
+    gu.row_scale = b.row_scale;
+    gu.sf = b.sf;
+    gu.h = b.h;
+    gu.y = static_cast<uint16_t*>(y);
+    gu.ldy = static_cast<int>(H);
+    gu.partials = b.partials;
+    Mx4Args down = gu;
+    gu.tile0 = 0;
+    gu.tile1 = per;
+    gu.K = Hp;
+    gu.M = Ip;
+    gu.tickets = b.tickets;
+    down.tile0 = 2 * per;
+    down.K = Ip;
+    down.M = Hp;
+    down.tickets = b.tickets + b.words1;
     if (b.nt == 16) return launch_mx4_products<16, false>(m, gu, down, b.tiles, sms, stream);
     if (b.nt == 32) return launch_mx4_products<32, false>(m, gu, down, b.tiles, sms, stream);
     if (b.nt == 64) return launch_mx4_products<64, false>(m, gu, down, b.tiles, sms, stream);
@@ -1216,6 +1238,7 @@ int layer_rows(const void* x, const void* gate, int64_t T, int64_t H, int64_t E,
     const int64_t N = T * top_k;
     const int m = w4 ? PDX_FFN_AUTO : resolve_mode(mode, N, E, H, I);
     if (w4) {
+        if (reinterpret_cast<uintptr_t>(x) & 15u) return fail(PDX_ERR_INVALID, "x must be 16-byte aligned");
         if ((st = check_mx4_ffn(T, N, E, H, I, true, w4))) return st;
     } else {
         if ((st = check_ffn_shape(H, I, m))) return st;
@@ -1586,6 +1609,8 @@ int pdx_mxfp4_ffn_grouped(const void* x, int64_t T, const int32_t* tokens, const
                           int64_t H, int64_t I, void* y_out, void* workspace, size_t workspace_bytes,
                           pdx_stream_t stream) {
     if (!x || !offsets || !active || !y_out) return fail(PDX_ERR_INVALID, "null FFN argument");
+    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y_out)) & 15u)
+        return fail(PDX_ERR_INVALID, "x and y must be 16-byte aligned");
     int st = check_mx4_ffn(T, rows, E, H, I, tokens != nullptr, weights);
     if (st) return st;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1)))
