@@ -28,9 +28,9 @@
 // of which every CTA takes an equal share, so a decode step of any batch keeps
 // every SM streaming; a tile that spans CTAs is summed in CTA order by the warp
 // that takes its last ticket (FP32, deterministic, nothing waits).
-// Roles (352 threads): warp 0 streams weights and scales, warp 10 the token
-// pieces, warp 1 issues the MMAs, warps 2..9 are the epilogue (32 weight rows,
-// = one scale block of h, and every other 8 token columns each).  Neither launch waits for another CTA; the
+// Roles: warp 0 streams weights and scales, the last warp the token pieces, warp
+// 1 issues the MMAs, the others are the epilogue (32 weight rows, = one scale
+// block of h, and every second or fourth 8 token columns each).  Neither launch waits for another CTA; the
 // weight stream of a launch starts before the launch before it has finished.
 #include <cuda.h>
 
@@ -40,8 +40,7 @@
 
 namespace pdx {
 
-constexpr int kMx4Threads = 352;
-constexpr int kMx4EpiWarps = 8;
+constexpr int kMx4MaxEpi = 16;                      // epilogue warps at most
 constexpr int kMx4Chunk = 8;                        // token columns an epilogue warp takes at a time
 constexpr int kMx4BK = 128;                         // K step: 4 MMAs of 32
 constexpr uint32_t kMx4ABytes = 128 * kMx4BK;       // one weight tile, a byte per code
@@ -182,8 +181,18 @@ struct Mx4Args {
     int ldy;                        // H
     int stages, table;              // ring stages, entries of the expert tables (mx4_layout)
     float* partials;                // [gridDim.x][2][columns][128]
-    unsigned int* tickets;          // [tiles * kMx4EpiWarps], zero on entry
+    unsigned int* tickets;          // [tiles * CTAs of a tile * epilogue warps], zero on entry
 };
+
+// Four words of four bytes, transposed: byte i of the words -> out[i].
+__device__ __forceinline__ void turn_bytes(const uint4& w, uint32_t (&out)[4]) {
+    const uint32_t a = __byte_perm(w.x, w.y, 0x5140), b = __byte_perm(w.z, w.w, 0x5140);
+    const uint32_t c = __byte_perm(w.x, w.y, 0x7362), d = __byte_perm(w.z, w.w, 0x7362);
+    out[0] = __byte_perm(a, b, 0x5410);
+    out[1] = __byte_perm(a, b, 0x7632);
+    out[2] = __byte_perm(c, d, 0x5410);
+    out[3] = __byte_perm(c, d, 0x7632);
+}
 
 // One more of the parts of a tile is stored: the parts written before it (by the
 // lanes of this warp, behind __syncwarp) are visible to whoever sees the count.
@@ -276,7 +285,12 @@ struct Mx4Shape {
     static constexpr uint32_t kB = 2 * kBRows * kMx4BK;
     static constexpr uint32_t kStage = kA + kB;                     // multiple of 1024
     static constexpr uint32_t kSf = 3 * kMx4SfBytes;                // both weight halves | tokens
-    static constexpr uint32_t kFixed = 1024 + 512 + 512 + kMx4EpiWarps * kMx4StageOut;   // alignment, ones, barriers, staging
+    // Eight columns take an epilogue warp 1000 (down) to 2000 cycles (SwiGLU), mostly
+    // latency.  Wide tiles have 14 such pieces to 6 K steps of MMAs (5600 cycles at
+    // NT = 112), so they take 16 warps; narrow ones keep the ring stage instead.
+    static constexpr int kEpi = NT >= 64 ? 16 : 8;
+    static constexpr int kThreads = 32 * (kEpi + 3);
+    static constexpr uint32_t kFixed = 1024 + 512 + 512 + kEpi * kMx4StageOut;   // alignment, ones, barriers, staging
     // Ring stages beside tables of `entries` experts, and the shared memory of both.
     static constexpr int stages(int entries) {
         return static_cast<int>((kMx4SmemLimit - kFixed - 16u * entries) / (kStage + kSf));
@@ -295,11 +309,12 @@ struct Mx4Shape {
 // leaves room for a fourth stage at NT = 112.  Rank 0's full barriers count the
 // bytes of both CTAs; rank 0 commits to the empty and TMEM barriers of both.
 template <int NT, bool SWIGLU, bool PAIR>
-__global__ void __launch_bounds__(kMx4Threads, 1)
+__global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
     k_mx4_gemm(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                const __grid_constant__ CUtensorMap tm_ws, const __grid_constant__ CUtensorMap tm_xs, Mx4Args args) {
     using S = Mx4Shape<NT, PAIR>;
     constexpr int kCtas = PAIR ? 2 : 1;
+    constexpr int kColStep = S::kEpi / 4 * kMx4Chunk;        // columns between an epilogue warp's chunks
     extern __shared__ __align__(1024) unsigned char smem_mx4[];
     unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
     const int stages = args.stages;
@@ -314,7 +329,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_misc = reinterpret_cast<int*>(tmem_slot + 2);
     unsigned char* s_out = s_one + 1024;                             // an epilogue warp's staging: kMx4StageOut
-    int* prefix = reinterpret_cast<int*>(s_out + kMx4EpiWarps * kMx4StageOut);   // tiles before an active expert
+    int* prefix = reinterpret_cast<int*>(s_out + S::kEpi * kMx4StageOut);   // tiles before an active expert
     int* t_seg0 = prefix + args.table;
     int* t_rows = t_seg0 + args.table;
     int* t_slot = t_rows + args.table;
@@ -341,7 +356,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tmem_full[b], 1);
-            mbar_init(&tmem_empty[b], kCtas * kMx4EpiWarps);
+            mbar_init(&tmem_empty[b], kCtas * S::kEpi);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -365,14 +380,14 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
         }
     }
     if (warp >= 3)
-        for (int i = static_cast<int>(threadIdx.x) - 96; i < 128; i += kMx4Threads - 96)
+        for (int i = static_cast<int>(threadIdx.x) - 96; i < 128; i += S::kThreads - 96)
             reinterpret_cast<uint32_t*>(s_one)[i] = 0x7F7F7F7Fu;
     fence_proxy_async_smem();
     // The routing tables are older than the launch before this one, which has
     // passed its own wait by the time this one starts; only that launch's
     // output (the token pieces) has to be waited for, by the warps that read it.
     const int n_active = max(0, min(__ldcg(args.active), args.table));
-    for (int i = static_cast<int>(threadIdx.x); i < n_active; i += kMx4Threads) {
+    for (int i = static_cast<int>(threadIdx.x); i < n_active; i += S::kThreads) {
         const int e = __ldcg(args.active + 1 + i);
         const int seg0 = __ldcg(args.offsets + e);
         int64_t slot = args.slot_of_expert ? __ldcg(args.slot_of_expert + e) : e;
@@ -495,7 +510,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 2 + kMx4EpiWarps) {
+    } else if (warp == 2 + S::kEpi) {
         // ---------------- token producer ----------------
         griddep_wait();
         griddep_launch();
@@ -580,12 +595,12 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             __syncwarp();
         }
     } else if (warp >= 2) {
-        // ---------------- epilogue (warps 2..9) ----------------
+        // ---------------- epilogue (S::kEpi warps from 2) ----------------
         griddep_wait();
         const int q = warp & 3;                                  // TMEM lane quadrant
-        const int half = (warp - 2) >> 2;                        // this warp's chunks: half, half + 2, ...
+        const int col0 = ((warp - 2) >> 2) * kMx4Chunk;          // first columns of this warp
         const int i_row = q * 32 + static_cast<int>(lane);
-        unsigned char* out = s_out + (warp - 2) * kMx4StageOut;
+        uint32_t* out = reinterpret_cast<uint32_t*>(s_out + (warp - 2) * kMx4StageOut);
         float rs[(NT + 31) / 32];                                // factor of the tile's row 32 i + lane (SWIGLU)
         // Token columns [c0, c0 + n), n <= 8, of a tile: the sums g of the first, u of the second 128 weight rows.
         auto finish = [&](const Tile& t, int c0, int n, float (&g)[kMx4Chunk], float (&u)[kMx4Chunk]) {
@@ -613,22 +628,32 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     g[j] *= mx4_inverse(by);
                     if (static_cast<int>(lane) == j) byte = by;
                 }
-                // [column][piece][32 rows] bytes in shared memory, out as 16 bytes a lane
+                // One word per weight row and 4 columns, [4 columns][piece][32 rows]; then half the
+                // lanes take 8 rows of 4 columns of a piece, turn them and store 8 bytes a column.
 #pragma unroll
-                for (int j = 0; j < kMx4Chunk; j += 2) {
-                    uint16_t hi, lo;
-                    e4m3_split2(g[j], g[j + 1], hi, lo);
-                    out[64 * j + lane] = static_cast<uint8_t>(hi);
-                    out[64 * j + 32 + lane] = static_cast<uint8_t>(lo);
-                    out[64 * j + 64 + lane] = static_cast<uint8_t>(hi >> 8);
-                    out[64 * j + 96 + lane] = static_cast<uint8_t>(lo >> 8);
+                for (int j = 0; j < kMx4Chunk; j += 4) {
+                    uint16_t h0, h1, l0, l1;
+                    e4m3_split2(g[j], g[j + 1], h0, l0);
+                    e4m3_split2(g[j + 2], g[j + 3], h1, l1);
+                    out[16 * j + lane] = h0 | (static_cast<uint32_t>(h1) << 16);
+                    out[16 * j + 32 + lane] = l0 | (static_cast<uint32_t>(l1) << 16);
                 }
                 __syncwarp();
-                const int j = static_cast<int>(lane) >> 2, piece = (static_cast<int>(lane) >> 1) & 1;
-                if (j < n)
-                    *reinterpret_cast<uint4*>(args.h + (piece * static_cast<int64_t>(args.rows) + p0 + j) * args.M +
-                                              part * 128 + q * 32 + (lane & 1) * 16) =
-                        *reinterpret_cast<const uint4*>(out + 16 * lane);
+                if (lane < 16) {
+                    const int j = (static_cast<int>(lane) >> 3) * 4, piece = (static_cast<int>(lane) >> 2) & 1;
+                    const uint4 w0 = reinterpret_cast<const uint4*>(out)[2 * lane];
+                    const uint4 w1 = reinterpret_cast<const uint4*>(out)[2 * lane + 1];
+                    uint32_t a[4], b[4];
+                    turn_bytes(w0, a);
+                    turn_bytes(w1, b);
+                    uint8_t* at = args.h + (piece * static_cast<int64_t>(args.rows) + p0 + j) * args.M + part * 128 +
+                                  q * 32 + (lane & 3) * 8;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (j + i < n) *reinterpret_cast<uint2*>(at) = make_uint2(a[i], b[i]);
+                        at += args.M;
+                    }
+                }
                 __syncwarp();
                 if (lane < kMx4Chunk) {
                     const int r = c0 + static_cast<int>(lane);   // row of the token tile
@@ -638,20 +663,27 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     if (S::kStack) sf[((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4] = static_cast<uint8_t>(byte);
                 }
             } else {
-                // [column][32 rows] BF16 in shared memory, out as 16 bytes a lane
+                // One word per weight row and 2 columns, [half][2 columns][32 rows]; then every
+                // lane takes 8 rows of 2 columns, turns them and stores 16 bytes a column.
                 const int col = part * 256 + q * 32;             // H is a multiple of 32: all lanes in or out
-                uint16_t* out16 = reinterpret_cast<uint16_t*>(out);
 #pragma unroll
-                for (int j = 0; j < kMx4Chunk; ++j) {
-                    out16[32 * j + lane] = f2bits(g[j]);
-                    out16[256 + 32 * j + lane] = f2bits(u[j]);
+                for (int j = 0; j < kMx4Chunk; j += 2) {
+                    out[16 * j + lane] = f2bits(g[j]) | (static_cast<uint32_t>(f2bits(g[j + 1])) << 16);
+                    out[128 + 16 * j + lane] = f2bits(u[j]) | (static_cast<uint32_t>(f2bits(u[j + 1])) << 16);
                 }
                 __syncwarp();
-                const int j = static_cast<int>(lane) >> 2;
-                uint16_t* at = args.y + (p0 + j) * args.ldy + col + (lane & 3) * 8;
-                if (j < n && col < args.ldy) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(out + 16 * lane);
-                if (j < n && col + 128 < args.ldy)
-                    *reinterpret_cast<uint4*>(at + 128) = *reinterpret_cast<const uint4*>(out + 512 + 16 * lane);
+                const int c8 = col + (static_cast<int>(lane) >> 4) * 128, j = (static_cast<int>(lane) >> 2 & 3) * 2;
+                const uint4 w0 = reinterpret_cast<const uint4*>(out)[2 * lane];
+                const uint4 w1 = reinterpret_cast<const uint4*>(out)[2 * lane + 1];
+                uint16_t* at = args.y + (p0 + j) * args.ldy + c8 + (lane & 3) * 8;
+                if (j < n && c8 < args.ldy)
+                    *reinterpret_cast<uint4*>(at) =
+                        make_uint4(__byte_perm(w0.x, w0.y, 0x5410), __byte_perm(w0.z, w0.w, 0x5410),
+                                   __byte_perm(w1.x, w1.y, 0x5410), __byte_perm(w1.z, w1.w, 0x5410));
+                if (j + 1 < n && c8 < args.ldy)
+                    *reinterpret_cast<uint4*>(at + args.ldy) =
+                        make_uint4(__byte_perm(w0.x, w0.y, 0x7632), __byte_perm(w0.z, w0.w, 0x7632),
+                                   __byte_perm(w1.x, w1.y, 0x7632), __byte_perm(w1.z, w1.w, 0x7632));
                 __syncwarp();
             }
         };
@@ -683,7 +715,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             // last tile (slot 1), every other part its CTA's first (slot 0)
             float* mine = args.partials +
                           (static_cast<int64_t>(blockIdx.x) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
-            for (int c = half * kMx4Chunk; c < ne; c += 2 * kMx4Chunk) {
+            for (int c = col0; c < ne; c += kColStep) {
                 const int n = min(kMx4Chunk, ne - c);
                 uint32_t r[4][kMx4Chunk];
                 tmem_ld8(taddr + c, r[0]);
@@ -693,7 +725,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                     tmem_ld8(taddr + S::kN + NT + c, r[3]);
                 }
                 tmem_wait_ld();
-                if (c + 2 * kMx4Chunk >= ne) {                   // this warp's last columns are read
+                if (c + kColStep >= ne) {                   // this warp's last columns are read
                     release(b);
                 }
                 float g[kMx4Chunk], u[kMx4Chunk];
@@ -713,7 +745,7 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
                         }
                 }
             }
-            if (half * kMx4Chunk >= ne) {
+            if (col0 >= ne) {
                 release(b);
             }
             if (whole) continue;
@@ -723,10 +755,10 @@ __global__ void __launch_bounds__(kMx4Threads, 1)
             const int c_last = static_cast<int>(((last + 1) * shares - 1) / work);
             __syncwarp();
             unsigned int prev = 0;
-            if (lane == 0) prev = ticket_acq_rel(&args.tickets[(t.index * kCtas + rank) * kMx4EpiWarps + warp - 2]);
+            if (lane == 0) prev = ticket_acq_rel(&args.tickets[(t.index * kCtas + rank) * S::kEpi + warp - 2]);
             prev = __shfl_sync(0xffffffffu, prev, 0);
             if (prev != static_cast<unsigned int>(c_last - c_first)) continue;
-            for (int col = half * kMx4Chunk; col < ne; col += 2 * kMx4Chunk) {
+            for (int col = col0; col < ne; col += kColStep) {
                 const int n = min(kMx4Chunk, ne - col);
                 float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll

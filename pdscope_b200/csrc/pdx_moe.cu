@@ -990,8 +990,8 @@ Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
     b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * kMx4SfBytes));
     b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * 2 * b.nt * 128 * 4));
     // a ticket per tile, CTA of a pair and epilogue warp; pairs round the tiles of 256 rows up to even
-    b.words1 = b.tiles * ((Ip / 128 + 1) / 2 * 2) * kMx4EpiWarps;
-    b.words2 = b.tiles * ((Hp + 511) / 512 * 2) * kMx4EpiWarps;
+    b.words1 = b.tiles * ((Ip / 128 + 1) / 2 * 2) * kMx4MaxEpi;
+    b.words2 = b.tiles * ((Hp + 511) / 512 * 2) * kMx4MaxEpi;
     b.tickets = static_cast<unsigned int*>(c.take((b.words1 + b.words2) * 4));
     return b;
 }
@@ -1066,7 +1066,7 @@ int launch_mx4_products(const Mx4Maps& m, Mx4Args gu, Mx4Args down, int64_t tile
     auto launch = [&](auto kernel, int64_t work, const CUtensorMap& tokens, const Mx4Args& a) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(ctas * std::min(most, work)));
-        cfg.blockDim = dim3(kMx4Threads);
+        cfg.blockDim = dim3(S::kThreads);
         cfg.dynamicSmemBytes = S::smem(a.table);
         cfg.stream = stream;
         cudaLaunchAttribute attr[2];
