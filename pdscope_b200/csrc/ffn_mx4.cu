@@ -152,8 +152,8 @@ __global__ void __launch_bounds__(kMx4SplitWarps * 32, 7)
                 h[i] = h0 | (static_cast<uint32_t>(h1) << 16);
                 l[i] = l0 | (static_cast<uint32_t>(l1) << 16);
             }
-            hi_row[c] = make_uint4(h[0], h[1], h[2], h[3]);
-            lo_row[c] = make_uint4(l[0], l[1], l[2], l[3]);
+            __stcs(hi_row + c, make_uint4(h[0], h[1], h[2], h[3]));   // streaming: x stays in L2
+            __stcs(lo_row + c, make_uint4(l[0], l[1], l[2], l[3]));
         };
 #pragma unroll
         for (int j = 0; j < kMx4SplitHeld; ++j)
@@ -600,6 +600,9 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
         const int q = warp & 3;                                  // TMEM lane quadrant
         const int col0 = ((warp - 2) >> 2) * kMx4Chunk;          // first columns of this warp
         const int i_row = q * 32 + static_cast<int>(lane);
+        // Staged words are read 32 bytes a lane; in every second group of 32 words the
+        // 16-byte halves change places, so eight lanes read eight different bank groups.
+        const uint32_t turn = lane >> 2 & 1u;
         uint32_t* out = reinterpret_cast<uint32_t*>(s_out + (warp - 2) * kMx4StageOut);
         float rs[(NT + 31) / 32];                                // factor of the tile's row 32 i + lane (SWIGLU)
         // Token columns [c0, c0 + n), n <= 8, of a tile: the sums g of the first, u of the second 128 weight rows.
@@ -636,13 +639,13 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
                     e4m3_split2(g[j], g[j + 1], h0, l0);
                     e4m3_split2(g[j + 2], g[j + 3], h1, l1);
                     out[16 * j + lane] = h0 | (static_cast<uint32_t>(h1) << 16);
-                    out[16 * j + 32 + lane] = l0 | (static_cast<uint32_t>(l1) << 16);
+                    out[16 * j + 32 + (lane ^ 4)] = l0 | (static_cast<uint32_t>(l1) << 16);   // see turn
                 }
                 __syncwarp();
                 if (lane < 16) {
                     const int j = (static_cast<int>(lane) >> 3) * 4, piece = (static_cast<int>(lane) >> 2) & 1;
-                    const uint4 w0 = reinterpret_cast<const uint4*>(out)[2 * lane];
-                    const uint4 w1 = reinterpret_cast<const uint4*>(out)[2 * lane + 1];
+                    const uint4 w0 = reinterpret_cast<const uint4*>(out)[2 * lane ^ turn];
+                    const uint4 w1 = reinterpret_cast<const uint4*>(out)[(2 * lane + 1) ^ turn];
                     uint32_t a[4], b[4];
                     turn_bytes(w0, a);
                     turn_bytes(w1, b);
@@ -668,13 +671,14 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
                 const int col = part * 256 + q * 32;             // H is a multiple of 32: all lanes in or out
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; j += 2) {
-                    out[16 * j + lane] = f2bits(g[j]) | (static_cast<uint32_t>(f2bits(g[j + 1])) << 16);
-                    out[128 + 16 * j + lane] = f2bits(u[j]) | (static_cast<uint32_t>(f2bits(u[j + 1])) << 16);
+                    const uint32_t at = 16 * j + (lane ^ (j & 2 ? 4u : 0u));                  // see turn
+                    out[at] = f2bits(g[j]) | (static_cast<uint32_t>(f2bits(g[j + 1])) << 16);
+                    out[128 + at] = f2bits(u[j]) | (static_cast<uint32_t>(f2bits(u[j + 1])) << 16);
                 }
                 __syncwarp();
                 const int c8 = col + (static_cast<int>(lane) >> 4) * 128, j = (static_cast<int>(lane) >> 2 & 3) * 2;
-                const uint4 w0 = reinterpret_cast<const uint4*>(out)[2 * lane];
-                const uint4 w1 = reinterpret_cast<const uint4*>(out)[2 * lane + 1];
+                const uint4 w0 = reinterpret_cast<const uint4*>(out)[2 * lane ^ turn];
+                const uint4 w1 = reinterpret_cast<const uint4*>(out)[(2 * lane + 1) ^ turn];
                 uint16_t* at = args.y + (p0 + j) * args.ldy + c8 + (lane & 3) * 8;
                 if (j < n && c8 < args.ldy)
                     *reinterpret_cast<uint4*>(at) =
