@@ -78,20 +78,20 @@ __device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint
 // Token rows in packed order as E4M3 pieces: out [2][rows][Hp] (hi rows, then lo
 // rows, zero past H) and the row's factor 2^(b - 127).  HBM-bound (the pieces
 // are written once, x comes from L2).  A group of WARPS warps takes a row, 16
-// values a lane at a time; up to kMx4SplitHeld of those stay in registers
-// between finding the row's largest value and splitting, longer rows are read
-// again.  One warp a row for many rows, four for few, where the trip to memory
+// values a lane at a time; the first four (four warps: two) of those stay in
+// registers between finding the row's largest value and splitting, longer rows
+// are read again.  One warp a row for many rows, four for few, where the trip to memory
 // is what a row costs.  The kernel also clears the tickets of the two products
 // that follow.
 constexpr int kMx4SplitWarps = 4;     // warps per CTA
-constexpr int kMx4SplitHeld = 4;
 template <int WARPS>
-__global__ void __launch_bounds__(kMx4SplitWarps * 32, 7)
+__global__ void __launch_bounds__(kMx4SplitWarps * 32, WARPS == 1 ? 7 : 12)
     k_mx4_split(const uint16_t* __restrict__ x, const int32_t* __restrict__ tokens, int T, int rows, int H, int Hp,
                 uint8_t* __restrict__ out, float* __restrict__ row_scale, unsigned int* __restrict__ zero_ptr,
                 int zero_words) {
     griddep_wait();
     griddep_launch();
+    constexpr int kMx4SplitHeld = WARPS == 1 ? 4 : 2;
     __shared__ uint32_t s_top[kMx4SplitWarps];
     for (int i = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x); i < zero_words;
          i += static_cast<int>(gridDim.x * blockDim.x))
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_misc = reinterpret_cast<int*>(tmem_slot + 2);
     unsigned char* s_out = s_one + 1024;                             // an epilogue warp's staging: kMx4StageOut
-    int* prefix = reinterpret_cast<int*>(s_out + S::kEpi * kMx4StageOut);   // tiles before an active expert
+    int* prefix = reinterpret_cast<int*>(s_out + S::kEpi * kMx4StageOut);   // token tiles before an active expert
     int* t_seg0 = prefix + args.table;
     int* t_rows = t_seg0 + args.table;
     int* t_slot = t_rows + args.table;
@@ -403,9 +403,8 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (warp == 2) {
-        const int total = warp_tile_prefix(n_active, prefix,
-                                           [&](int a) { return m_tiles * ((t_rows[a] + NT - 1) / NT); });
-        if (lane == 0) s_misc[0] = total;
+        const int total = warp_tile_prefix(n_active, prefix, [&](int a) { return (t_rows[a] + NT - 1) / NT; });
+        if (lane == 0) s_misc[0] = total * m_tiles;
     }
     __syncwarp();
     if (PAIR)
@@ -432,7 +431,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
     const int64_t w1 = cta < shares ? work * (cta + 1) / shares : 0;
 
     struct Tile {
-        int index, a, mt, nb, kb0, kb1;
+        int index, token, a, mt, nb, kb0, kb1;   // tile, its token tile, ...
         int64_t w;    // next step of the share
         int wave;     // next wave
     };
@@ -456,10 +455,10 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
         } else {
             return false;
         }
-        t.a = find_expert(prefix, n_active, t.index);
-        const int local = t.index - prefix[t.a];
-        t.nb = local / m_tiles;
-        t.mt = local - t.nb * m_tiles;
+        t.token = t.index / m_tiles;
+        t.mt = t.index - t.token * m_tiles;
+        t.a = find_expert(prefix, n_active, t.token);
+        t.nb = t.token - prefix[t.a];
         return true;
     };
 
@@ -520,7 +519,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
             bool ok = true;
             for (Tile t = begin(); ok && next(t);) {
                 const int row = t_seg0[t.a] + t.nb * NT + rank * S::kBRows;
-                const int64_t tt = prefix[t.a] / m_tiles + t.nb;
+                const int64_t tt = t.token;
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     if (!wait(&empty_bar[stage], phase ^ 1u)) { ok = false; break; }
                     if (PAIR) {
@@ -660,8 +659,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
                 __syncwarp();
                 if (lane < kMx4Chunk) {
                     const int r = c0 + static_cast<int>(lane);   // row of the token tile
-                    const int64_t tt = prefix[t.a] / m_tiles + t.nb;
-                    uint8_t* sf = args.sf + (tt * m_blocks + part) * kMx4SfBytes + q;
+                    uint8_t* sf = args.sf + (static_cast<int64_t>(t.token) * m_blocks + part) * kMx4SfBytes + q;
                     sf[(r & 31) * 16 + (r >> 5) * 4] = static_cast<uint8_t>(byte);
                     if (S::kStack) sf[((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4] = static_cast<uint8_t>(byte);
                 }

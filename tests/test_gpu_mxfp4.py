@@ -120,6 +120,8 @@ SHAPES = [  # tokens, hidden, inter, experts, top_k
     (1, 32, 32, 1, 1), (1, 128, 128, 4, 2), (1, 2048, 768, 16, 8), (2, 96, 160, 3, 3), (7, 256, 128, 8, 2),
     (16, 1056, 416, 6, 4), (33, 512, 96, 5, 1), (64, 384, 256, 24, 8), (65, 2048, 768, 4, 2), (129, 640, 288, 3, 2),
     (257, 256, 128, 2, 1), (300, 128, 1024, 9, 3), (1000, 256, 256, 4, 4),
+    # several tiles for every CTA or pair: narrow, middle and wide token tiles, odd numbers of 128-row blocks
+    (200, 640, 640, 120, 8), (380, 384, 1152, 100, 8), (600, 256, 1280, 100, 6), (4100, 1152, 896, 4, 2),
 ]
 
 
