@@ -14,9 +14,10 @@ _MXFP4_NAMES = ("Mxfp4", "Mxfp4ExpertSlab", "dequantize_mxfp4", "moe_ffn_mxfp4",
 
 def __getattr__(name):
     if name in _RUNTIME_NAMES:
-        from . import runtime
-        return getattr(runtime, name)
-    if name in _MXFP4_NAMES:
-        from . import mxfp4
-        return getattr(mxfp4, name)
-    raise AttributeError(name)
+        from . import runtime as module
+    elif name in _MXFP4_NAMES:
+        from . import mxfp4 as module
+    else:
+        raise AttributeError(name)
+    value = globals()[name] = getattr(module, name)   # later uses find it without this function
+    return value

@@ -1098,12 +1098,14 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     const int64_t tps = slots > 1 ? w->code_stride / kMx4TileBytes : 0;
     const bool pair = b.nt == kMx4PairTile;
     const int box = pair ? b.nt / 2 : b.nt;
-    Mx4Maps m;
+    Mx4Maps m{};
     if ((st = encode_mx4_weights(&m.w, w->codes, (slots - 1) * tps + 3 * per))) return st;
     if ((st = encode_mx4_tokens(&m.x, b.x, rows, Hp, box))) return st;
     if ((st = encode_mx4_tokens(&m.h, b.h, rows, Ip, box))) return st;
-    if ((st = encode_mx4_scales(&m.ws, w->scales, (slots - 1) * (ss / kMx4SfBytes) + 3 * per))) return st;
-    if ((st = encode_mx4_scales(&m.hs, b.sf, b.tiles * (Ip / 128)))) return st;
+    if (pair) {
+        if ((st = encode_mx4_scales(&m.ws, w->scales, (slots - 1) * (ss / kMx4SfBytes) + 3 * per))) return st;
+        if ((st = encode_mx4_scales(&m.hs, b.sf, b.tiles * (Ip / 128)))) return st;
+    }
     const bool few = rows <= kMx4SplitFew;
     const int64_t split_ctas = few ? rows : (rows + kMx4SplitWarps - 1) / kMx4SplitWarps;
     PDX_PDL_TRY(launch_pdl(few ? k_mx4_split<kMx4SplitWarps> : k_mx4_split<1>,

@@ -16,8 +16,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import Mxfp4Weights, check, lib
-from .runtime import PROJECTIONS, Packed, _on, _raw_stream, _require_cuda_bf16, ffn_workspace_bytes
+from ._lib import Mxfp4Weights, lib
+from .runtime import PROJECTIONS, Packed, _call, _require_cuda_bf16, ffn_workspace_bytes
 
 BLOCK = 32
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
@@ -57,9 +57,8 @@ def quantize_mxfp4(x):
     rows, cols, ld = _matrix(x)
     codes = x.new_empty((*shape[:-1], cols // 2), dtype=torch.uint8)
     scales = x.new_empty((*shape[:-1], cols // BLOCK), dtype=torch.uint8)
-    with _on(x.device):
-        check(lib.pdx_mxfp4_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, cols, ld, codes.data_ptr(),
-                                     scales.data_ptr(), _raw_stream(x.device)))
+    _call(x.device, lib.pdx_mxfp4_quantize, x.data_ptr(), _DTYPES[x.dtype], rows, cols, ld, codes.data_ptr(),
+          scales.data_ptr())
     return Mxfp4(codes, scales)
 
 
@@ -84,9 +83,8 @@ def dequantize_mxfp4(q, dtype=torch.bfloat16):
     shape = q.shape
     out = q.codes.new_empty(shape, dtype=dtype)
     cols = shape[-1]
-    with _on(out.device):
-        check(lib.pdx_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.numel() // cols, cols, cols,
-                                       _DTYPES[dtype], out.data_ptr(), _raw_stream(out.device)))
+    _call(out.device, lib.pdx_mxfp4_dequantize, q.codes.data_ptr(), q.scales.data_ptr(), out.numel() // cols, cols, cols,
+          _DTYPES[dtype], out.data_ptr())
     return out
 
 
@@ -220,11 +218,10 @@ def moe_ffn_mxfp4(x, packed, slab, out=None):
         _require_cuda_bf16("out", out, 2)
         if out.shape != (rows, hidden) or out.device != x.device:
             raise ValueError("out must be [T*k, H] on the device of x")
-    with _on(x.device):
-        # from the stream-ordered allocator: calls on two streams or in two graphs share no scratch
-        nbytes = ffn_workspace_bytes(slab, rows, experts)
-        ws = x.new_empty((nbytes,), dtype=torch.uint8)
-        check(lib.pdx_mxfp4_ffn_grouped(x.data_ptr(), t_count, packed.tokens.data_ptr(), packed.offsets.data_ptr(),
-                                        packed.active.data_ptr(), experts, rows, ctypes.byref(slab.struct), hidden,
-                                        slab.inter, out.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(x.device)))
+    # from the stream-ordered allocator: calls on two streams or in two graphs share no scratch
+    nbytes = ffn_workspace_bytes(slab, rows, experts)
+    ws = x.new_empty((nbytes,), dtype=torch.uint8)
+    _call(x.device, lib.pdx_mxfp4_ffn_grouped, x.data_ptr(), t_count, packed.tokens.data_ptr(),
+          packed.offsets.data_ptr(), packed.active.data_ptr(), experts, rows, ctypes.byref(slab.struct), hidden,
+          slab.inter, out.data_ptr(), ws.data_ptr(), nbytes)
     return out

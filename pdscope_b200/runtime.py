@@ -22,7 +22,6 @@ from __future__ import annotations
 import ctypes
 import hashlib
 from collections import Counter
-from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -41,14 +40,17 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
 
-def _raw_stream(device):
-    """Handle of ``device``'s current stream, as an int (``_stream`` of another device, without the Stream object)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _on(device):
-    """Context in which ``device`` is current."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _call(device, entry, *args):
+    """One C-ABI call on ``device``'s current stream (the last argument of every
+    entry point), with ``device`` current; raises on a bad status."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
 
 
 class _Workspace:
@@ -430,10 +432,8 @@ def block_norm(y, residual, *, norm=None, stream_out=None, out=None, **options):
         if y.shape != residual.shape or y.device != residual.device:
             raise ValueError("y and residual shapes differ")
     t_count, hidden = residual.shape
-    with _on(residual.device):
-        check(lib.pdx_block_norm(y.data_ptr() if y is not None else None, residual.data_ptr(), t_count, hidden,
-                                 ctypes.byref(args), stream_out.data_ptr(), out.data_ptr(),
-                                 _raw_stream(residual.device)))
+    _call(residual.device, lib.pdx_block_norm, y.data_ptr() if y is not None else None, residual.data_ptr(), t_count,
+          hidden, ctypes.byref(args), stream_out.data_ptr(), out.data_ptr())
     return stream_out, out
 
 
@@ -451,10 +451,8 @@ def combine_block_norm(rows, weights, inverse, residual, *, norm=None, stream_ou
     args, stream_out, out = _block_norm_outputs(norm, options, residual, stream_out, out, apart=rows)
     if residual.shape != (t_count, rows.shape[1]) or residual.device != device or weights.device != device:
         raise ValueError("residual must be [T, H] on the device of rows")
-    with _on(device):
-        check(lib.pdx_combine_block_norm(rows.data_ptr(), rows.shape[0], weights.data_ptr(), inverse.data_ptr(),
-                                         t_count, k, rows.shape[1], residual.data_ptr(), ctypes.byref(args),
-                                         stream_out.data_ptr(), out.data_ptr(), _raw_stream(device)))
+    _call(device, lib.pdx_combine_block_norm, rows.data_ptr(), rows.shape[0], weights.data_ptr(), inverse.data_ptr(),
+          t_count, k, rows.shape[1], residual.data_ptr(), ctypes.byref(args), stream_out.data_ptr(), out.data_ptr())
     return stream_out, out
 
 
