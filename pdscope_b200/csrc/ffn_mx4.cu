@@ -20,14 +20,12 @@
 // Two launches of k_mx4_gemm, each on tiles of 256 weight rows (two accumulators
 // over one token operand): 128 rows of gate and the same 128 of up with the
 // SwiGLU, then 256 rows of down.  Tokens are the N operand, NT packed rows of
-// one expert a tile; up to NT = 32 the two pieces are stacked along N (one pass
-// over the weights in shared memory), above that they accumulate into the same
-// columns.
-// Work is cut evenly: full waves of tiles go round robin (neighbouring CTAs share
-// a token tile in L2), and the (tile, K step) pairs of the rest form one sequence
-// of which every CTA takes an equal share, so a decode step of any batch keeps
-// every SM streaming; a tile that spans CTAs is summed in CTA order by the warp
-// that takes its last ticket (FP32, deterministic, nothing waits).
+// one expert a tile.  Narrow tiles (NT = 16, 32) stack the two pieces along N (one
+// pass over the weights in shared memory); wide ones (NT = 112, on pairs of CTAs)
+// accumulate both into the same columns.
+// Tiles go round robin over the CTAs, neighbours sharing a token tile in L2.  When
+// there are fewer tiles than CTAs their K is cut up; a tile's parts are added in
+// order by the warp that takes its last ticket (FP32, deterministic, nothing waits).
 // Roles: warp 0 streams weights and scales, the last warp the token pieces, warp
 // 1 issues the MMAs, the others are the epilogue (32 weight rows, = one scale
 // block of h, and every second or fourth 8 token columns each).  Neither launch waits for another CTA; the
@@ -180,7 +178,7 @@ struct Mx4Args {
     uint16_t* y;                    // [rows, ldy] (down)
     int ldy;                        // H
     int stages, table;              // ring stages, entries of the expert tables (mx4_layout)
-    float* partials;                // [gridDim.x][2][columns][128]
+    float* partials;                // [gridDim.x][2 NT][128]
     unsigned int* tickets;          // [tiles * CTAs of a tile * epilogue warps], zero on entry
 };
 
@@ -273,13 +271,14 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, ui
         : "memory");
 }
 
-template <int NT, bool PAIR>
+template <int NT>
 struct Mx4Shape {
-    static constexpr bool kStack = NT <= 32;                        // pieces side by side along N
+    static constexpr bool kPair = NT > 32;                          // two CTAs share a tile
+    static constexpr bool kStack = !kPair;                          // pieces side by side along N
     static constexpr int kN = kStack ? 2 * NT : NT;                 // N of one MMA
     static constexpr int kAcc = 2 * kN;                             // accumulator columns of a tile
     static constexpr int kCols = 2 * NT;                            // FP32 columns of a partial tile
-    static constexpr int kBRows = PAIR ? NT / 2 : NT;               // token rows a CTA stages
+    static constexpr int kBRows = kPair ? NT / 2 : NT;               // token rows a CTA stages
     static constexpr uint32_t kA = 2 * kMx4ABytes;
     static constexpr uint32_t kATx = kA / 2;                        // the copy counts the packed bytes it reads
     static constexpr uint32_t kB = 2 * kBRows * kMx4BK;
@@ -288,7 +287,7 @@ struct Mx4Shape {
     // Eight columns take an epilogue warp 1000 (down) to 2000 cycles (SwiGLU), mostly
     // latency.  Wide tiles have 14 such pieces to 6 K steps of MMAs (5600 cycles at
     // NT = 112), so they take 16 warps; narrow ones keep the ring stage instead.
-    static constexpr int kEpi = NT >= 64 ? 16 : 8;
+    static constexpr int kEpi = kPair ? 16 : 8;
     static constexpr int kThreads = 32 * (kEpi + 3);
     static constexpr uint32_t kFixed = 1024 + 512 + 512 + kEpi * kMx4StageOut;   // alignment, ones, barriers, staging
     // Ring stages beside tables of `entries` experts, and the shared memory of both.
@@ -297,23 +296,25 @@ struct Mx4Shape {
     }
     static constexpr size_t smem(int entries) { return kFixed + 16u * entries + stages(entries) * (kStage + kSf); }
     static constexpr int kMaxStages = stages(1);
-    static_assert(NT % 16 == 0 && kBRows % 8 == 0 && !(PAIR && kStack) && stages(kMx4MaxActive) >= 3 && 2 * kMaxStages + 5 <= 56 &&
+    static_assert(NT % 16 == 0 && kBRows % 8 == 0 && stages(kMx4MaxActive) >= 3 && 2 * kMaxStages + 5 <= 56 &&
                       2 * kAcc <= static_cast<int>(kMx4SfCol),
                   "token tile");
 };
 
-// PAIR: a cluster of two CTAs shares a tile of 512 weight rows (tcgen05
+// NT > 32: a cluster of two CTAs shares a tile of 512 weight rows (tcgen05
 // cta_group::2): each CTA stages its own 256 weight rows and half of the token
 // rows, rank 0 issues the MMAs for both, each CTA's TMEM holds the sums of its own
 // weight rows.  Token bytes from L2 and their shared memory are halved, which
 // leaves room for a fourth stage at NT = 112.  Rank 0's full barriers count the
 // bytes of both CTAs; rank 0 commits to the empty and TMEM barriers of both.
-template <int NT, bool SWIGLU, bool PAIR>
-__global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
+template <int NT, bool SWIGLU>
+__global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     k_mx4_gemm(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                const __grid_constant__ CUtensorMap tm_ws, const __grid_constant__ CUtensorMap tm_xs, Mx4Args args) {
-    using S = Mx4Shape<NT, PAIR>;
+    using S = Mx4Shape<NT>;
+    constexpr bool PAIR = S::kPair;
     constexpr int kCtas = PAIR ? 2 : 1;
+    constexpr int kJoin = PAIR ? 1 : 4;                      // parts in flight when a tile is joined
     constexpr int kColStep = S::kEpi / 4 * kMx4Chunk;        // columns between an epilogue warp's chunks
     extern __shared__ __align__(1024) unsigned char smem_mx4[];
     unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
@@ -414,52 +415,38 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
     const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full_bar), 0) : 0u;          // rank 0's barriers
     const uint32_t tmem_empty0 = PAIR ? mapa_shared(smem_u32(tmem_empty), 0) : 0u;
     const uint32_t tmem_base = *tmem_slot;
-    // CTA (or pair) c takes the whole tiles c, c + G, ... of the full waves of G tiles, and
-    // before them its share [w0, w1) of the (tile, K step) sequence of the rest
-    // (`work` steps), at least one step per sharing CTA, so every CTA between two
-    // sharers of a tile shares it too.  Without a full wave (a few tokens) joining
-    // the parts is what a shared tile costs, so a tile is cut into equal parts of
-    // at least kMx4MinPart steps or not at all: one token at H = 2048, I = 768, 8
-    // experts takes 48 gate/up tiles of 16 steps in 3 parts, 64 down tiles of 6 whole.
+    // CTA (or pair) c of G takes the tiles c, c + G, ...  When there are fewer tiles
+    // than CTAs (a few tokens), K is cut into `parts` equal parts of at least
+    // kMx4MinPart steps and CTA c takes part c % parts of tile c / parts: one token at
+    // H = 2048, I = 768, 8 experts has 48 gate/up tiles of 16 steps (3 parts) and 64
+    // down tiles of 6 (1 part).  Cutting up the last, partial wave of many tiles the
+    // same way costs more in joining than it evens out (T = 2048: 225 us against 215,
+    // T = 1024 at H = 1024, I = 512, 32 experts: 42 against 35).
     const int grid = static_cast<int>(gridDim.x) / kCtas, cta = static_cast<int>(blockIdx.x) / kCtas;
-    const int waves = s_misc[0] / grid, whole_tiles = waves * grid;
-    const int rest = s_misc[0] - whole_tiles;
-    const int64_t work = static_cast<int64_t>(rest) * nkb;
-    const int64_t shares = waves > 0 ? max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), work))
-                                     : rest * max(1, min(grid / max(rest, 1), nkb / kMx4MinPart));
-    const int64_t w0 = cta < shares ? work * cta / shares : 0;
-    const int64_t w1 = cta < shares ? work * (cta + 1) / shares : 0;
+    const int tiles = s_misc[0];
+    const int parts = max(1, min(grid / max(tiles, 1), nkb / kMx4MinPart));
 
     struct Tile {
-        int index, token, a, mt, nb, kb0, kb1;   // tile, its token tile, ...
-        int64_t w;    // next step of the share
-        int wave;     // next wave
-    };
-    auto begin = [&]() {
-        Tile t;
-        t.w = w0;
-        t.wave = 0;
-        return t;
+        int unit;                                  // tile * parts + part
+        int index, token, a, mt, nb, kb0, kb1;     // tile, its token tile, expert, weight tile, tile of the expert, steps
     };
     auto next = [&](Tile& t) {
-        if (t.w < w1) {
-            const int at = static_cast<int>(t.w / nkb);
-            t.index = whole_tiles + at;
-            t.kb0 = static_cast<int>(t.w - static_cast<int64_t>(at) * nkb);
-            t.kb1 = static_cast<int>(min(static_cast<int64_t>(nkb), t.kb0 + (w1 - t.w)));
-            t.w += t.kb1 - t.kb0;
-        } else if (t.wave < waves) {
-            t.index = t.wave++ * grid + cta;
-            t.kb0 = 0;
-            t.kb1 = nkb;
-        } else {
-            return false;
-        }
+        t.unit += grid;
+        if (t.unit >= tiles * parts) return false;
+        t.index = t.unit / parts;
+        const int part = t.unit - t.index * parts;
+        t.kb0 = part * nkb / parts;
+        t.kb1 = (part + 1) * nkb / parts;
         t.token = t.index / m_tiles;
         t.mt = t.index - t.token * m_tiles;
         t.a = find_expert(prefix, n_active, t.token);
         t.nb = t.token - prefix[t.a];
         return true;
+    };
+    auto begin = [&]() {
+        Tile t;
+        t.unit = cta - grid;
+        return t;
     };
 
     if (warp == 0) {
@@ -712,11 +699,8 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
             if (!wait(&tmem_full[b], acc_phase)) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(b * S::kAcc);
-            const bool whole = t.kb0 == 0 && t.kb1 == nkb;
-            // a share of a tile: the part with the tile's first K step is its CTA's
-            // last tile (slot 1), every other part its CTA's first (slot 0)
-            float* mine = args.partials +
-                          (static_cast<int64_t>(blockIdx.x) * 2 + (t.kb0 == 0 ? 1 : 0)) * S::kCols * 128 + i_row;
+            // a part's sums; with parts > 1 a CTA has one unit
+            float* mine = args.partials + static_cast<int64_t>(blockIdx.x) * S::kCols * 128 + i_row;
             for (int c = col0; c < ne; c += kColStep) {
                 const int n = min(kMx4Chunk, ne - c);
                 uint32_t r[4][kMx4Chunk];
@@ -736,7 +720,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
                     g[j] = __uint_as_float(r[0][j]) + (S::kStack ? __uint_as_float(r[2][j]) : 0.f);
                     u[j] = __uint_as_float(r[1][j]) + (S::kStack ? __uint_as_float(r[3][j]) : 0.f);
                 }
-                if (whole) {
+                if (parts == 1) {
                     finish(t, c, n, g, u);
                 } else {
 #pragma unroll
@@ -750,26 +734,22 @@ __global__ void __launch_bounds__(Mx4Shape<NT, PAIR>::kThreads, 1)
             if (col0 >= ne) {
                 release(b);
             }
-            if (whole) continue;
-            // the CTAs that share the tile: step w belongs to CTA floor(((w + 1) shares - 1) / work)
-            const int64_t first = static_cast<int64_t>(t.index - whole_tiles) * nkb, last = first + nkb - 1;
-            const int c_first = static_cast<int>(((first + 1) * shares - 1) / work);
-            const int c_last = static_cast<int>(((last + 1) * shares - 1) / work);
+            if (parts == 1) continue;
+            // the warp that takes a tile's last ticket adds the parts, in their order
             __syncwarp();
             unsigned int prev = 0;
             if (lane == 0) prev = ticket_acq_rel(&args.tickets[(t.index * kCtas + rank) * S::kEpi + warp - 2]);
             prev = __shfl_sync(0xffffffffu, prev, 0);
-            if (prev != static_cast<unsigned int>(c_last - c_first)) continue;
+            if (prev != static_cast<unsigned int>(parts - 1)) continue;
             for (int col = col0; col < ne; col += kColStep) {
                 const int n = min(kMx4Chunk, ne - col);
                 float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) g[j] = u[j] = 0.f;
-#pragma unroll 2
-                for (int c = c_first; c <= c_last; ++c) {
-                    // c_first holds the tile's first K step
+#pragma unroll kJoin
+                for (int i = 0; i < parts; ++i) {
                     const float* p = args.partials +
-                                     (static_cast<int64_t>(c * kCtas + rank) * 2 + (c == c_first ? 1 : 0)) * S::kCols * 128 + i_row;
+                                     static_cast<int64_t>((t.index * parts + i) * kCtas + rank) * S::kCols * 128 + i_row;
                     float pg[kMx4Chunk], pu[kMx4Chunk];
 #pragma unroll
                     for (int j = 0; j < kMx4Chunk; ++j) {

@@ -202,12 +202,12 @@ int device_setup(int* sms_out) {
         PDX_DEC_ATTR(true, 64, 16); PDX_DEC_ATTR(true, 64, 32); PDX_DEC_ATTR(true, 64, 64);
         PDX_DEC_ATTR(false, 16, 16); PDX_DEC_ATTR(false, 32, 32); PDX_DEC_ATTR(false, 64, 64);
 #undef PDX_DEC_ATTR
-#define PDX_MX4_ATTR(NT, PAIR)                                                                                     \
-    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, true, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,     \
+#define PDX_MX4_ATTR(NT)                                                                                           \
+    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,           \
                                       kMx4SmemLimit));                                                             \
-    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, false, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,    \
+    PDX_CUDA_TRY(cudaFuncSetAttribute(k_mx4_gemm<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,          \
                                       kMx4SmemLimit))
-        PDX_MX4_ATTR(16, false); PDX_MX4_ATTR(32, false); PDX_MX4_ATTR(64, false); PDX_MX4_ATTR(112, true);
+        PDX_MX4_ATTR(16); PDX_MX4_ATTR(32); PDX_MX4_ATTR(112);
 #undef PDX_MX4_ATTR
         g_num_sms[dev] = sms;
         g_attrs_set[dev] = true;
@@ -954,14 +954,17 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
     return PDX_OK;
 }
 
-// Token tile of the MXFP4 path: the smallest that holds an expert's average
-// rows with room to spare (a tile's MMAs cost its full width), 112 at most (two
-// gate/up accumulators of 2 x 112 columns and the scales fill TMEM).
-constexpr int kMx4PairTile = 112;
+// Token tile of the MXFP4 path, from the average rows of an expert.  A tile's MMAs
+// cost its full width and its weights are read once, so the tile should hold an
+// expert's rows.  Measured at H = 2048, I = 768, 128 experts (us, uniform routing):
+// 8 rows 68.5 (16) 70.3 (32); 16 rows 84.1 (16) 73.1 (32); 48 rows 121 (32) 122
+// (112), with a skewed router 121 (32) 137 (112); 64 rows 144 (32) 128 (112), skewed
+// 148 and 149; 128 rows 246 (32) 215 (112).  112 is the widest of which two
+// accumulators of gate and up (2 x 112 columns each) and the scales fit TMEM.
 int mx4_tile(int64_t rows, int64_t E) {
     const int64_t est = std::max<int64_t>(1, std::min(E, rows));
     const int64_t avg = (rows + est - 1) / est;
-    return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 48 ? 64 : kMx4PairTile));
+    return avg <= 8 ? 16 : (avg <= 56 ? 32 : 112);
 }
 
 // Rows up to which the split takes four warps a row (all rows in flight at once).
@@ -974,7 +977,7 @@ struct Mx4Bufs {
     float* row_scale;       // [rows]
     uint8_t* h;             // [2][rows][Ip] pieces
     uint8_t* sf;            // [tiles][Ip / 128] scale tiles of h
-    float* partials;        // [kPlanSMs][2][2 nt][128]
+    float* partials;        // [kPlanSMs][2 nt][128]
     unsigned int* tickets;  // words1 of the gate/up tiles, words2 of the down tiles
     int64_t words1, words2;
 };
@@ -988,7 +991,7 @@ Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
     b.row_scale = static_cast<float*>(c.take(rows * 4));
     b.h = static_cast<uint8_t*>(c.take(2 * rows * Ip));
     b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * kMx4SfBytes));
-    b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * 2 * b.nt * 128 * 4));
+    b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * b.nt * 128 * 4));
     // a ticket per tile, CTA of a pair and epilogue warp; pairs round the tiles of 256 rows up to even
     b.words1 = b.tiles * ((Ip / 128 + 1) / 2 * 2) * kMx4MaxEpi;
     b.words2 = b.tiles * ((Hp + 511) / 512 * 2) * kMx4MaxEpi;
@@ -1053,14 +1056,14 @@ struct Mx4Maps {
     CUtensorMap x, h, hs;   // token pieces of both products, scales of h
 };
 
-// The two products on tiles of NT tokens; PAIR: as clusters of two CTAs.
-template <int NT, bool PAIR>
-int launch_mx4_products(const Mx4Maps& m, Mx4Args gu, Mx4Args down, int64_t tiles, int sms,
-                        cudaStream_t stream) {
-    using S = Mx4Shape<NT, PAIR>;
-    constexpr int64_t ctas = PAIR ? 2 : 1;
+// The two products on tiles of NT tokens.
+template <int NT>
+int launch_mx4_products(const Mx4Maps& m, Mx4Args gu, Mx4Args down, int64_t tiles, int sms, cudaStream_t stream) {
+    using S = Mx4Shape<NT>;
+    constexpr int64_t ctas = S::kPair ? 2 : 1;
     gu.stages = down.stages = S::stages(gu.table);
     const int64_t most = std::min(sms, kPlanSMs) / ctas;   // the partial sums are sized for kPlanSMs CTAs
+    // no more CTAs than K steps
     const int64_t work1 = tiles * ((gu.M / 128 + ctas - 1) / ctas) * (gu.K / kMx4BK);
     const int64_t work2 = tiles * ((down.M / 128 + 2 * ctas - 1) / (2 * ctas)) * (down.K / kMx4BK);
     auto launch = [&](auto kernel, int64_t work, const CUtensorMap& tokens, const Mx4Args& a) {
@@ -1076,11 +1079,11 @@ int launch_mx4_products(const Mx4Maps& m, Mx4Args gu, Mx4Args down, int64_t tile
         attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
         attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = PAIR ? 2 : 1;
+        cfg.numAttrs = S::kPair ? 2 : 1;
         return cudaLaunchKernelEx(&cfg, kernel, m.w, tokens, m.ws, m.hs, a);
     };
-    PDX_PDL_TRY(launch(k_mx4_gemm<NT, true, PAIR>, work1, m.x, gu));
-    PDX_PDL_TRY(launch(k_mx4_gemm<NT, false, PAIR>, work2, m.h, down));
+    PDX_PDL_TRY(launch(k_mx4_gemm<NT, true>, work1, m.x, gu));
+    PDX_PDL_TRY(launch(k_mx4_gemm<NT, false>, work2, m.h, down));
     return PDX_OK;
 }
 
@@ -1096,7 +1099,7 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     const int per = (Hp / 128) * (Ip / 128);        // weight tiles of a projection
     const int64_t slots = w->num_slots, ss = slots > 1 ? w->scale_stride : 0;
     const int64_t tps = slots > 1 ? w->code_stride / kMx4TileBytes : 0;
-    const bool pair = b.nt == kMx4PairTile;
+    const bool pair = b.nt == 112;
     const int box = pair ? b.nt / 2 : b.nt;
     Mx4Maps m{};
     if ((st = encode_mx4_weights(&m.w, w->codes, (slots - 1) * tps + 3 * per))) return st;
@@ -1139,10 +1142,9 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     down.K = Ip;
     down.M = Hp;
     down.tickets = b.tickets + b.words1;
-    if (b.nt == 16) return launch_mx4_products<16, false>(m, gu, down, b.tiles, sms, stream);
-    if (b.nt == 32) return launch_mx4_products<32, false>(m, gu, down, b.tiles, sms, stream);
-    if (b.nt == 64) return launch_mx4_products<64, false>(m, gu, down, b.tiles, sms, stream);
-    return launch_mx4_products<kMx4PairTile, true>(m, gu, down, b.tiles, sms, stream);
+    if (b.nt == 16) return launch_mx4_products<16>(m, gu, down, b.tiles, sms, stream);
+    if (b.nt == 32) return launch_mx4_products<32>(m, gu, down, b.tiles, sms, stream);
+    return launch_mx4_products<112>(m, gu, down, b.tiles, sms, stream);
 }
 
 // ---- block norms ---------------------------------------------------------------------
