@@ -179,7 +179,7 @@ struct Mx4Args {
     int ldy;                        // H
     int stages, table;              // ring stages, entries of the expert tables (mx4_layout)
     float* partials;                // [gridDim.x][2 NT][128]
-    unsigned int* tickets;          // [tiles * CTAs of a tile * epilogue warps], zero on entry
+    unsigned int* tickets;          // [CTAs * epilogue warps], zero on entry
 };
 
 // Four words of four bytes, transposed: byte i of the words -> out[i].

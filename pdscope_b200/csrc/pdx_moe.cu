@@ -970,6 +970,9 @@ int mx4_tile(int64_t rows, int64_t E) {
 // Rows up to which the split takes four warps a row (all rows in flight at once).
 constexpr int64_t kMx4SplitFew = 4 * kPlanSMs;
 
+// Tickets of a product: tiles have parts only while they are fewer than the CTAs.
+constexpr int kMx4Tickets = kPlanSMs * kMx4MaxEpi;
+
 struct Mx4Bufs {
     int nt;
     int64_t tiles;          // token tiles at most, over all experts
@@ -978,8 +981,7 @@ struct Mx4Bufs {
     uint8_t* h;             // [2][rows][Ip] pieces
     uint8_t* sf;            // [tiles][Ip / 128] scale tiles of h
     float* partials;        // [kPlanSMs][2 nt][128]
-    unsigned int* tickets;  // words1 of the gate/up tiles, words2 of the down tiles
-    int64_t words1, words2;
+    unsigned int* tickets;  // [2][kMx4Tickets]: gate/up, down
 };
 
 Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
@@ -992,10 +994,7 @@ Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
     b.h = static_cast<uint8_t*>(c.take(2 * rows * Ip));
     b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * kMx4SfBytes));
     b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * b.nt * 128 * 4));
-    // a ticket per tile, CTA of a pair and epilogue warp; pairs round the tiles of 256 rows up to even
-    b.words1 = b.tiles * ((Ip / 128 + 1) / 2 * 2) * kMx4MaxEpi;
-    b.words2 = b.tiles * ((Hp + 511) / 512 * 2) * kMx4MaxEpi;
-    b.tickets = static_cast<unsigned int*>(c.take((b.words1 + b.words2) * 4));
+    b.tickets = static_cast<unsigned int*>(c.take(2 * kMx4Tickets * 4));
     return b;
 }
 
@@ -1115,7 +1114,7 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
                            dim3(static_cast<unsigned>(std::min<int64_t>(split_ctas, 16 * kPlanSMs))),
                            dim3(kMx4SplitWarps * 32), 0, stream, static_cast<const uint16_t*>(x), tokens,
                            static_cast<int>(T), n, static_cast<int>(H), Hp, b.x, b.row_scale, b.tickets,
-                           static_cast<int>(b.words1 + b.words2)));
+                           2 * kMx4Tickets));
     Mx4Args gu{};
     gu.offsets = offsets;
     gu.active = active;
@@ -1141,7 +1140,7 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     down.tile0 = 2 * per;
     down.K = Ip;
     down.M = Hp;
-    down.tickets = b.tickets + b.words1;
+    down.tickets = b.tickets + kMx4Tickets;
     if (b.nt == 16) return launch_mx4_products<16>(m, gu, down, b.tiles, sms, stream);
     if (b.nt == 32) return launch_mx4_products<32>(m, gu, down, b.tiles, sms, stream);
     return launch_mx4_products<112>(m, gu, down, b.tiles, sms, stream);

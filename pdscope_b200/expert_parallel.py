@@ -172,6 +172,8 @@ class ExpertParallelMoE:
         if self.experts % world:
             raise ValueError("experts must divide evenly over the ranks")
         self.local = self.experts // world
+        if isinstance(getattr(local_slab, "struct", None), _lib.Mxfp4Weights):
+            raise ValueError("expert parallelism runs on BF16 experts")
         if local_slab.num_slots < self.local:
             raise ValueError("local slab holds fewer experts than this rank owns")
         self.rank, self.world = rank, world

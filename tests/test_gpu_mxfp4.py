@@ -122,6 +122,8 @@ SHAPES = [  # tokens, hidden, inter, experts, top_k
     (257, 256, 128, 2, 1), (300, 128, 1024, 9, 3), (1000, 256, 256, 4, 4),
     # several tiles for every CTA or pair: narrow, middle and wide token tiles, odd numbers of 128-row blocks
     (200, 640, 640, 120, 8), (380, 384, 1152, 100, 8), (600, 256, 1280, 100, 6), (4100, 1152, 896, 4, 2),
+    # as many experts as the tables hold
+    (70, 128, 128, 1024, 8), (1, 8192, 64, 2, 1),
 ]
 
 
@@ -224,18 +226,18 @@ def test_bad_slot_and_bad_token_are_reported(pdx):
     runtime.raise_device_error()
 
 
-def test_two_streams_and_two_graphs(pdx):
-    """Calls on two streams at once and two captured graphs replayed in turn
+def test_streams_and_graphs_at_once(pdx):
+    """Calls on several streams at once and captured graphs replayed in turn
     give what single calls give."""
     cases = []
-    for tokens, seed in ((48, 1), (3, 2)):
+    for tokens, seed in ((48, 1), (3, 2), (900, 3)):   # the three token tiles
         slab, _ = _slab(pdx, 8, 512, 256, seed=seed)
         x = torch.randn(tokens, 512, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).cuda()
         sel = _selected(tokens, 8, 4, seed=seed)
         packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 8)
         cases.append((x, packed, slab, pdx.moe_ffn_mxfp4(x, packed, slab)))
     torch.cuda.synchronize()
-    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    streams = [torch.cuda.Stream() for _ in cases]
     outs = []
     for _ in range(10):
         for stream, (x, packed, slab, _) in zip(streams, cases):
@@ -243,7 +245,7 @@ def test_two_streams_and_two_graphs(pdx):
                 outs.append(pdx.moe_ffn_mxfp4(x, packed, slab))
     torch.cuda.synchronize()
     for i, out in enumerate(outs):
-        assert torch.equal(out, cases[i % 2][3])
+        assert torch.equal(out, cases[i % len(cases)][3])
     graphs = []
     for x, packed, slab, want in cases:
         g = torch.cuda.CUDAGraph()

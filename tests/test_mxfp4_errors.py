@@ -68,6 +68,11 @@ def test_ffn_status():
     assert _ffn(_weights(codes=None)) == _lib.PDX_ERR_INVALID
     assert _ffn(_weights(codes=264)) == _lib.PDX_ERR_INVALID
     assert _ffn(_weights(num_slots=0)) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(), experts=1025) == _lib.PDX_ERR_UNSUPPORTED
+    assert _ffn(_weights(scale_stride=3 * 128 * 4 + 16)) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(num_slots=1 << 23)) == _lib.PDX_ERR_UNSUPPORTED
+    assert _lib.lib.pdx_mxfp4_ffn_grouped(ctypes.c_void_p(264), 2, PTR, PTR, PTR, 2, 4, ctypes.byref(_weights()), 128,
+                                          128, PTR, PTR, 1 << 40, NULL) == _lib.PDX_ERR_INVALID
     assert _ffn(_weights(code_stride=128)) == _lib.PDX_ERR_INVALID
     assert _ffn(_weights(), ws=NULL) == _lib.PDX_ERR_WORKSPACE
     assert _ffn(_weights(), ws=ctypes.c_void_p(128)) == _lib.PDX_ERR_WORKSPACE
@@ -156,3 +161,10 @@ def test_stack_refuses_norms():
         ResidentMoEStack([gate], [slab], residual_dtype=torch.float32)
     with pytest.raises(ValueError, match="residual stream"):
         ResidentMoEStack([gate], [slab]).residual(1)
+
+
+def test_expert_parallel_refuses_mxfp4():
+    from pdscope_b200.expert_parallel import ExpertParallelMoE
+    gate = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="BF16 experts"):
+        ExpertParallelMoE(gate, pdx.Mxfp4ExpertSlab(4, 64, 64, "cpu"), rank=0, world=1)
