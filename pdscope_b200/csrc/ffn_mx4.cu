@@ -26,6 +26,11 @@
 // Tiles go round robin over the CTAs, neighbours sharing a token tile in L2.  When
 // there are fewer tiles than CTAs their K is cut up; a tile's parts are added in
 // order by the warp that takes its last ticket (FP32, deterministic, nothing waits).
+// Bound by HBM while an expert has few rows, by the power cap at prefill.  Device
+// time of the three launches at H = 2048, I = 768, 128 experts, top-8, with the
+// least the measured copy and BF16 rates allow: one token 16.2 us (3.1), 64 tokens
+// 68 (48.5; 6.0-6.6 TB/s between the launches' starts and tails), 12,450 tokens
+// 810-860 (578; 1.09-1.16 PFLOP/s, the BF16 experts take 1042).
 // Roles: warp 0 streams weights and scales, the last warp the token pieces, warp
 // 1 issues the MMAs, the others are the epilogue (32 weight rows, = one scale
 // block of h, and every second or fourth 8 token columns each).  Neither launch waits for another CTA; the
@@ -284,9 +289,10 @@ struct Mx4Shape {
     static constexpr uint32_t kB = 2 * kBRows * kMx4BK;
     static constexpr uint32_t kStage = kA + kB;                     // multiple of 1024
     static constexpr uint32_t kSf = 3 * kMx4SfBytes;                // both weight halves | tokens
-    // Eight columns take an epilogue warp 1000 (down) to 2000 cycles (SwiGLU), mostly
-    // latency.  Wide tiles have 14 such pieces to 6 K steps of MMAs (5600 cycles at
-    // NT = 112), so they take 16 warps; narrow ones keep the ring stage instead.
+    // Eight columns take one of eight epilogue warps 1000 (down) to 2000 cycles
+    // (SwiGLU), mostly latency.  Wide tiles have 14 such pieces to 6 K steps of MMAs
+    // (5600 cycles at NT = 112, I = 768), so they take 16 warps (prefill 884 -> 846 us);
+    // narrow ones keep the shared memory for the ring.
     static constexpr int kEpi = kPair ? 16 : 8;
     static constexpr int kThreads = 32 * (kEpi + 3);
     static constexpr uint32_t kFixed = 1024 + 512 + 512 + kEpi * kMx4StageOut;   // alignment, ones, barriers, staging
