@@ -9,13 +9,13 @@
 // The activations keep BF16's precision in that 8-bit product as TWO E4M3
 // pieces.  With v scaled by a power of two so that the largest value of its
 // scaling group lies in [128, 256):
-//   hi = e4m3(v),  lo = e4m3(v - hi)
-// e4m3 keeps 4 significant bits, so |v - hi| <= 2^-4 |v| and the rest after lo
-// is at most 2^-8 |v|: BF16's half step.  A BF16 v is represented exactly down
-// to 2^-10 of its group's largest value; below that the error is at most 2^-10
-// (half of e4m3's smallest step), 2^-17 of the largest value.  x is scaled per
-// row (a factor on the row of the result), h per 32 values of I (an E8M0 scale
-// of the second product).  W hi and W lo cost what one BF16 product would.
+//   hi = e4m3(v),  lo = e4m3(16 (v - hi)), read back through a scale of 1/16
+// e4m3 keeps 4 significant bits, so |v - hi| <= 2^-4 |v| (16 of it at most 256)
+// and the rest after lo is at most 2^-8 |v|: BF16's half step.  A BF16 v is
+// represented exactly down to 2^-13 of its group's largest value; below that the
+// error is at most 2^-14 (half of lo's smallest step), 2^-21 of the largest value.
+// x is scaled per row (a factor on the row of the result), h per 32 values of I (an
+// E8M0 scale of the second product).  W hi and W lo cost what one BF16 product would.
 //
 // Two launches of k_mx4_gemm, each on tiles of 256 weight rows (two accumulators
 // over one token operand): 128 rows of gate and the same 128 of up with the
@@ -33,8 +33,9 @@
 // 810-860 (578; 1.09-1.16 PFLOP/s, the BF16 experts take 1042).
 // Roles: warp 0 streams weights and scales, the last warp the token pieces, warp
 // 1 issues the MMAs, the others are the epilogue (32 weight rows, = one scale
-// block of h, and every second or fourth 8 token columns each).  Neither launch waits for another CTA; the
-// weight stream of a launch starts before the launch before it has finished.
+// block of h, and every second or fourth 8 token columns each).  Neither launch
+// waits for another CTA (but for the other of its pair); the weight stream of a
+// launch starts before the launch before it has finished.
 #include <cuda.h>
 
 #include "ffn_decode.cu"
@@ -53,15 +54,17 @@ constexpr int kMx4MaxActive = 1024;
 constexpr int kMx4MinPart = 4;                      // K steps of a part of a tile, at least
 constexpr uint32_t kMx4StageOut = 1024;             // 8 token columns x 64 weight rows on their way out
 constexpr uint32_t kMx4TmemCols = 512;
-constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of (gate | up | token) scales, 4 columns each
-constexpr uint32_t kMx4OneCol = 496;                // token scales of 1 (x is scaled by its row factor)
+constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of weight and token scales, 4 columns a tile
+constexpr uint32_t kMx4OneCol = 488;                // gate/up's token scales, constant: x has a row factor
+constexpr int kMx4LoShift = 4;                      // lo pieces are held times 2^4
 constexpr int kMx4SmemLimit = 227 * 1024;
 
 // Scale byte b of a group from the bits of its largest magnitude, which 2^(127 - b)
-// takes into [128, 256); 248 if the group holds an infinity or NaN.
+// takes into [128, 256); 248 if the group holds an infinity or NaN; at least
+// kMx4LoShift, so that the lo pieces' byte b - kMx4LoShift exists.
 __device__ __forceinline__ uint32_t mx4_group_byte(uint32_t max_bits) {
     const uint32_t e = max_bits >> 23;
-    return e > 7u ? e - 7u : 0u;
+    return e > 7u + kMx4LoShift ? e - 7u : kMx4LoShift;
 }
 // 2^(127 - b), or NaN for a non-finite group: e4m3 has no infinity, and
 // saturating would hide one.
@@ -75,7 +78,8 @@ __device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint
     uint32_t h2;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(hi));
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b - f.y), "f"(a - f.x));
+    constexpr float up = 1 << kMx4LoShift;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"((b - f.y) * up), "f"((a - f.x) * up));
 }
 
 // Token rows in packed order as E4M3 pieces: out [2][rows][Hp] (hi rows, then lo
@@ -178,7 +182,7 @@ struct Mx4Args {
     int K, M;                       // multiples of 128: reduction length, weight rows
     int rows;
     const float* row_scale;         // [rows] factor of a packed row of x (SWIGLU)
-    uint8_t* sf;                    // h scales: [token tile][Ip / 128] tiles of 512 bytes (out of SWIGLU, else in)
+    uint8_t* sf;                    // h scales: [token tile][Ip / 128][kSfTiles] tiles of 512 bytes (out of SWIGLU, else in)
     uint8_t* h;                     // [2][rows][M] pieces (SWIGLU)
     uint16_t* y;                    // [rows, ldy] (down)
     int ldy;                        // H
@@ -288,14 +292,15 @@ struct Mx4Shape {
     static constexpr uint32_t kATx = kA / 2;                        // the copy counts the packed bytes it reads
     static constexpr uint32_t kB = 2 * kBRows * kMx4BK;
     static constexpr uint32_t kStage = kA + kB;                     // multiple of 1024
-    static constexpr uint32_t kSf = 3 * kMx4SfBytes;                // both weight halves | tokens
+    static constexpr int kSfTiles = kStack ? 1 : 2;                 // token scales: stacked, or hi | lo
+    static constexpr uint32_t kSf = (2 + kSfTiles) * kMx4SfBytes;   // both weight halves | tokens
     // Eight columns take one of eight epilogue warps 1000 (down) to 2000 cycles
     // (SwiGLU), mostly latency.  Wide tiles have 14 such pieces to 6 K steps of MMAs
     // (5600 cycles at NT = 112, I = 768), so they take 16 warps (prefill 884 -> 846 us);
     // narrow ones keep the shared memory for the ring.
     static constexpr int kEpi = kPair ? 16 : 8;
     static constexpr int kThreads = 32 * (kEpi + 3);
-    static constexpr uint32_t kFixed = 1024 + 512 + 512 + kEpi * kMx4StageOut;   // alignment, ones, barriers, staging
+    static constexpr uint32_t kFixed = 1024 + 1024 + 512 + kEpi * kMx4StageOut;  // alignment, constants, barriers, staging
     // Ring stages beside tables of `entries` experts, and the shared memory of both.
     static constexpr int stages(int entries) {
         return static_cast<int>((kMx4SmemLimit - kFixed - 16u * entries) / (kStage + kSf));
@@ -326,8 +331,8 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
     const int stages = args.stages;
     unsigned char* s_sf = smem + stages * S::kStage;                 // stages x kSf
-    unsigned char* s_one = s_sf + stages * S::kSf;                   // 512 bytes of scale 1
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_one + 512);
+    unsigned char* s_one = s_sf + stages * S::kSf;                   // constant token scales, kSfTiles tiles
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_one + 1024);
     uint64_t* empty_bar = full_bar + stages;
     uint64_t* tmem_full = empty_bar + stages;
     uint64_t* tmem_empty = tmem_full + 2;
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_misc = reinterpret_cast<int*>(tmem_slot + 2);
-    unsigned char* s_out = s_one + 1024;                             // an epilogue warp's staging: kMx4StageOut
+    unsigned char* s_out = s_one + 1536;                             // an epilogue warp's staging: kMx4StageOut
     int* prefix = reinterpret_cast<int*>(s_out + S::kEpi * kMx4StageOut);   // token tiles before an active expert
     int* t_seg0 = prefix + args.table;
     int* t_rows = t_seg0 + args.table;
@@ -387,8 +392,11 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
         }
     }
     if (warp >= 3)
-        for (int i = static_cast<int>(threadIdx.x) - 96; i < 128; i += S::kThreads - 96)
-            reinterpret_cast<uint32_t*>(s_one)[i] = 0x7F7F7F7Fu;
+        for (int i = static_cast<int>(threadIdx.x) - 96; i < 128 * S::kSfTiles; i += S::kThreads - 96) {
+            // word i of a tile: row 32 (i % 4) + i / 4; scale 1 of hi, 2^-kMx4LoShift of lo
+            const bool low = S::kStack ? 32 * (i & 3) + (i >> 2) >= NT : i >= 128;
+            reinterpret_cast<uint32_t*>(s_one)[i] = (127u - (low ? kMx4LoShift : 0)) * 0x01010101u;
+        }
     fence_proxy_async_smem();
     // The routing tables are older than the launch before this one, which has
     // passed its own wait by the time this one starts; only that launch's
@@ -477,7 +485,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                     const int y0 = static_cast<int>(tile0 + b0 + kb) * 128, y1 = static_cast<int>(tile0 + b1 + kb) * 128;
                     if (rank == 0)
                         mbar_arrive_expect_tx(&full_bar[stage],
-                                              kCtas * (S::kATx + S::kB + (SWIGLU ? 2 : 3) * kMx4SfBytes));
+                                              kCtas * (S::kATx + S::kB + (SWIGLU ? 2 : 2 + S::kSfTiles) * kMx4SfBytes));
                     if (PAIR) {
                         const uint32_t fb = full0 + static_cast<uint32_t>(stage) * 8u;
                         tma_load_2d_pair(sa, &tm_w, fb, 0, y0);
@@ -518,9 +526,9 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                     if (PAIR) {
                         const uint32_t fb = full0 + static_cast<uint32_t>(stage) * 8u;
                         tma_load_3d_pair(smem + stage * S::kStage + S::kA, &tm_x, fb, kb * kMx4BK, row, 0);
-                        if (!SWIGLU)
-                            tma_load_2d_pair(s_sf + stage * S::kSf + 2 * kMx4SfBytes, &tm_xs, fb, 0,
-                                             static_cast<int>(tt * nkb + kb));
+                        for (int i = 0; !SWIGLU && i < S::kSfTiles; ++i)
+                            tma_load_2d_pair(s_sf + stage * S::kSf + (2 + i) * kMx4SfBytes, &tm_xs, fb, 0,
+                                             static_cast<int>(tt * nkb + kb) * S::kSfTiles + i);
                         if (++stage == stages) { stage = 0; phase ^= 1u; }
                         continue;
                     }
@@ -536,7 +544,10 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     } else if (warp == 1 && rank == 0) {
         // ---------------- MMA issuer (of the pair: rank 0) ----------------
         constexpr uint32_t idesc = mx4_idesc(128 * kCtas, S::kN);
-        if (elect_one()) tmem_cp_sf<PAIR>(tmem_base + kMx4OneCol, mx4_sf_desc(smem_u32(s_one)));
+        constexpr uint32_t kSlot = SWIGLU ? 8 : 8 + 4 * S::kSfTiles;   // scale columns of a K step
+        if (SWIGLU && elect_one())
+            for (int i = 0; i < S::kSfTiles; ++i)
+                tmem_cp_sf<PAIR>(tmem_base + kMx4OneCol + 4 * i, mx4_sf_desc(smem_u32(s_one) + i * kMx4SfBytes));
         __syncwarp();
         auto commit = [&](uint64_t* bar) {   // to this barrier of every CTA of the tile
             if (PAIR) {
@@ -561,11 +572,12 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                 if (elect_one()) {
                     const uint32_t sa = smem_u32(smem + stage * S::kStage);
                     const uint32_t ss = smem_u32(s_sf + stage * S::kSf);
-                    const uint32_t sf = tmem_base + kMx4SfCol + static_cast<uint32_t>(step & 3) * 12;
+                    const uint32_t sf = tmem_base + kMx4SfCol + static_cast<uint32_t>(step & 3) * kSlot;
                     tmem_cp_sf<PAIR>(sf, mx4_sf_desc(ss));
                     tmem_cp_sf<PAIR>(sf + 4, mx4_sf_desc(ss + kMx4SfBytes));
-                    if (!SWIGLU) tmem_cp_sf<PAIR>(sf + 8, mx4_sf_desc(ss + 2 * kMx4SfBytes));
-                    const uint32_t sfb = SWIGLU ? tmem_base + kMx4OneCol : sf + 8;
+                    for (int i = 0; !SWIGLU && i < S::kSfTiles; ++i)
+                        tmem_cp_sf<PAIR>(sf + 8 + 4 * i, mx4_sf_desc(ss + (2 + i) * kMx4SfBytes));
+                    const uint32_t sfb = SWIGLU ? tmem_base + kMx4OneCol : sf + 8, sfb_lo = sfb + 4;
                     const uint64_t a0 = sw128_desc(sa), a1 = sw128_desc(sa + kMx4ABytes);
                     const uint64_t hi = sw128_desc(sa + S::kA), lo = sw128_desc(sa + S::kA + S::kBRows * kMx4BK);
 #pragma unroll
@@ -573,9 +585,9 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                         const uint32_t acc = (kb > t.kb0 || kk > 0) ? 1u : 0u;
                         const uint32_t id = idesc | (static_cast<uint32_t>(kk) << 29) | (static_cast<uint32_t>(kk) << 4);
                         umma_mx4<PAIR>(d, a0 + 2u * kk, hi + 2u * kk, id, sf, sfb, acc);
-                        if (!S::kStack) umma_mx4<PAIR>(d, a0 + 2u * kk, lo + 2u * kk, id, sf, sfb, 1u);
+                        if (!S::kStack) umma_mx4<PAIR>(d, a0 + 2u * kk, lo + 2u * kk, id, sf, sfb_lo, 1u);
                         umma_mx4<PAIR>(d + S::kN, a1 + 2u * kk, hi + 2u * kk, id, sf + 4, sfb, acc);
-                        if (!S::kStack) umma_mx4<PAIR>(d + S::kN, a1 + 2u * kk, lo + 2u * kk, id, sf + 4, sfb, 1u);
+                        if (!S::kStack) umma_mx4<PAIR>(d + S::kN, a1 + 2u * kk, lo + 2u * kk, id, sf + 4, sfb_lo, 1u);
                     }
                     commit(&empty_bar[stage]);
                 }
@@ -652,9 +664,12 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                 __syncwarp();
                 if (lane < kMx4Chunk) {
                     const int r = c0 + static_cast<int>(lane);   // row of the token tile
-                    uint8_t* sf = args.sf + (static_cast<int64_t>(t.token) * m_blocks + part) * kMx4SfBytes + q;
-                    sf[(r & 31) * 16 + (r >> 5) * 4] = static_cast<uint8_t>(byte);
-                    if (S::kStack) sf[((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4] = static_cast<uint8_t>(byte);
+                    uint8_t* sf =
+                        args.sf + (static_cast<int64_t>(t.token) * m_blocks + part) * (S::kSfTiles * kMx4SfBytes) + q;
+                    const int hi_at = (r & 31) * 16 + (r >> 5) * 4;
+                    const int lo_at = S::kStack ? ((r + NT) & 31) * 16 + ((r + NT) >> 5) * 4 : hi_at + kMx4SfBytes;
+                    sf[hi_at] = static_cast<uint8_t>(byte);
+                    sf[lo_at] = static_cast<uint8_t>(byte - kMx4LoShift);
                 }
             } else {
                 // One word per weight row and 2 columns, [half][2 columns][32 rows]; then every

@@ -979,7 +979,8 @@ struct Mx4Bufs {
     uint8_t* x;             // [2][rows][Hp] pieces of the gathered rows
     float* row_scale;       // [rows]
     uint8_t* h;             // [2][rows][Ip] pieces
-    uint8_t* sf;            // [tiles][Ip / 128] scale tiles of h
+    uint8_t* sf;            // [tiles][Ip / 128][sf_tiles] scale tiles of h
+    int sf_tiles;
     float* partials;        // [kPlanSMs][2 nt][128]
     unsigned int* tickets;  // [2][kMx4Tickets]: gate/up, down
 };
@@ -992,7 +993,8 @@ Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
     b.x = static_cast<uint8_t*>(c.take(2 * rows * Hp));
     b.row_scale = static_cast<float*>(c.take(rows * 4));
     b.h = static_cast<uint8_t*>(c.take(2 * rows * Ip));
-    b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * kMx4SfBytes));
+    b.sf_tiles = b.nt > 32 ? 2 : 1;
+    b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * b.sf_tiles * kMx4SfBytes));
     b.partials = static_cast<float*>(c.take(static_cast<size_t>(kPlanSMs) * 2 * b.nt * 128 * 4));
     b.tickets = static_cast<unsigned int*>(c.take(2 * kMx4Tickets * 4));
     return b;
@@ -1106,7 +1108,7 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     if ((st = encode_mx4_tokens(&m.h, b.h, rows, Ip, box))) return st;
     if (pair) {
         if ((st = encode_mx4_scales(&m.ws, w->scales, (slots - 1) * (ss / kMx4SfBytes) + 3 * per))) return st;
-        if ((st = encode_mx4_scales(&m.hs, b.sf, b.tiles * (Ip / 128)))) return st;
+        if ((st = encode_mx4_scales(&m.hs, b.sf, b.tiles * (Ip / 128) * b.sf_tiles))) return st;
     }
     const bool few = rows <= kMx4SplitFew;
     const int64_t split_ctas = few ? rows : (rows + kMx4SplitWarps - 1) / kMx4SplitWarps;

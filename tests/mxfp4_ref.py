@@ -34,19 +34,19 @@ def ffn_rows(x, g, u, d):
     """(y, bound) of one expert on rows x [n, H] in float64.
 
     The bound covers what the kernels round: x as two E4M3 pieces (an absolute
-    2^-17 of the row's largest value at most), FP32 sums (n 2^-24 of the sum of
-    magnitudes), h as two E4M3 pieces (2^-8 of the value, or 2^-17 of the
+    2^-21 of the row's largest value at most), FP32 sums (n 2^-24 of the sum of
+    magnitudes), h as two E4M3 pieces (2^-8 of the value, or 2^-21 of the
     largest of 32), and one BF16 rounding (2^-8)."""
     gl, ul = x @ g.T, x @ u.T
     sig = 1 / (1 + np.exp(-gl))
     h = gl * sig * ul
     top = np.abs(x).max(-1, keepdims=True)
-    dg = 2.0 ** -17 * top * np.abs(g).sum(-1) + x.shape[1] * 2.0 ** -24 * (np.abs(x) @ np.abs(g).T)
-    du = 2.0 ** -17 * top * np.abs(u).sum(-1) + x.shape[1] * 2.0 ** -24 * (np.abs(x) @ np.abs(u).T)
+    dg = 2.0 ** -21 * top * np.abs(g).sum(-1) + x.shape[1] * 2.0 ** -24 * (np.abs(x) @ np.abs(g).T)
+    du = 2.0 ** -21 * top * np.abs(u).sum(-1) + x.shape[1] * 2.0 ** -24 * (np.abs(x) @ np.abs(u).T)
     # |silu'| <= 1.1; a few FP32 roundings in the activation
     dh = 1.1 * dg * (np.abs(ul) + du) + np.abs(gl * sig) * du + 2.0 ** -20 * np.abs(h)
     blocks = np.pad(np.abs(h), ((0, 0), (0, -h.shape[1] % 32))).reshape(h.shape[0], -1, 32).max(-1)
-    dh = dh + 2.0 ** -8 * np.abs(h) + 2.0 ** -17 * np.repeat(blocks, 32, axis=1)[:, :h.shape[1]]
+    dh = dh + 2.0 ** -8 * np.abs(h) + 2.0 ** -21 * np.repeat(blocks, 32, axis=1)[:, :h.shape[1]]
     y = h @ d.T
     dy = dh @ np.abs(d).T + h.shape[1] * 2.0 ** -24 * (np.abs(h) @ np.abs(d).T)
     return y, dy + 2.0 ** -8 * (np.abs(y) + dy) + 1e-38

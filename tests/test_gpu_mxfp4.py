@@ -155,6 +155,28 @@ def test_grouped_ffn_ranges(pdx, std, scale):
     assert (got[zero] == 0).all()
 
 
+@pytest.mark.parametrize("tokens", (3, 40, 300))      # the three token tiles
+def test_outlier_the_weights_ignore(pdx, tokens):
+    """A channel 4000 times the rest whose weights are zero: what is left of the
+    others' precision (2^-21 of the row's largest value each) decides."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    ws = [torch.randn(2, r, c, device="cuda", generator=gen) * 0.05 for r, c in ((128, 512), (128, 512), (512, 128))]
+    ws[0][:, :, 77], ws[1][:, :, 77] = 0, 0
+    qs = [pdx.quantize_mxfp4(w) for w in ws]
+    slab = pdx.Mxfp4ExpertSlab.from_quantized(*qs)
+    x = torch.randn(tokens, 512, device="cuda", generator=gen)
+    x[:, 77] = 4000.0
+    x = x.to(torch.bfloat16)
+    sel = _selected(tokens, 2, 1, seed=1)
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 2)
+    got = pdx.moe_ffn_mxfp4(x, packed, slab)
+    _check_rows(got, x, packed, qs, 2)
+    x[:, 77] = 0
+    clean = pdx.moe_ffn_mxfp4(x, packed, slab)
+    # 4000 2^-21 = 2^-9 at most of values of about 1, averaged over 512: below BF16's own rounding
+    assert (got.double() - clean.double()).norm() <= 2.0 ** -8 * clean.double().norm()
+
+
 @pytest.mark.parametrize("bad", (float("inf"), float("nan")))
 def test_non_finite_rows_stay_in_their_rows(pdx, bad):
     slab, _ = _slab(pdx, 4, 256, 128, seed=3)
