@@ -545,10 +545,6 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
         // ---------------- MMA issuer (of the pair: rank 0) ----------------
         constexpr uint32_t idesc = mx4_idesc(128 * kCtas, S::kN);
         constexpr uint32_t kSlot = SWIGLU ? 8 : 8 + 4 * S::kSfTiles;   // scale columns of a K step
-        if (SWIGLU && elect_one())
-            for (int i = 0; i < S::kSfTiles; ++i)
-                tmem_cp_sf<PAIR>(tmem_base + kMx4OneCol + 4 * i, mx4_sf_desc(smem_u32(s_one) + i * kMx4SfBytes));
-        __syncwarp();
         auto commit = [&](uint64_t* bar) {   // to this barrier of every CTA of the tile
             if (PAIR) {
                 umma_commit_pair(smem_u32(bar));
@@ -573,6 +569,8 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                     const uint32_t sa = smem_u32(smem + stage * S::kStage);
                     const uint32_t ss = smem_u32(s_sf + stage * S::kSf);
                     const uint32_t sf = tmem_base + kMx4SfCol + static_cast<uint32_t>(step & 3) * kSlot;
+                    for (int i = 0; SWIGLU && step == 0 && i < S::kSfTiles; ++i)
+                        tmem_cp_sf<PAIR>(tmem_base + kMx4OneCol + 4 * i, mx4_sf_desc(smem_u32(s_one) + i * kMx4SfBytes));
                     tmem_cp_sf<PAIR>(sf, mx4_sf_desc(ss));
                     tmem_cp_sf<PAIR>(sf + 4, mx4_sf_desc(ss + kMx4SfBytes));
                     for (int i = 0; !SWIGLU && i < S::kSfTiles; ++i)
@@ -732,9 +730,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                     tmem_ld8(taddr + S::kN + NT + c, r[3]);
                 }
                 tmem_wait_ld();
-                if (c + kColStep >= ne) {                   // this warp's last columns are read
-                    release(b);
-                }
+                if (c + kColStep >= ne) release(b);         // this warp's last columns are read
                 float g[kMx4Chunk], u[kMx4Chunk];
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) {
@@ -752,9 +748,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                         }
                 }
             }
-            if (col0 >= ne) {
-                release(b);
-            }
+            if (col0 >= ne) release(b);
             if (parts == 1) continue;
             // the warp that takes a tile's last ticket adds the parts, in their order
             __syncwarp();
