@@ -380,13 +380,31 @@ def _norm_weight(name, w, norm, hidden, device):
 
 
 def _span(t):
-    """First byte and end of a contiguous tensor."""
+    """First byte and end of the memory a tensor's elements lie in."""
     at = t.data_ptr()
-    return at, at + t.numel() * t.element_size()
+    return at, at + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else at
 
 
-def _block_norm_outputs(norm, options, residual, stream_out, out, apart=None):
-    """Checked (arguments, stream_out, out) of a block norm; ``apart`` must not overlap the outputs."""
+def _overlap(a, b):
+    return a[0] < b[1] and b[0] < a[1]
+
+
+def _check_outputs(outputs, inputs, apart):
+    """Outputs may be an input of their own type (each row is read before it is
+    written), but not lie across one, nor touch one of ``apart`` or each other."""
+    spans = [_span(t) for t in outputs]
+    if _overlap(*spans):
+        raise ValueError("stream_out and out must not overlap")
+    for t, span in zip(outputs, spans):
+        for u in inputs:
+            if u is not None and _overlap(span, _span(u)) and (t.data_ptr() != u.data_ptr() or t.dtype != u.dtype):
+                raise ValueError("an output must be an input of its own type or lie apart from it")
+        if any(_overlap(span, _span(u)) for u in apart if u is not None):
+            raise ValueError("the outputs must not overlap the expert rows or the gate")
+
+
+def _block_norm_outputs(norm, options, y, residual, stream_out, out, rows=None):
+    """Checked (arguments, stream_out, out) of a block norm of ``y`` or of the combine of ``rows``."""
     if norm is None:
         norm = BlockNorm(**options)
     elif options or not isinstance(norm, BlockNorm):
@@ -394,6 +412,10 @@ def _block_norm_outputs(norm, options, residual, stream_out, out, apart=None):
     if not isinstance(residual, torch.Tensor) or not residual.is_cuda or residual.ndim != 2 \
             or residual.dtype not in (torch.bfloat16, torch.float32) or not residual.is_contiguous():
         raise ValueError("residual must be a contiguous [T, H] BF16 or FP32 CUDA tensor")
+    if y is not None:
+        _require_cuda_bf16("y", y, 2)
+        if y.shape != residual.shape or y.device != residual.device:
+            raise ValueError("y and residual shapes differ")
     fresh = stream_out is None and out is None
     if stream_out is None:
         stream_out = torch.empty_like(residual)
@@ -407,13 +429,7 @@ def _block_norm_outputs(norm, options, residual, stream_out, out, apart=None):
         if out.shape != residual.shape or out.device != residual.device:
             raise ValueError("out must have residual's shape and device")
     if not fresh:
-        spans = [_span(stream_out), _span(out)]
-        if spans[0][0] < spans[1][1] and spans[1][0] < spans[0][1]:
-            raise ValueError("stream_out and out must not overlap")
-        if apart is not None:
-            first, end = _span(apart)
-            if any(a < end and first < b for a, b in spans):
-                raise ValueError("the outputs must not alias rows")
+        _check_outputs((stream_out, out), (y, residual), (rows, norm.gate))
     return norm.args(*residual.shape, residual.dtype, residual.device), stream_out, out
 
 
@@ -426,11 +442,7 @@ def block_norm(y, residual, *, norm=None, stream_out=None, out=None, **options):
     FP32.  The options are ``BlockNorm``'s fields, or ``norm=BlockNorm(...)``.
     ``stream`` has residual's type, ``normed`` is BF16; ``stream_out`` and
     ``out`` may be ``y`` or ``residual``."""
-    args, stream_out, out = _block_norm_outputs(norm, options, residual, stream_out, out)
-    if y is not None:
-        _require_cuda_bf16("y", y, 2)
-        if y.shape != residual.shape or y.device != residual.device:
-            raise ValueError("y and residual shapes differ")
+    args, stream_out, out = _block_norm_outputs(norm, options, y, residual, stream_out, out)
     t_count, hidden = residual.shape
     _call(residual.device, lib.pdx_block_norm, y.data_ptr() if y is not None else None, residual.data_ptr(), t_count,
           hidden, ctypes.byref(args), stream_out.data_ptr(), out.data_ptr())
@@ -448,7 +460,7 @@ def combine_block_norm(rows, weights, inverse, residual, *, norm=None, stream_ou
     if not isinstance(inverse, torch.Tensor) or inverse.dtype != torch.int32 or inverse.device != device \
             or inverse.numel() != t_count * k or not inverse.is_contiguous():
         raise ValueError("inverse must be a contiguous int32 tensor of T*k entries on the device of rows")
-    args, stream_out, out = _block_norm_outputs(norm, options, residual, stream_out, out, apart=rows)
+    args, stream_out, out = _block_norm_outputs(norm, options, None, residual, stream_out, out, rows)
     if residual.shape != (t_count, rows.shape[1]) or residual.device != device or weights.device != device:
         raise ValueError("residual must be [T, H] on the device of rows")
     _call(device, lib.pdx_combine_block_norm, rows.data_ptr(), rows.shape[0], weights.data_ptr(), inverse.data_ptr(),
@@ -595,6 +607,8 @@ class ResidentMoELayer:
         _require_cuda_bf16("x", x, 2)
         t_count = x.shape[0]
         dev = x.device
+        if x.shape[1] != self.hidden:
+            raise ValueError("activation and expert hidden sizes differ")
         if outputs is None:
             outputs = LayerOutputs(
                 out=torch.empty((t_count, self.hidden), dtype=torch.bfloat16, device=dev),

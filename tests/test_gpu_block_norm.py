@@ -117,6 +117,24 @@ def test_strided_gates_and_aliased_outputs(pdx, hidden):
     assert torch.equal(r, want[0]) and torch.equal(y, want[1])
 
 
+def test_overlapping_outputs_are_refused(pdx):
+    t = _inputs(4, 64, torch.bfloat16, "full", seed=3)
+    both = torch.zeros(5, 64, dtype=torch.bfloat16, device="cuda")
+    wide = torch.zeros(4, 64, dtype=torch.float32, device="cuda")
+    half = wide.view(-1)[:128].view(torch.bfloat16).view(4, 64)     # BF16 over the first half of an FP32 stream
+    for kw, match in ((dict(stream_out=both[:4], out=both[1:]), "must not overlap"),
+                      (dict(y=both[1:], out=both[:4]), "lie apart"),
+                      (dict(residual=wide, out=half), "lie apart"),
+                      (dict(out=t["gate"]), "gate")):
+        args = dict(dict(y=t["y"], residual=t["residual"]), **kw)
+        with pytest.raises(ValueError, match=match):
+            pdx.block_norm(args.pop("y"), args.pop("residual"), gate=t["gate"], **args)
+    rows = torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="expert rows"):
+        pdx.combine_block_norm(rows, torch.ones(4, 2, dtype=torch.bfloat16, device="cuda"),
+                               torch.arange(8, dtype=torch.int32, device="cuda"), t["residual"], out=rows[4:])
+
+
 @pytest.mark.parametrize("tokens,hidden,top_k", ((1, 64, 1), (1, 2048, 8), (7, 1003, 3), (64, 2048, 8), (5, 4096, 12),
                                                  (3, 8192, 32)))
 @pytest.mark.parametrize("residual", (torch.bfloat16, torch.float32))
