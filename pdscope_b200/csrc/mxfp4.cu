@@ -94,11 +94,14 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
     }
 }
 
-// Both kernels are copies with a conversion: HBM-bound (98,304 x 2048 BF16 to
-// MXFP4 and back: 192 us, 5.3 TB/s).  A thread takes kMxUnroll pieces of eight values, a CTA's threads neighbouring pieces, and
-// issues all its loads before converting.  FLAT: rows without gaps, so a piece's
-// place needs no division by the row length.
-constexpr int kMxUnroll = 4;
+// Both kernels are copies with a conversion: HBM-bound.  98,304 x 2048: BF16 to
+// MXFP4 96 us (5.3 TB/s), back 78 us (6.5 TB/s); half as much FP32 to MXFP4 65 us
+// (7.0 TB/s).  A thread takes a few pieces of eight values, a CTA's threads
+// neighbouring pieces, and issues all its loads before converting (quantising: 2
+// pieces 96 us, 4 pieces 112, 1 piece 109; back: 4 pieces 78, 2 pieces 80, 1 piece
+// 105).  FLAT: rows without gaps, so a piece's place needs no division by the row
+// length.
+constexpr int kMxUnroll = 2, kMxUnrollBack = 4;
 
 template <bool FLAT>
 __device__ __forceinline__ int64_t mx_at(int64_t c, int64_t per_row, int64_t ld) {
@@ -149,10 +152,10 @@ __global__ void __launch_bounds__(kMxThreads) k_mx4_dequantize(const uint32_t* _
                                                                int64_t per_row, int64_t ld, T* __restrict__ out) {
     griddep_wait();
     griddep_launch();
-    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * (kMxThreads * kMxUnroll) + threadIdx.x;
-    uint32_t code[kMxUnroll], scale[kMxUnroll];
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * (kMxThreads * kMxUnrollBack) + threadIdx.x;
+    uint32_t code[kMxUnrollBack], scale[kMxUnrollBack];
 #pragma unroll
-    for (int j = 0; j < kMxUnroll; ++j) {
+    for (int j = 0; j < kMxUnrollBack; ++j) {
         const int64_t c = c0 + j * kMxThreads;
         if (c < chunks) {
             code[j] = __ldg(codes + c);
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(kMxThreads) k_mx4_dequantize(const uint32_t* _
         }
     }
 #pragma unroll
-    for (int j = 0; j < kMxUnroll; ++j) {
+    for (int j = 0; j < kMxUnrollBack; ++j) {
         const int64_t c = c0 + j * kMxThreads;
         if (c >= chunks) return;
         const float s = mx_scale(scale[j]);

@@ -927,8 +927,8 @@ cudaError_t with_mx4_type(int32_t dtype, bool aligned, bool flat, F f) {
     return with_type(float{});
 }
 
-dim3 mx4_grid(int64_t chunks) {
-    return dim3(static_cast<unsigned>((chunks + kMxThreads * kMxUnroll - 1) / (kMxThreads * kMxUnroll)));
+dim3 mx4_grid(int64_t chunks, int unroll) {
+    return dim3(static_cast<unsigned>((chunks + kMxThreads * unroll - 1) / (kMxThreads * unroll)));
 }
 
 int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool gathered,
@@ -1581,8 +1581,8 @@ int pdx_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols,
     const int64_t chunks = rows * cols / 8;
     PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(x, ld, dtype), ld == cols, [&](auto type, auto aligned, auto flat) {
         using T = decltype(type);
-        return launch_pdl(k_mx4_quantize<T, decltype(aligned)::value, decltype(flat)::value>, mx4_grid(chunks),
-                          dim3(kMxThreads), 0, stream, static_cast<const T*>(x), chunks, cols / 8, ld,
+        return launch_pdl(k_mx4_quantize<T, decltype(aligned)::value, decltype(flat)::value>,
+                          mx4_grid(chunks, kMxUnroll), dim3(kMxThreads), 0, stream, static_cast<const T*>(x), chunks, cols / 8, ld,
                           static_cast<uint32_t*>(codes), static_cast<uint8_t*>(scales));
     }));
     return ok();
@@ -1598,8 +1598,8 @@ int pdx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, in
     const int64_t chunks = rows * cols / 8;
     PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(out, ld, dtype), ld == cols, [&](auto type, auto aligned, auto flat) {
         using T = decltype(type);
-        return launch_pdl(k_mx4_dequantize<T, decltype(aligned)::value, decltype(flat)::value>, mx4_grid(chunks),
-                          dim3(kMxThreads), 0, stream, static_cast<const uint32_t*>(codes),
+        return launch_pdl(k_mx4_dequantize<T, decltype(aligned)::value, decltype(flat)::value>,
+                          mx4_grid(chunks, kMxUnrollBack), dim3(kMxThreads), 0, stream, static_cast<const uint32_t*>(codes),
                           static_cast<const uint8_t*>(scales), chunks, cols / 8, ld, static_cast<T*>(out));
     }));
     return ok();
