@@ -28,9 +28,9 @@
 // order by the warp that takes its last ticket (FP32, deterministic, nothing waits).
 // Bound by HBM while an expert has few rows, by the power cap at prefill.  Device
 // time of the three launches at H = 2048, I = 768, 128 experts, top-8, with the
-// least the measured copy and BF16 rates allow: one token 16.2 us (3.1), 64 tokens
-// 68 (48.5; 6.0-6.6 TB/s between the launches' starts and tails), 12,450 tokens
-// 810-860 (578; 1.09-1.16 PFLOP/s, the BF16 experts take 1042).
+// least the measured copy and BF16 rates allow: one token 16.3 us (3.1), 64 tokens
+// 68-71 (48.5; 6.0-6.6 TB/s between the launches' starts and tails), 12,450 tokens
+// 810-850 (578; 1.11-1.16 PFLOP/s, the BF16 experts take 1042).
 // Roles: warp 0 streams weights and scales, the last warp the token pieces, warp
 // 1 issues the MMAs, the others are the epilogue (32 weight rows, = one scale
 // block of h, and every second or fourth 8 token columns each).  Neither launch
@@ -51,7 +51,6 @@ constexpr uint32_t kMx4ABytes = 128 * kMx4BK;       // one weight tile, a byte p
 constexpr int kMx4TileBytes = 128 * kMx4BK / 2;     // its codes in memory
 constexpr uint32_t kMx4SfBytes = 512;               // scales of 128 rows x 128 columns
 constexpr int kMx4MaxActive = 1024;
-constexpr int kMx4MinPart = 4;                      // K steps of a part of a tile, at least
 constexpr uint32_t kMx4StageOut = 1024;             // 8 token columns x 64 weight rows on their way out
 constexpr uint32_t kMx4TmemCols = 512;
 constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of weight and token scales, 4 columns a tile
@@ -325,6 +324,10 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     using S = Mx4Shape<NT>;
     constexpr bool PAIR = S::kPair;
     constexpr int kCtas = PAIR ? 2 : 1;
+    // K steps of a part of a tile, at least.  Joining wide parts costs more (T = 200,
+    // two experts, H = 4096, I = 1536: parts of 4 steps 47 us, 8 39, uncut 39; one
+    // token, two experts of 16, H = 2048, I = 768: parts of 4 steps 12.8, 8 14.0).
+    constexpr int kMinPart = PAIR ? 16 : 4;
     constexpr int kJoin = PAIR ? 1 : 4;                      // parts in flight when a tile is joined
     constexpr int kColStep = S::kEpi / 4 * kMx4Chunk;        // columns between an epilogue warp's chunks
     extern __shared__ __align__(1024) unsigned char smem_mx4[];
@@ -431,14 +434,14 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     // CTA (or pair) c of G takes the tiles c, c + G, ...  When there are fewer tiles
     // than CTAs (a few tokens), K is cut into `parts` equal parts of at least
-    // kMx4MinPart steps and CTA c takes part c % parts of tile c / parts: one token at
+    // kMinPart steps and CTA c takes part c % parts of tile c / parts: one token at
     // H = 2048, I = 768, 8 experts has 48 gate/up tiles of 16 steps (3 parts) and 64
     // down tiles of 6 (1 part).  Cutting up the last, partial wave of many tiles the
     // same way costs more in joining than it evens out (T = 2048: 225 us against 215,
     // T = 1024 at H = 1024, I = 512, 32 experts: 42 against 35).
     const int grid = static_cast<int>(gridDim.x) / kCtas, cta = static_cast<int>(blockIdx.x) / kCtas;
     const int tiles = s_misc[0];
-    const int parts = max(1, min(grid / max(tiles, 1), nkb / kMx4MinPart));
+    const int parts = max(1, min(grid / max(tiles, 1), nkb / kMinPart));
 
     struct Tile {
         int unit;                                  // tile * parts + part

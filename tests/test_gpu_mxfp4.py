@@ -124,6 +124,8 @@ SHAPES = [  # tokens, hidden, inter, experts, top_k
     (200, 640, 640, 120, 8), (380, 384, 1152, 100, 8), (600, 256, 1280, 100, 6), (4100, 1152, 896, 4, 2),
     # as many experts as the tables hold
     (70, 128, 128, 1024, 8), (1, 8192, 64, 2, 1),
+    # wide tiles whose K is cut up: in the first product, in the second
+    (120, 4096, 128, 1, 1), (120, 128, 4096, 1, 1),
 ]
 
 
