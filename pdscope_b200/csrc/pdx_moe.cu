@@ -1191,14 +1191,21 @@ int launch_block_norm(const BlockNormArgs& a, int64_t T, bool fp32, cudaStream_t
                      reinterpret_cast<uintptr_t>(a.stream) | reinterpret_cast<uintptr_t>(a.normed);
     if (a.gate && a.gate_col == 1) bits |= reinterpret_cast<uintptr_t>(a.gate) | static_cast<uintptr_t>(a.gate_row * 2);
     const bool vec = a.H % 8 == 0 && (bits & 15u) == 0;
-    const bool early = !vec || a.H > 4096 || T <= 4 * kPlanSMs;   // few rows, or few rows to an SM
-    const int ch = early ? 1 : 2;
+    const bool early = T <= 4 * kPlanSMs || (!vec && a.H > 4096);   // few rows, or few rows to an SM
+    const int ch = early || !vec ? 1 : 2;
     const dim3 grid(static_cast<unsigned>(T)), block(static_cast<unsigned>((a.H + 256 * ch - 1) / (256 * ch) * 32));
     auto launch = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, stream, a); };
     auto launch_as = [&](auto res) {
         using RES = decltype(res);
-        if (!vec) return launch(k_block_norm<RES, COMBINE, false, 1, 1024, true>);
-        if (!early) return launch(k_block_norm<RES, COMBINE, true, 2, 256, false>);
+        if (!vec) {
+            if (early) return launch(k_block_norm<RES, COMBINE, false, 1, 1024, true>);
+            if (a.H > 2048) return launch(k_block_norm<RES, COMBINE, false, 1, 512, false>);
+            return launch(k_block_norm<RES, COMBINE, false, 1, 256, false>);
+        }
+        if (!early) {
+            if (a.H > 4096) return launch(k_block_norm<RES, COMBINE, true, 2, 512, false>);
+            return launch(k_block_norm<RES, COMBINE, true, 2, 256, false>);
+        }
         if (a.H > 2048) return launch(k_block_norm<RES, COMBINE, true, 1, 1024, true>);
         return launch(k_block_norm<RES, COMBINE, true, 1, 256, true>);
     };
