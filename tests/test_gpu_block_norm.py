@@ -65,7 +65,8 @@ def _check(got, y, residual, options):
 
 
 @pytest.mark.parametrize("tokens,hidden", ((1, 1), (3, 7), (2, 8), (5, 1003), (4, 1032), (33, 2048), (1, 4096), (2, 5003),
-                                           (3, 8192), (300, 96)))
+                                           (3, 8192), (300, 96), (700, 1), (700, 13), (700, 260), (601, 2041), (600, 4099),
+                                           (597, 8175), (597, 8190)))
 @pytest.mark.parametrize("residual", (torch.bfloat16, torch.float32))
 @pytest.mark.parametrize("post,pre,gate,act", (("rms", "rms", "none", "none"), ("layer", "rms", "token", "sigmoid"),
                                                ("none", "layer", "channel", "none"), ("rms", "none", "full", "sigmoid"),
