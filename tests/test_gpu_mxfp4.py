@@ -231,6 +231,47 @@ def test_slots_empty_experts_and_spare_rows(pdx):
     assert (out[:a] == 7).all() and (out[b:] == 7).all()
 
 
+@pytest.mark.parametrize("tokens", (2, 60, 400))      # the three token tiles
+def test_active_list_may_name_empty_experts(pdx, tokens):
+    slab, qs = _slab(pdx, 6, 256, 128, seed=12)
+    x = torch.randn(tokens, 256, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    sel = _selected(tokens, 6, 2, seed=3, only=[1, 4])
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 6)
+    want = pdx.moe_ffn_mxfp4(x, packed, slab)
+    _check_rows(want, x, packed, qs, 6)
+    n = min(6, packed.tokens.shape[0])                   # every expert, the empty ones too
+    packed.active[:n + 1] = torch.tensor([n, 0, 1, 2, 3, 4, 5][:n + 1], dtype=torch.int32)
+    if n == 6:
+        assert torch.equal(pdx.moe_ffn_mxfp4(x, packed, slab), want)
+
+
+@pytest.mark.parametrize("tokens", (1, 60, 400))
+def test_inputs_written_just_before_the_call(pdx, tokens):
+    """Weights, routing and activations written on the same stream right before:
+    the launches that start early must not read what was there."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    sets = []
+    for i in range(2):
+        slab, qs = _slab(pdx, 8, 512, 256, seed=20 + i)
+        x = torch.randn(tokens, 512, device="cuda", generator=gen).to(torch.bfloat16)
+        sel = _selected(tokens, 8, 2, seed=30 + i)
+        packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 8)
+        sets.append((slab, x, sel, pdx.moe_ffn_mxfp4(x, packed, slab)))
+    slab, x = pdx.Mxfp4ExpertSlab(8, 512, 256, "cuda"), torch.empty_like(sets[0][1])
+    sel, ones = torch.empty_like(sets[0][2]), torch.ones(sets[0][2].shape, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    got = []
+    for i in range(12):
+        src = sets[i % 2]
+        sel.copy_(src[2])
+        x.copy_(src[1])
+        slab.scales.copy_(src[0].scales)
+        slab.codes.copy_(src[0].codes)
+        got.append(pdx.moe_ffn_mxfp4(x, pdx.pack(sel, ones, 8), slab))
+    for i, y in enumerate(got):
+        assert torch.equal(y, sets[i % 2][3]), i
+
+
 def test_bad_slot_and_bad_token_are_reported(pdx):
     from pdscope_b200 import runtime
     slab, qs = _slab(pdx, 4, 256, 128, seed=11)
