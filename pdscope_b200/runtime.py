@@ -609,6 +609,8 @@ class ResidentMoELayer:
         dev = x.device
         if x.shape[1] != self.hidden:
             raise ValueError("activation and expert hidden sizes differ")
+        if dev != self.gate.device:
+            raise ValueError("x must be on the router's device")
         if outputs is None:
             outputs = LayerOutputs(
                 out=torch.empty((t_count, self.hidden), dtype=torch.bfloat16, device=dev),
@@ -619,11 +621,10 @@ class ResidentMoELayer:
         if workspace is None:
             workspace = _scratch(self.slab, dev, self.workspace_bytes(t_count, mode), "layer")
         layer = lib.pdx_mxfp4_moe_layer if is_mxfp4(self.slab) else lib.pdx_moe_layer
-        check(layer(_ptr(x), _ptr(self.gate), t_count, self.hidden, self.experts, self.top_k,
-                    int(self.normalize), ctypes.byref(self.slab.struct), self.inter, _ptr(residual),
-                    _ptr(outputs.out), _ptr(outputs.logits), _ptr(outputs.selected),
-                    _ptr(outputs.weights), _ptr(outputs.counts), mode, _ptr(workspace),
-                    workspace.numel(), _stream()))
+        _call(dev, layer, _ptr(x), _ptr(self.gate), t_count, self.hidden, self.experts, self.top_k,
+              int(self.normalize), ctypes.byref(self.slab.struct), self.inter, _ptr(residual), _ptr(outputs.out),
+              _ptr(outputs.logits), _ptr(outputs.selected), _ptr(outputs.weights), _ptr(outputs.counts), mode,
+              _ptr(workspace), workspace.numel())
         return outputs
 
 
@@ -654,7 +655,8 @@ class PDScopeCudaRuntime:
     """Layer-level drop-in for ``PDScopeCudaRuntime.forward`` with HBM-resident experts.
 
     ``layers`` maps layer index -> ExpertSlab or Mxfp4ExpertSlab (slot e =
-    expert e, or an explicit ``slot_of_expert``).  ``forward`` keeps the reference's signature,
+    expert e, or an explicit ``slot_of_expert``).  ``forward`` keeps the
+    reference's signature,
     checks and return value ``(output, Routing, row)``
     (expertbench/pdscope_runtime.py:208-512); ``row`` carries the keys the
     reference harness reads (benchmarks/pdscope_compare.py:412-420).
