@@ -759,6 +759,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
             if (lane == 0) prev = ticket_acq_rel(&args.tickets[(t.index * kCtas + rank) * S::kEpi + warp - 2]);
             prev = __shfl_sync(0xffffffffu, prev, 0);
             if (prev != static_cast<unsigned int>(parts - 1)) continue;
+            __syncwarp();   // lane 0 acquired the other CTAs' parts; this orders it before the reads of all lanes
             for (int col = col0; col < ne; col += kColStep) {
                 const int n = min(kMx4Chunk, ne - col);
                 float g[kMx4Chunk], u[kMx4Chunk];

@@ -371,3 +371,22 @@ def test_runtime_forward_on_mxfp4(pdx):
     out, routing, row = rt.forward(x, gate, layer=0, step=0, top_k=2)
     assert torch.equal(out, pdx.ResidentMoELayer(gate, slab, top_k=2).forward(x).out)
     assert row["counters"]["gpu_completed_experts"] == len(row["token_counts"])
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", ((1, 2048, 768, 16, 8), (3, 1024, 1024, 4, 2),
+                                                               (120, 4096, 128, 1, 1), (120, 128, 4096, 1, 1)))
+def test_joined_parts_repeat(pdx, tokens, hidden, inter, experts, top_k):
+    """Tiles whose K is cut up between CTAs, back to back: every join reads the
+    parts of its own call, whichever CTA comes last."""
+    slab, qs = _slab(pdx, experts, hidden, inter, seed=21)
+    sets = []
+    for i in range(2):
+        x = torch.randn(tokens, hidden, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).cuda()
+        sel = _selected(tokens, experts, top_k, seed=i)
+        packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), experts)
+        want = pdx.moe_ffn_mxfp4(x, packed, slab)
+        _check_rows(want, x, packed, qs, experts)
+        sets.append((x, packed, want))
+    outs = [pdx.moe_ffn_mxfp4(*sets[i % 2][:2], slab) for i in range(200)]
+    for i, out in enumerate(outs):
+        assert torch.equal(out, sets[i % 2][2]), i
