@@ -367,6 +367,20 @@ class BlockNorm:
             a.gate_row, a.gate_col = g.stride()
         return a
 
+    def state(self):
+        """Everything ``args`` puts into a launch: two equal states launch alike
+        as long as the memory of the tensors in them lives (``tensors``)."""
+        return (self.post, self.pre, self.gate_act, self.residual_scale, self.block_scale, self.eps,
+                _tensor_state(self.post_weight), _tensor_state(self.gate), _tensor_state(self.pre_weight))
+
+    def tensors(self):
+        """The norm's tensors, as views that keep their present memory alive."""
+        return [t.detach() for t in (self.post_weight, self.gate, self.pre_weight) if isinstance(t, torch.Tensor)]
+
+
+def _tensor_state(t):
+    return (t.data_ptr(), t.shape, t.stride(), t.dtype) if isinstance(t, torch.Tensor) else t
+
 
 def _norm_weight(name, w, norm, hidden, device):
     if w is None:

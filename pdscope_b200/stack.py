@@ -70,6 +70,7 @@ class ResidentMoEStack:
         self.top_k, self.normalize = top_k, normalize
         self.device = self.gates[0].device
         self._graphs = {}
+        self._captured = {}       # graph key -> the norms' states at the capture, and their tensors
         self._bufs = {}
 
     @property
@@ -211,19 +212,28 @@ class ResidentMoEStack:
 
         With ``counts_to_host`` the step ends with one asynchronous copy of every
         layer's routed-token counts into pinned host memory (``expert_counts``
-        reads them once the step has finished)."""
+        reads them once the step has finished).
+
+        With ``graph`` the first step of a size captures a CUDA graph that later
+        steps replay.  A step after ``norms`` changed (a field, or a ``BlockNorm``
+        put in place of another) captures again, which takes far longer than a
+        step; a gate that differs from step to step is best written in place."""
         if not graph:
             self._step_fused(t_count, mode, counts_to_host)
         else:
             key = ("fused", t_count, mode, counts_to_host)
             g = self._graphs.get(key)
-            if g is None:
+            # a capture holds the norms' pointers and scalars
+            norms = [n.state() for n in self.norms] if self.norms is not None else None
+            if g is None or (norms is not None and self._captured[key][0] != norms):
                 self._step_fused(t_count, mode, counts_to_host)  # warm: device attributes, tensor maps
                 torch.cuda.synchronize(self.device)
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g):
                     self._step_fused(t_count, mode, counts_to_host)
                 self._graphs[key] = g
+                if norms is not None:
+                    self._captured[key] = norms, [n.tensors() for n in self.norms]
             g.replay()
         if counts_to_host:
             self.buffers(t_count, mode)["counts_ready"].record()
@@ -291,6 +301,7 @@ class ResidentMoEStack:
 
     def release_graphs(self):
         self._graphs.clear()
+        self._captured.clear()
 
 
 class ExpertLoadTracker:

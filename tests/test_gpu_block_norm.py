@@ -228,3 +228,97 @@ def test_two_layer_protocol_on_mxfp4(pdx, tokens):
         x = residual_layernorm(pdx.ResidentMoELayer(gate, slab, top_k=2).forward(x).out, x)
     assert torch.equal(stack.output(tokens), x)
     stack.release_graphs()
+
+
+def _norm_stack(pdx, layers=2, hidden=128, experts=4, mx=True, seed=5):
+    from pdscope_b200.stack import ResidentMoEStack
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    gates = [(torch.randn(experts, hidden, device="cuda", generator=gen) * 0.05).to(torch.bfloat16)
+             for _ in range(layers)]
+    slabs = [pdx.ExpertSlab.allocate(experts, hidden, 64, "cuda", std=0.1, generator=gen) for _ in range(layers)]
+    if mx:
+        slabs = [pdx.Mxfp4ExpertSlab.from_slab(s) for s in slabs]
+    norms = [pdx.BlockNorm(post="rms", residual_scale=0.9, block_scale=0.5) for _ in range(layers + 1)]
+    return ResidentMoEStack(gates, slabs, top_k=2, norms=norms)
+
+
+def _both(stack, tokens):
+    """Outputs of the captured step and of the step without a graph."""
+    got = []
+    for graph in (True, False):
+        stack.output(tokens).zero_()
+        stack.residual(tokens).zero_()
+        stack.step(tokens, graph=graph)
+        got.append((stack.output(tokens).clone(), stack.residual(tokens).clone()))
+    return got
+
+
+@pytest.mark.parametrize("mx", (False, True))
+def test_captured_step_follows_its_norms(pdx, mx):
+    """Scales, norm kinds, eps, weights and gates changed between two steps: the
+    captured step gives what the step without a graph gives."""
+    stack, tokens = _norm_stack(pdx, mx=mx), 6
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    stack.input(tokens).copy_(torch.randn(tokens, 128, device="cuda", generator=gen))
+    vector = lambda *shape: torch.randn(*shape, device="cuda", generator=gen).to(torch.bfloat16)
+    kept = [vector(tokens, 1), vector(tokens, 1), vector(tokens, 128)]      # all alive throughout
+    changes = [None, dict(residual_scale=0.5), dict(block_scale=-2.0), dict(pre="layer"), dict(post="none"),
+               dict(post="layer", eps=0.5), dict(pre_weight=vector(128)), dict(pre_weight=vector(128)),
+               dict(gate=kept[0]), dict(gate=kept[1]), dict(gate_act="sigmoid"), dict(gate=kept[2]),
+               dict(gate=kept[2][:, :1]), dict(gate=kept[2][0]), dict(gate=None)]
+    previous = None
+    for change in changes:
+        for name, value in (change or {}).items():
+            setattr(stack.norms[1], name, value)
+        graph, eager = _both(stack, tokens)
+        assert torch.equal(graph[0], eager[0]) and torch.equal(graph[1], eager[1]), change
+        assert previous is None or not torch.equal(eager[0], previous) or change == dict(gate_act="sigmoid"), change
+        previous = eager[0]
+    stack.norms[0] = pdx.BlockNorm(residual_scale=3.0, pre="none")
+    graph, eager = _both(stack, tokens)
+    assert torch.equal(graph[0], eager[0]) and torch.equal(graph[1], eager[1])
+    stack.release_graphs()
+
+
+def test_captured_step_keeps_its_gates(pdx):
+    """A gate replaced every step, the old one dropped: each step reads its own.
+    A gate written in place needs no new capture."""
+    stack, tokens = _norm_stack(pdx), 6
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    stack.input(tokens).copy_(torch.randn(tokens, 128, device="cuda", generator=gen))
+    for i in range(4):
+        stack.norms[1].gate = torch.randn(tokens, 1, device="cuda", generator=gen).to(torch.bfloat16)
+        stack.step(tokens)
+        got = stack.output(tokens).clone()
+        junk = [torch.full((tokens, 1), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(8)]
+        stack.step(tokens)
+        stack.step(tokens, graph=False)
+        assert torch.equal(got, stack.output(tokens)), i
+        del junk
+    stack.step(tokens)
+    graphs = dict(stack._graphs)
+    stack.norms[1].gate.fill_(0.25)
+    graph, eager = _both(stack, tokens)
+    assert torch.equal(graph[0], eager[0]) and not torch.equal(graph[0], got)
+    assert stack._graphs == graphs and len(graphs) == 1
+    stack.release_graphs()
+
+
+def test_captured_step_refuses_bad_norms(pdx):
+    """A norm that no longer fits is refused, not replayed from the capture; set
+    right again, the step runs."""
+    stack, tokens = _norm_stack(pdx), 6
+    stack.input(tokens).fill_(0.5)
+    stack.step(tokens)
+    want = stack.output(tokens).clone()
+    good = stack.norms[1]
+    for bad in (dict(gate=torch.zeros(5, 1, dtype=torch.bfloat16, device="cuda")), dict(post="batch"), dict(eps=0.0),
+                dict(pre_weight=torch.ones(64, dtype=torch.bfloat16, device="cuda"))):
+        stack.norms[1] = pdx.BlockNorm(**dict(dict(post="rms", residual_scale=0.9, block_scale=0.5), **bad))
+        with pytest.raises(ValueError):
+            stack.step(tokens)
+        stack.norms[1] = good
+        stack.output(tokens).zero_()
+        stack.step(tokens)
+        assert torch.equal(stack.output(tokens), want)
+    stack.release_graphs()
