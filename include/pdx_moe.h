@@ -372,10 +372,10 @@ int pdx_mxfp4_moe_layer(const void *x, const void *gate, int64_t T, int64_t H, i
  * ((v - mean) / sqrt(var + eps), population variance); weights BF16 [H] or
  * NULL (ones).  gate: BF16 with element strides gate_row, gate_col (0 =
  * broadcast), or NULL; gate_sigmoid applies the logistic function to it.
- * y BF16 [T, H], or NULL: s = residual_scale * residual.  residual and
- * stream_out are FP32 if residual_fp32, else BF16; normed_out is BF16; either
- * output may be NULL and may alias y or residual of the same type.
- * 1 <= H <= 8192. */
+ * y BF16 [T, H], or NULL: s = residual_scale * residual, and post, gate and
+ * block_scale do not enter.  residual and stream_out are FP32 if
+ * residual_fp32, else BF16; normed_out is BF16; either output may be NULL and
+ * may alias y or residual of the same type.  1 <= H <= 8192. */
 #define PDX_NORM_NONE 0
 #define PDX_NORM_RMS 1
 #define PDX_NORM_LAYER 2

@@ -1638,6 +1638,10 @@ int pdx_block_norm(const void* y, const void* residual, int64_t T, int64_t H, co
     if (st) return st;
     BlockNormArgs a = to_block_norm(args, residual, H, stream_out, normed_out);
     a.y = static_cast<const uint16_t*>(y);
+    if (!y) {   // no block: its gate and scale do not enter, 0 * inf would
+        a.gate = nullptr;
+        a.block_scale = 0.f;
+    }
     st = launch_block_norm<false>(a, T, args->residual_fp32 != 0, stream);
     return st ? st : ok();
 }

@@ -452,7 +452,8 @@ def block_norm(y, residual, *, norm=None, stream_out=None, out=None, **options):
     the next block in one pass; returns ``(stream, normed)``.
 
     ``y`` [T, H] BF16 is the block's output (None: ``s = residual_scale *
-    residual``, the norm before a first block), ``residual`` [T, H] BF16 or
+    residual``, the norm before a first block; post, gate and block scale do not
+    enter), ``residual`` [T, H] BF16 or
     FP32.  The options are ``BlockNorm``'s fields, or ``norm=BlockNorm(...)``.
     ``stream`` has residual's type, ``normed`` is BF16; ``stream_out`` and
     ``out`` may be ``y`` or ``residual``."""

@@ -322,3 +322,18 @@ def test_captured_step_refuses_bad_norms(pdx):
         stack.step(tokens)
         assert torch.equal(stack.output(tokens), want)
     stack.release_graphs()
+
+
+@pytest.mark.parametrize("tokens", (4, 700))
+@pytest.mark.parametrize("hidden", (264, 1003))
+def test_without_a_block_its_terms_do_not_apply(pdx, tokens, hidden):
+    """y = None: neither the gate nor the block scale enters, whatever they hold."""
+    t = _inputs(tokens, hidden, torch.float32, "full", seed=5)
+    t["gate"][0, 1], t["gate"][1, 2], t["gate"][2, 3] = float("inf"), float("nan"), float("-inf")
+    options = dict(pre_weight=t["pre_weight"], residual_scale=0.5)
+    want = pdx.block_norm(None, t["residual"], **options)
+    _check(want, None, _f64(t["residual"]), options)
+    for extra in (dict(gate=t["gate"]), dict(gate=t["gate"], gate_act="sigmoid"), dict(gate=t["gate"][1, 2]),
+                  dict(block_scale=float("inf")), dict(block_scale=float("nan"), post="layer")):
+        got = pdx.block_norm(None, t["residual"], **options, **extra)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), list(extra)
