@@ -347,7 +347,11 @@ typedef struct pdx_mxfp4_weights {
 /* pdx_moe_ffn_grouped on MXFP4 experts:
  *   y[p] = bf16( Wd (silu(Wg x) * (Wu x)) ),  x = x[tokens[p]] (BF16)
  * with exactly dequantised weights, FP32 sums and one rounding at the end.
- * H, I multiples of 32; rows of no active expert are left as they are. */
+ * H, I multiples of 32; rows of no active expert are left as they are.
+ * active may list experts without rows, in any order.  A list of more than E
+ * entries, ids outside [0, E), offsets that fall or leave [0, rows], and experts
+ * listed again until there is more work than a batch has raise
+ * PDX_DEVERR_BAD_EXPERT, and rows that only those name may stay as they are. */
 size_t pdx_mxfp4_ffn_workspace_bytes(int64_t rows, int64_t E, int64_t H, int64_t I);
 int pdx_mxfp4_ffn_grouped(const void *x, int64_t T, const int32_t *tokens, const int32_t *offsets,
                           const int32_t *active, int64_t E, int64_t rows, const pdx_mxfp4_weights *weights,

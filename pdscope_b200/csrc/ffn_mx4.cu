@@ -185,7 +185,8 @@ struct Mx4Args {
     uint8_t* h;                     // [2][rows][M] pieces (SWIGLU)
     uint16_t* y;                    // [rows, ldy] (down)
     int ldy;                        // H
-    int stages, table;              // ring stages, entries of the expert tables (mx4_layout)
+    int stages, table;              // ring stages, entries of the expert tables: E
+    int max_tiles;                  // token tiles that sf has room for
     float* partials;                // [gridDim.x][2 NT][128]
     unsigned int* tickets;          // [CTAs * epilogue warps], zero on entry
 };
@@ -404,17 +405,26 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     // The routing tables are older than the launch before this one, which has
     // passed its own wait by the time this one starts; only that launch's
     // output (the token pieces) has to be waited for, by the warps that read it.
-    const int n_active = max(0, min(__ldcg(args.active), args.table));
+    // The list may name experts without rows, but none outside [0, E) and no more
+    // than E; an expert's rows lie in [0, rows).  What breaks that has no rows here.
+    const int listed = __ldcg(args.active), n_active = max(0, min(listed, args.table));
+    if (listed != n_active && threadIdx.x == 0) raise_error(PDX_DEVERR_BAD_EXPERT);
     for (int i = static_cast<int>(threadIdx.x); i < n_active; i += S::kThreads) {
-        const int e = __ldcg(args.active + 1 + i);
-        const int seg0 = __ldcg(args.offsets + e);
+        int e = __ldcg(args.active + 1 + i);
+        const bool known = e >= 0 && e < args.table;
+        if (!known) e = 0;
+        int seg0 = __ldcg(args.offsets + e), end = __ldcg(args.offsets + e + 1);
+        if (!known || seg0 < 0 || end < seg0 || end > args.rows) {
+            raise_error(PDX_DEVERR_BAD_EXPERT);
+            seg0 = end = 0;
+        }
         int64_t slot = args.slot_of_expert ? __ldcg(args.slot_of_expert + e) : e;
         if (slot < 0 || slot >= args.num_slots) {
             raise_error(PDX_DEVERR_BAD_SLOT);
             slot = 0;
         }
         t_seg0[i] = seg0;
-        t_rows[i] = __ldcg(args.offsets + e + 1) - seg0;
+        t_rows[i] = end - seg0;
         t_slot[i] = static_cast<int>(slot);
     }
     tc_fence_before();
@@ -422,7 +432,10 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     tc_fence_after();
     if (warp == 2) {
         const int total = warp_tile_prefix(n_active, prefix, [&](int a) { return (t_rows[a] + NT - 1) / NT; });
-        if (lane == 0) s_misc[0] = total * m_tiles;
+        if (lane == 0) {
+            if (total > args.max_tiles) raise_error(PDX_DEVERR_BAD_EXPERT);   // an expert listed again and again
+            s_misc[0] = min(total, args.max_tiles) * m_tiles;
+        }
     }
     __syncwarp();
     if (PAIR)

@@ -1126,7 +1126,8 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     gu.scale_stride = ss;
     gu.tiles_per_slot = tps;
     gu.rows = n;
-    gu.table = static_cast<int>(std::min(E, rows));
+    gu.table = static_cast<int>(E);
+    gu.max_tiles = static_cast<int>(b.tiles);
     gu.row_scale = b.row_scale;
     gu.sf = b.sf;
     gu.h = b.h;

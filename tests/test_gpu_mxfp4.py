@@ -390,3 +390,63 @@ def test_joined_parts_repeat(pdx, tokens, hidden, inter, experts, top_k):
     outs = [pdx.moe_ffn_mxfp4(*sets[i % 2][:2], slab) for i in range(200)]
     for i, out in enumerate(outs):
         assert torch.equal(out, sets[i % 2][2]), i
+
+
+@pytest.mark.parametrize("tokens,experts", ((1, 6), (2, 6), (8, 6), (2, 1024), (40, 6), (400, 6)))
+def test_active_list_longer_than_the_rows(pdx, tokens, experts):
+    """Every expert listed, the empty ones first: those with rows still run."""
+    slab, qs = _slab(pdx, experts, 128, 128, seed=12)
+    x = torch.randn(tokens, 128, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    sel = _selected(tokens, experts, 2, seed=3, only=[1, 4])
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), experts)
+    want = pdx.moe_ffn_mxfp4(x, packed, slab)
+    _check_rows(want, x, packed, qs, experts)
+    ids = torch.arange(experts - 1, -1, -1, dtype=torch.int32)
+    packed.active.copy_(torch.cat([torch.tensor([experts], dtype=torch.int32), ids]))
+    out = torch.full_like(want, 7.0)
+    assert torch.equal(pdx.moe_ffn_mxfp4(x, packed, slab, out=out), want)
+
+
+@pytest.mark.parametrize("tokens", (2, 60, 400))      # the three token tiles
+@pytest.mark.parametrize("active", ((2, 1, 1), (2, 1, 99), (2, 1, 6), (1, -1), (7, 0, 1, 2, 3, 4, 5), (6, 1, 1, 1, 1, 1, 1)))
+def test_bad_active_lists_are_reported(pdx, tokens, active):
+    """Ids out of range, more entries than experts, an expert named again and
+    again: an error word, and nothing outside the rows is touched."""
+    from pdscope_b200 import runtime
+    slab, _ = _slab(pdx, 6, 128, 128, seed=12)
+    x = torch.randn(tokens, 128, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    sel = _selected(tokens, 6, 2, seed=3, only=[1, 4])
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 6)
+    want = pdx.moe_ffn_mxfp4(x, packed, slab)
+    good = packed.active.clone()
+    packed.active[:len(active)] = torch.tensor(active, dtype=torch.int32)
+    guard = torch.full((2 * tokens + 2, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    pdx.moe_ffn_mxfp4(x, packed, slab, out=guard[1:-1])
+    assert (guard[0] == 7).all() and (guard[-1] == 7).all()
+    if active == (2, 1, 1):                               # the same rows twice, the same values
+        a, b = packed.offsets[1].item(), packed.offsets[2].item()
+        assert torch.equal(guard[1 + a:1 + b], want[a:b])
+    else:
+        with pytest.raises(ValueError, match="expert ID"):
+            runtime.raise_device_error()
+    runtime.raise_device_error()
+    packed.active.copy_(good)
+    assert torch.equal(pdx.moe_ffn_mxfp4(x, packed, slab), want)
+
+
+@pytest.mark.parametrize("tokens", (2, 400))
+def test_bad_offsets_are_reported(pdx, tokens):
+    from pdscope_b200 import runtime
+    slab, _ = _slab(pdx, 6, 128, 128, seed=12)
+    x = torch.randn(tokens, 128, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    sel = _selected(tokens, 6, 2, seed=3, only=[1, 4])
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 6)
+    good = packed.offsets.clone()
+    for bad in ((5, 2 * tokens + 1), (1, -1), (2, -5)):       # past the rows, before them, falling
+        packed.offsets.copy_(good)
+        packed.offsets[bad[0]] = bad[1]
+        guard = torch.full((2 * tokens + 2, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+        pdx.moe_ffn_mxfp4(x, packed, slab, out=guard[1:-1])
+        assert (guard[0] == 7).all() and (guard[-1] == 7).all()
+        with pytest.raises(ValueError, match="expert ID"):
+            runtime.raise_device_error()
