@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import Mxfp4Weights, lib
-from .runtime import PROJECTIONS, Packed, _call, _require_cuda_bf16, ffn_workspace_bytes
+from .runtime import PROJECTIONS, Packed, _call, _require_cuda_bf16, check_slab, ffn_workspace_bytes
 
 BLOCK = 32
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
@@ -202,12 +202,9 @@ def moe_ffn_mxfp4(x, packed, slab, out=None):
     t_count, hidden = x.shape
     if not isinstance(slab, Mxfp4ExpertSlab) or not isinstance(packed, Packed):
         raise ValueError("moe_ffn_mxfp4 needs pack()'s result and an Mxfp4ExpertSlab")
-    if hidden != slab.hidden:
-        raise ValueError("activation and expert hidden sizes differ")
     experts = packed.counts.shape[0]
-    if (slab.slot_of_expert.shape[0] if slab.slot_of_expert is not None else slab.num_slots) < experts:
-        raise ValueError("the slab holds fewer experts than the routing names")
-    if packed.tokens.device != x.device or slab.codes.device != x.device:
+    check_slab(slab, experts, hidden, x.device)
+    if packed.tokens.device != x.device:
         raise ValueError("x, the packing and the slab must be on one device")
     rows = packed.tokens.shape[0]
     if t_count < 1 or rows % t_count:

@@ -554,6 +554,20 @@ def is_mxfp4(slab):
     return isinstance(slab.struct, _lib.Mxfp4Weights)
 
 
+def check_slab(slab, experts, hidden, device):
+    """Refuse a slab on which a router of ``experts`` experts over ``hidden``
+    channels on ``device`` cannot run."""
+    if slab.hidden != hidden:
+        raise ValueError("activation and expert hidden sizes differ")
+    slots, mx = slab.slot_of_expert, is_mxfp4(slab)
+    # the device reads slot_of_expert[e] unchecked; without it a BF16 slab may hold the first experts only,
+    # and an expert behind them sets the error word
+    if (slots is not None and slots.shape[0] < experts) or (mx and slots is None and slab.num_slots < experts):
+        raise ValueError("the slab holds fewer experts than the routing names")
+    if (slab.codes if mx else slab.storage).device != device or (slots is not None and slots.device != device):
+        raise ValueError("the activations, the router and the slab must be on one device")
+
+
 def layer_workspace_bytes(slab, t_count, experts, top_k, mode=_lib.FFN_AUTO):
     """Workspace of one layer call on ``slab`` (BF16 or MXFP4 experts)."""
     if is_mxfp4(slab):
@@ -610,6 +624,7 @@ class ResidentMoELayer:
         _require_cuda_bf16("gate", gate, 2)
         if gate.shape[1] != slab.hidden:
             raise ValueError("router and expert hidden sizes differ")
+        check_slab(slab, gate.shape[0], gate.shape[1], gate.device)
         self.gate, self.slab = gate, slab
         self.experts, self.hidden = gate.shape
         self.inter = slab.inter
@@ -779,6 +794,7 @@ class PDScopeCudaRuntime:
         experts, hidden = gate.shape
         t_count = inputs.shape[0]
         dev = inputs.device
+        check_slab(slab, experts, inputs.shape[1], dev)
         routing = route(inputs, gate, top_k, normalize)
         p = pack(routing.selected, routing.weights, experts)
         offsets = p.offsets.cpu()                # synchronises, as the reference's grouping does (:26)

@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .runtime import (LN_EPS, BlockNorm, ExpertSlab, _ptr, _stream, block_norm, combine_block_norm,
+from .runtime import (LN_EPS, BlockNorm, ExpertSlab, _ptr, _stream, block_norm, check_slab, combine_block_norm,
                       ffn_workspace_bytes, grouped_ffn, is_mxfp4, layer_workspace_bytes)
 
 
@@ -66,7 +66,11 @@ class ResidentMoEStack:
         self.norms, self.residual_dtype = list(norms) if norms is not None else None, residual_dtype
         self.gates, self.slabs = list(gates), list(slabs)
         self.experts, self.hidden = self.gates[0].shape
-        self.inter = self.slabs[0].inter
+        self.inter = self.slabs[0].inter          # of the first layer; each layer runs on its slab's own
+        for gate, slab in zip(self.gates, self.slabs):
+            if gate.shape != self.gates[0].shape or gate.device != self.gates[0].device:
+                raise ValueError("the routers of a stack must be alike and on one device")
+            check_slab(slab, self.experts, self.hidden, gate.device)
         self.top_k, self.normalize = top_k, normalize
         self.device = self.gates[0].device
         self._graphs = {}
@@ -138,13 +142,13 @@ class ResidentMoEStack:
                 args = self.norms[l + 1].args(t_count, self.hidden, self.residual_dtype, self.device)
                 check(lib.pdx_moe_block(_ptr(x_in), _ptr(self.gates[l]), t_count, self.hidden, self.experts, self.top_k,
                                         int(self.normalize), *((None, weights) if is_mxfp4(slab) else (weights, None)),
-                                        self.inter, _ptr(stream), ctypes.byref(args), _ptr(stream), _ptr(x_out),
+                                        slab.inter, _ptr(stream), ctypes.byref(args), _ptr(stream), _ptr(x_out),
                                         _ptr(st.logits), _ptr(st.selected), _ptr(st.weights), _ptr(st.counts), mode,
                                         _ptr(ws), ws.numel(), s))
                 continue
             layer = lib.pdx_mxfp4_moe_layer if is_mxfp4(slab) else lib.pdx_moe_layer
             check(layer(_ptr(x_in), _ptr(self.gates[l]), t_count, self.hidden, self.experts,
-                        self.top_k, int(self.normalize), weights, self.inter,
+                        self.top_k, int(self.normalize), weights, slab.inter,
                         _ptr(x_in), _ptr(x_out), _ptr(st.logits), _ptr(st.selected),
                         _ptr(st.weights), _ptr(st.counts), mode | _lib.LAYER_OUT_NORM, _ptr(ws),
                         ws.numel(), s))

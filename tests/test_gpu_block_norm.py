@@ -337,3 +337,50 @@ def test_without_a_block_its_terms_do_not_apply(pdx, tokens, hidden):
                   dict(block_scale=float("inf")), dict(block_scale=float("nan"), post="layer")):
         got = pdx.block_norm(None, t["residual"], **options, **extra)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), list(extra)
+
+
+@pytest.mark.parametrize("mx", (False, True))
+@pytest.mark.parametrize("with_norms", (False, True))
+@pytest.mark.parametrize("inters", ((128, 320), (320, 96, 128)))
+def test_stack_of_experts_of_several_sizes(pdx, mx, with_norms, inters):
+    """Layers whose experts differ in I: the fused step, its graph and the staged path agree with single layers."""
+    from pdscope_b200.runtime import residual_layernorm
+    from pdscope_b200.stack import ResidentMoEStack
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    experts, hidden, tokens = 4, 256, 9
+    gates = [(torch.randn(experts, hidden, device="cuda", generator=gen) * 0.05).to(torch.bfloat16) for _ in inters]
+    slabs = [pdx.ExpertSlab.allocate(experts, hidden, i, "cuda", std=0.1, generator=gen) for i in inters]
+    if mx:
+        slabs = [pdx.Mxfp4ExpertSlab.from_slab(s) for s in slabs]
+    norms = [pdx.BlockNorm(post="rms") for _ in range(len(inters) + 1)] if with_norms else None
+    stack = ResidentMoEStack(gates, slabs, top_k=2, norms=norms)
+    x = torch.randn(tokens, hidden, device="cuda", generator=gen).to(torch.bfloat16)
+    stack.input(tokens).copy_(x)
+    stack.stage_once(tokens)
+    want = stack.output(tokens).clone()
+    if not with_norms:
+        for gate, slab in zip(gates, slabs):
+            x = residual_layernorm(pdx.ResidentMoELayer(gate, slab, top_k=2).forward(x).out, x)
+        assert torch.equal(want, x)
+    for graph in (False, True):
+        stack.output(tokens).zero_()
+        stack.step(tokens, graph=graph)
+        assert torch.equal(stack.output(tokens), want)
+    stack.release_graphs()
+
+
+def test_layer_and_runtime_refuse_short_slabs(pdx):
+    """Slabs whose slots or slot table do not cover the router's experts, or of another hidden size."""
+    gate = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(2, 64, dtype=torch.bfloat16, device="cuda")
+    short = torch.zeros(3, dtype=torch.int32, device="cuda")
+    storage = torch.zeros(4 * 3 * 64 * 64, dtype=torch.bfloat16, device="cuda")
+    for slab in (pdx.Mxfp4ExpertSlab(3, 64, 64, "cuda"), pdx.Mxfp4ExpertSlab(4, 64, 64, "cuda", slot_of_expert=short),
+                 pdx.ExpertSlab(storage, 64, 64, slot_of_expert=short)):
+        with pytest.raises(ValueError, match="fewer experts"):
+            pdx.ResidentMoELayer(gate, slab)
+        with pytest.raises(ValueError, match="fewer experts"):
+            pdx.PDScopeCudaRuntime({0: slab}, top_k=2).forward(x, gate, layer=0, step=0, top_k=2)
+    wide = pdx.Mxfp4ExpertSlab(4, 128, 64, "cuda")
+    with pytest.raises(ValueError, match="hidden"):
+        pdx.PDScopeCudaRuntime({0: wide}, top_k=2).forward(x, gate, layer=0, step=0, top_k=2)

@@ -168,3 +168,28 @@ def test_expert_parallel_refuses_mxfp4():
     gate = torch.zeros(4, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="BF16 experts"):
         ExpertParallelMoE(gate, pdx.Mxfp4ExpertSlab(4, 64, 64, "cpu"), rank=0, world=1)
+
+
+def _bf16_slab(slots, hidden, inter, slot_of_expert=None):
+    """What a BF16 slab shows of itself, on the CPU (an ExpertSlab needs a CUDA tensor)."""
+    from types import SimpleNamespace
+    return SimpleNamespace(hidden=hidden, inter=inter, num_slots=slots, slot_of_expert=slot_of_expert,
+                           storage=torch.zeros(1, dtype=torch.bfloat16), struct=_lib.ExpertWeights())
+
+
+def test_stack_refuses_slabs_that_do_not_fit():
+    gate = torch.zeros(4, 64, dtype=torch.bfloat16)
+    slab, short = pdx.Mxfp4ExpertSlab(4, 64, 64, "cpu"), torch.zeros(3, dtype=torch.int32)
+    ResidentMoEStack([gate, gate], [slab, pdx.Mxfp4ExpertSlab(4, 64, 96, "cpu")])      # sizes of I may differ
+    ResidentMoEStack([gate, gate], [slab, _bf16_slab(4, 64, 96)])
+    for bad, match in ((pdx.Mxfp4ExpertSlab(4, 32, 64, "cpu"), "hidden"), (pdx.Mxfp4ExpertSlab(3, 64, 64, "cpu"), "fewer"),
+                       (pdx.Mxfp4ExpertSlab(4, 64, 64, "cpu", slot_of_expert=short), "fewer"),
+                       (pdx.Mxfp4ExpertSlab(4, 64, 64, "meta"), "device"),
+                       (_bf16_slab(4, 32, 64), "hidden"), (_bf16_slab(4, 64, 64, short), "fewer"),
+                       (_bf16_slab(4, 64, 64, torch.zeros(4, dtype=torch.int32, device="meta")), "device")):
+        with pytest.raises(ValueError, match=match):
+            ResidentMoEStack([gate, gate], [slab, bad])
+    with pytest.raises(ValueError, match="alike"):
+        ResidentMoEStack([gate, torch.zeros(5, 64, dtype=torch.bfloat16)], [slab, slab])
+    # fewer slots than experts is an error of the routing, not of a BF16 slab
+    ResidentMoEStack([gate], [_bf16_slab(3, 64, 64)])
