@@ -414,11 +414,12 @@ def _check_outputs(outputs, inputs, apart):
             if u is not None and _overlap(span, _span(u)) and (t.data_ptr() != u.data_ptr() or t.dtype != u.dtype):
                 raise ValueError("an output must be an input of its own type or lie apart from it")
         if any(_overlap(span, _span(u)) for u in apart if u is not None):
-            raise ValueError("the outputs must not overlap the expert rows or the gate")
+            raise ValueError("the outputs must not overlap the gate, a norm's weights, the expert rows, their weights "
+                             "or their order")
 
 
-def _block_norm_outputs(norm, options, y, residual, stream_out, out, rows=None):
-    """Checked (arguments, stream_out, out) of a block norm of ``y`` or of the combine of ``rows``."""
+def _block_norm_outputs(norm, options, y, residual, stream_out, out, combined=()):
+    """Checked (arguments, stream_out, out) of a block norm of ``y`` or of the combine of ``combined``."""
     if norm is None:
         norm = BlockNorm(**options)
     elif options or not isinstance(norm, BlockNorm):
@@ -442,9 +443,10 @@ def _block_norm_outputs(norm, options, y, residual, stream_out, out, rows=None):
         _require_cuda_bf16("out", out, 2)
         if out.shape != residual.shape or out.device != residual.device:
             raise ValueError("out must have residual's shape and device")
+    args = norm.args(*residual.shape, residual.dtype, residual.device)
     if not fresh:
-        _check_outputs((stream_out, out), (y, residual), (rows, norm.gate))
-    return norm.args(*residual.shape, residual.dtype, residual.device), stream_out, out
+        _check_outputs((stream_out, out), (y, residual), (*combined, norm.gate, norm.post_weight, norm.pre_weight))
+    return args, stream_out, out
 
 
 def block_norm(y, residual, *, norm=None, stream_out=None, out=None, **options):
@@ -475,7 +477,8 @@ def combine_block_norm(rows, weights, inverse, residual, *, norm=None, stream_ou
     if not isinstance(inverse, torch.Tensor) or inverse.dtype != torch.int32 or inverse.device != device \
             or inverse.numel() != t_count * k or not inverse.is_contiguous():
         raise ValueError("inverse must be a contiguous int32 tensor of T*k entries on the device of rows")
-    args, stream_out, out = _block_norm_outputs(norm, options, None, residual, stream_out, out, rows)
+    args, stream_out, out = _block_norm_outputs(norm, options, None, residual, stream_out, out,
+                                                (rows, weights, inverse))
     if residual.shape != (t_count, rows.shape[1]) or residual.device != device or weights.device != device:
         raise ValueError("residual must be [T, H] on the device of rows")
     _call(device, lib.pdx_combine_block_norm, rows.data_ptr(), rows.shape[0], weights.data_ptr(), inverse.data_ptr(),

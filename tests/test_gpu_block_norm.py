@@ -384,3 +384,22 @@ def test_layer_and_runtime_refuse_short_slabs(pdx):
     wide = pdx.Mxfp4ExpertSlab(4, 128, 64, "cuda")
     with pytest.raises(ValueError, match="hidden"):
         pdx.PDScopeCudaRuntime({0: wide}, top_k=2).forward(x, gate, layer=0, step=0, top_k=2)
+
+
+def test_outputs_over_weights_are_refused(pdx):
+    """Every row reads the weights, the combine's weights and its order: no output may lie over them."""
+    t = _inputs(4, 64, torch.bfloat16, "none", seed=3)
+    out = torch.ones(4, 64, dtype=torch.bfloat16, device="cuda")
+    wide = torch.ones(4, 64, dtype=torch.float32, device="cuda")
+    for kw in (dict(out=out, pre_weight=out[2]), dict(stream_out=out, post="rms", post_weight=out[0])):
+        with pytest.raises(ValueError, match="weights"):
+            pdx.block_norm(t["y"], t["residual"], **kw)
+    rows = torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    weights, order = torch.ones(4, 2, dtype=torch.bfloat16, device="cuda"), torch.arange(8, dtype=torch.int32, device="cuda")
+    for args, kw in (((out.view(-1)[:8].view(4, 2), order, t["residual"]), dict(out=out)),
+                     ((weights, wide.view(torch.int32).view(-1)[:8], wide.clone()), dict(stream_out=wide)),
+                     ((weights, order, t["residual"]), dict(stream_out=out, pre_weight=out[3]))):
+        with pytest.raises(ValueError, match="weights"):
+            pdx.combine_block_norm(rows, *args, **kw)
+    with pytest.raises(ValueError):
+        pdx.block_norm(t["y"], t["residual"], out=out, pre_weight=[1.0] * 64)
