@@ -378,8 +378,9 @@ int pdx_mxfp4_moe_layer(const void *x, const void *gate, int64_t T, int64_t H, i
  * broadcast), or NULL; gate_sigmoid applies the logistic function to it.
  * y BF16 [T, H], or NULL: s = residual_scale * residual, and post, gate and
  * block_scale do not enter.  residual and stream_out are FP32 if
- * residual_fp32, else BF16; normed_out is BF16; either output may be NULL and
- * may alias y or residual of the same type.  1 <= H <= 8192. */
+ * residual_fp32, else BF16; normed_out is BF16; either output may be NULL, and may
+ * be y or residual of the same type, but must not lie over the gate or a norm's
+ * weights.  Pointers are aligned to their elements.  1 <= H <= 8192. */
 #define PDX_NORM_NONE 0
 #define PDX_NORM_RMS 1
 #define PDX_NORM_LAYER 2
@@ -397,7 +398,7 @@ int pdx_block_norm(const void *y, const void *residual, int64_t T, int64_t H, co
 /* The same with y[t] = sum_s weights[t,s] * rows[inverse[t*k+s]] formed in
  * FP32 (the combine of the expert rows).  Entries of inverse outside
  * [0, y_rows) raise PDX_DEVERR_BAD_EXPERT and count as zero rows.  Outputs must
- * not alias rows. */
+ * not lie over rows, weights, inverse, the gate or the norms' weights. */
 int pdx_combine_block_norm(const void *rows, int64_t y_rows, const void *weights, const int32_t *inverse, int64_t T,
                            int32_t top_k, int64_t H, const void *residual, const pdx_block_norm_args *args,
                            void *stream_out, void *normed_out, pdx_stream_t stream);

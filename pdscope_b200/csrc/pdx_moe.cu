@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <type_traits>
@@ -911,8 +912,17 @@ int check_mx4_matrix(int64_t rows, int64_t cols, int64_t ld, int32_t dtype) {
     return PDX_OK;
 }
 
+// Pointers of `size`-byte elements that an access per element can take.
+bool element_aligned(std::initializer_list<const void*> ptrs, uintptr_t size) {
+    for (const void* p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % size) return false;
+    return true;
+}
+
+int64_t mx4_element(int32_t dtype) { return dtype == PDX_DTYPE_FP32 ? 4 : 2; }
+
 bool mx4_aligned(const void* p, int64_t ld, int32_t dtype) {
-    const int64_t size = dtype == PDX_DTYPE_FP32 ? 4 : 2;
+    const int64_t size = mx4_element(dtype);
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld * size % 16 == 0;
 }
 
@@ -949,7 +959,8 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
     if (w->num_slots > 1 && (w->code_stride < 3 * Hp * Ip / 2 || w->scale_stride < 3 * Hp * Ip / 32 ||
                              w->code_stride % kMx4TileBytes || w->scale_stride % kMx4SfBytes))
         return fail(PDX_ERR_INVALID, "slot strides must cover one expert and be whole tiles");
-    if (w->num_slots * (std::max(w->code_stride, 3 * Hp * Ip / 2) / (kMx4BK / 2)) >= (int64_t(1) << 31))
+    if (!element_aligned({w->slot_of_expert}, 4)) return fail(PDX_ERR_INVALID, "slot_of_expert must be 4-byte aligned");
+    if (std::max(w->code_stride, 3 * Hp * Ip / 2) / (kMx4BK / 2) > ((int64_t(1) << 31) - 1) / w->num_slots)
         return fail(PDX_ERR_UNSUPPORTED, "expert slab too large for 32-bit TMA row coordinates");
     return PDX_OK;
 }
@@ -1160,6 +1171,9 @@ int check_block_norm(const pdx_block_norm_args* a, const void* residual, int64_t
         return fail(PDX_ERR_INVALID, "unknown norm");
     if (!(a->eps > 0.f)) return fail(PDX_ERR_INVALID, "eps must be positive");
     if (a->gate && (a->gate_row < 0 || a->gate_col < 0)) return fail(PDX_ERR_INVALID, "negative gate stride");
+    if (!element_aligned({residual, stream_out}, a->residual_fp32 ? 4 : 2) ||
+        !element_aligned({normed_out, a->post_weight, a->pre_weight, a->gate}, 2))
+        return fail(PDX_ERR_INVALID, "block-norm pointer not aligned to its elements");
     return PDX_OK;
 }
 
@@ -1585,6 +1599,7 @@ int pdx_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols,
     if (st) return st;
     if (rows == 0) return ok();
     if (!x || !codes || !scales) return fail(PDX_ERR_INVALID, "null quantisation argument");
+    if (!element_aligned({x}, mx4_element(dtype))) return fail(PDX_ERR_INVALID, "x not aligned to its elements");
     if (reinterpret_cast<uintptr_t>(codes) & 3u) return fail(PDX_ERR_INVALID, "codes must be 4-byte aligned");
     const int64_t chunks = rows * cols / 8;
     PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(x, ld, dtype), ld == cols, [&](auto type, auto aligned, auto flat) {
@@ -1602,6 +1617,7 @@ int pdx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, in
     if (st) return st;
     if (rows == 0) return ok();
     if (!out || !codes || !scales) return fail(PDX_ERR_INVALID, "null quantisation argument");
+    if (!element_aligned({out}, mx4_element(dtype))) return fail(PDX_ERR_INVALID, "out not aligned to its elements");
     if (reinterpret_cast<uintptr_t>(codes) & 3u) return fail(PDX_ERR_INVALID, "codes must be 4-byte aligned");
     const int64_t chunks = rows * cols / 8;
     PDX_PDL_TRY(with_mx4_type(dtype, mx4_aligned(out, ld, dtype), ld == cols, [&](auto type, auto aligned, auto flat) {
@@ -1624,6 +1640,8 @@ int pdx_mxfp4_ffn_grouped(const void* x, int64_t T, const int32_t* tokens, const
     if (!x || !offsets || !active || !y_out) return fail(PDX_ERR_INVALID, "null FFN argument");
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y_out)) & 15u)
         return fail(PDX_ERR_INVALID, "x and y must be 16-byte aligned");
+    if (!element_aligned({tokens, offsets, active}, 4))
+        return fail(PDX_ERR_INVALID, "the packing must be 4-byte aligned");
     int st = check_mx4_ffn(T, rows, E, H, I, tokens != nullptr, weights);
     if (st) return st;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1)))
@@ -1637,6 +1655,7 @@ int pdx_block_norm(const void* y, const void* residual, int64_t T, int64_t H, co
                    void* stream_out, void* normed_out, pdx_stream_t stream) {
     int st = check_block_norm(args, residual, T, H, stream_out, normed_out);
     if (st) return st;
+    if (!element_aligned({y}, 2)) return fail(PDX_ERR_INVALID, "block-norm pointer not aligned to its elements");
     BlockNormArgs a = to_block_norm(args, residual, H, stream_out, normed_out);
     a.y = static_cast<const uint16_t*>(y);
     if (!y) {   // no block: its gate and scale do not enter, 0 * inf would
@@ -1656,6 +1675,8 @@ int pdx_combine_block_norm(const void* rows, int64_t y_rows, const void* weights
     if (top_k < 1 || y_rows < 1) return fail(PDX_ERR_INVALID, "empty combine");
     if (top_k > kMaxTopK) return fail(PDX_ERR_UNSUPPORTED, "top_k > %d", kMaxTopK);
     if (y_rows >= (int64_t(1) << 31)) return fail(PDX_ERR_UNSUPPORTED, "y_rows too large");
+    if (!element_aligned({rows, weights}, 2) || !element_aligned({inverse}, 4))
+        return fail(PDX_ERR_INVALID, "combine pointer not aligned to its elements");
     BlockNormArgs a = to_block_norm(args, residual, H, stream_out, normed_out);
     a.y = static_cast<const uint16_t*>(rows);
     a.weights = static_cast<const uint16_t*>(weights);

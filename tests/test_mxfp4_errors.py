@@ -193,3 +193,39 @@ def test_stack_refuses_slabs_that_do_not_fit():
         ResidentMoEStack([gate, torch.zeros(5, 64, dtype=torch.bfloat16)], [slab, slab])
     # fewer slots than experts is an error of the routing, not of a BF16 slab
     ResidentMoEStack([gate], [_bf16_slab(3, 64, 64)])
+
+
+@pytest.mark.parametrize("dtype,at", ((0, 257), (1, 257), (2, 258), (2, 257)))
+def test_matrix_refuses_split_elements(dtype, at):
+    """A pointer between two elements would fault on the device."""
+    odd = ctypes.c_void_p(at)
+    assert _lib.lib.pdx_mxfp4_quantize(odd, dtype, 1, 32, 32, PTR, PTR, NULL) == _lib.PDX_ERR_INVALID
+    assert _lib.lib.pdx_mxfp4_dequantize(PTR, PTR, 1, 32, 32, dtype, odd, NULL) == _lib.PDX_ERR_INVALID
+
+
+def test_block_norm_refuses_split_elements():
+    def a(**kw):
+        return _lib.BlockNormArgs(**dict(dict(eps=1e-6, pre=1, residual_scale=1, block_scale=1), **kw))
+    odd, half = ctypes.c_void_p(257), ctypes.c_void_p(258)
+    assert _norm(a(), y=odd) == _lib.PDX_ERR_INVALID
+    assert _norm(a(), residual=odd) == _lib.PDX_ERR_INVALID
+    assert _norm(a(residual_fp32=1), residual=half) == _lib.PDX_ERR_INVALID
+    assert _norm(a(residual_fp32=1), stream=half) == _lib.PDX_ERR_INVALID
+    assert _norm(a(), normed=odd) == _lib.PDX_ERR_INVALID
+    for name in ("post_weight", "pre_weight", "gate"):
+        assert _norm(a(**{name: 257})) == _lib.PDX_ERR_INVALID
+    args = a()
+    for rows, weights, inverse in ((odd, PTR, PTR), (PTR, odd, PTR), (PTR, PTR, half)):
+        assert _lib.lib.pdx_combine_block_norm(rows, 4, weights, inverse, 2, 2, 64, PTR, ctypes.byref(args), PTR, PTR,
+                                               NULL) == _lib.PDX_ERR_INVALID
+
+
+def test_ffn_refuses_split_elements_and_huge_slabs():
+    half, w = ctypes.c_void_p(258), _weights()
+    for tokens, offsets, active in ((half, PTR, PTR), (PTR, half, PTR), (PTR, PTR, half)):
+        assert _lib.lib.pdx_mxfp4_ffn_grouped(PTR, 2, tokens, offsets, active, 2, 4, ctypes.byref(w), 128, 128, PTR, PTR,
+                                              1 << 40, NULL) == _lib.PDX_ERR_INVALID
+    assert _ffn(_weights(slot_of_expert=258)) == _lib.PDX_ERR_INVALID
+    # slots x tiles past 64 bits: 384 rows of codes a slot x 2^57 slots = 3 2^64
+    assert _ffn(_weights(num_slots=1 << 57)) == _lib.PDX_ERR_UNSUPPORTED
+    assert _ffn(_weights(num_slots=(1 << 63) - 1)) == _lib.PDX_ERR_UNSUPPORTED
