@@ -403,3 +403,60 @@ def test_outputs_over_weights_are_refused(pdx):
             pdx.combine_block_norm(rows, *args, **kw)
     with pytest.raises(ValueError):
         pdx.block_norm(t["y"], t["residual"], out=out, pre_weight=[1.0] * 64)
+
+
+# From 593 rows on other kernels run than for few: two vectors a thread (256 threads to H = 4096, 512 beyond), or
+# value by value (256 threads to H = 2048, 512 to 4096), with the weights and beside expert rows the gate loaded late.
+MANY_ROWS = ((593, 8), (601, 264), (700, 2048), (595, 4096), (593, 4104), (600, 8192),       # vectors
+             (593, 9), (600, 2047), (601, 2049), (593, 3001), (594, 4095), (593, 5001))      # value by value
+
+
+@pytest.mark.parametrize("tokens,hidden", MANY_ROWS)
+@pytest.mark.parametrize("residual", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("post,pre,gate,act", (("rms", "rms", "none", "none"), ("layer", "rms", "full", "sigmoid"),
+                                               ("none", "layer", "channel", "none"), ("rms", "none", "token", "sigmoid"),
+                                               ("layer", "layer", "full", "none")))
+def test_many_rows(pdx, tokens, hidden, residual, post, pre, gate, act):
+    t = _inputs(tokens, hidden, residual, gate, seed=tokens * 10000 + hidden)
+    options = dict(post=post, pre=pre, gate=t["gate"], gate_act=act, residual_scale=0.75, block_scale=-1.5,
+                   post_weight=t["post_weight"] if post != "none" else None,
+                   pre_weight=t["pre_weight"] if pre != "none" else None)
+    want = pdx.block_norm(t["y"], t["residual"], **options)
+    _check(want, _f64(t["y"]), _f64(t["residual"]), options)
+    # in place
+    y, r = t["y"].clone(), t["residual"].clone()
+    got = pdx.block_norm(y, r, stream_out=r, out=y, **options)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("tokens,hidden,top_k", tuple((t, h, (1, 3, 5, 8)[i % 4]) for i, (t, h) in enumerate(MANY_ROWS))
+                         + ((593, 2048, 32), (593, 511, 32)))
+@pytest.mark.parametrize("residual", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("post,pre,gate,act", (("rms", "rms", "token", "sigmoid"), ("layer", "layer", "full", "sigmoid"),
+                                               ("none", "rms", "channel", "none")))
+def test_many_combined_rows(pdx, tokens, hidden, top_k, residual, post, pre, gate, act):
+    t = _inputs(tokens, hidden, residual, gate, seed=hidden + top_k)
+    gen = torch.Generator().manual_seed(tokens)
+    rows = torch.randn(tokens * top_k, hidden, generator=gen).to(torch.bfloat16).cuda()
+    weights = torch.rand(tokens, top_k, generator=gen).to(torch.bfloat16).cuda()
+    inverse = torch.randperm(tokens * top_k, generator=gen).to(torch.int32).cuda()
+    options = dict(post=post, pre=pre, gate=t["gate"], gate_act=act, pre_weight=t["pre_weight"],
+                   post_weight=t["post_weight"] if post != "none" else None)
+    want = pdx.combine_block_norm(rows, weights, inverse, t["residual"], **options)
+    y = np.einsum("tkh,tk->th", _f64(rows)[inverse.cpu().numpy()].reshape(tokens, top_k, hidden), _f64(weights))
+    # the FP32 combine is off by top_k 2^-24 of the magnitudes of its terms, which for up to 32 terms of both
+    # signs stays inside _check's 2^-17 of the row's largest sum
+    _check(want, y, _f64(t["residual"]), options)
+    r = t["residual"].clone()
+    got = pdx.combine_block_norm(rows, weights, inverse, r, stream_out=r, **options)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_many_rows_from_an_odd_address(pdx):
+    """Rows of whole vectors whose base is no multiple of 16 bytes go value by value."""
+    t = _inputs(600, 1024, torch.bfloat16, "full", seed=3)
+    want = pdx.block_norm(t["y"], t["residual"], post="rms", gate=t["gate"])
+    _check(want, _f64(t["y"]), _f64(t["residual"]), dict(post="rms", gate=t["gate"]))
+    odd = torch.empty(600 * 1024 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(600, 1024).copy_(t["y"])
+    options = dict(post="rms", gate=t["gate"])
+    _check(pdx.block_norm(odd, t["residual"], **options), _f64(t["y"]), _f64(t["residual"]), options)
