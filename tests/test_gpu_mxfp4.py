@@ -450,3 +450,20 @@ def test_bad_offsets_are_reported(pdx, tokens):
         assert (guard[0] == 7).all() and (guard[-1] == 7).all()
         with pytest.raises(ValueError, match="expert ID"):
             runtime.raise_device_error()
+
+
+# more than 592 packed rows of more than 2048 channels: one warp a row, rows longer than it holds at once
+LONG_ROWS = ((80, 4096, 64, 120, 8), (100, 2080, 96, 100, 7), (200, 2176, 96, 40, 8), (700, 4128, 96, 3, 1),
+             (640, 8192, 64, 2, 1))
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", LONG_ROWS)
+def test_many_long_rows(pdx, tokens, hidden, inter, experts, top_k):
+    slab, qs = _slab(pdx, experts, hidden, inter, seed=hidden + tokens)
+    x = torch.randn(tokens, hidden, generator=torch.Generator().manual_seed(tokens)).to(torch.bfloat16)
+    x[:, hidden - 3] *= 50        # in the last values of a row
+    x = x.cuda()
+    sel = _selected(tokens, experts, top_k, seed=tokens + 1)
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), experts)
+    got = pdx.moe_ffn_mxfp4(x, packed, slab)
+    _check_rows(got, x, packed, qs, experts)
