@@ -7,15 +7,16 @@
 // instruction is spent on dequantising, and HBM is read at 4.25 bits a weight.
 //
 // The activations keep BF16's precision in that 8-bit product as TWO E4M3
-// pieces.  With v scaled by a power of two so that the largest value of its
-// scaling group lies in [128, 256):
+// pieces.  x and h are scaled by powers of two, one E8M0 scale per 32 values of K
+// like the weights', that take a block's largest value into [128, 256):
 //   hi = e4m3(v),  lo = e4m3(16 (v - hi)), read back through a scale of 1/16
-// e4m3 keeps 4 significant bits, so |v - hi| <= 2^-4 |v| (16 of it at most 256)
-// and the rest after lo is at most 2^-8 |v|: BF16's half step.  A BF16 v is
-// represented exactly down to 2^-13 of its group's largest value; below that the
-// error is at most 2^-14 (half of lo's smallest step), 2^-21 of the largest value.
-// x is scaled per row (a factor on the row of the result), h per 32 values of I (an
-// E8M0 scale of the second product).  W hi and W lo cost what one BF16 product would.
+// e4m3 keeps 4 significant bits, so |v - hi| <= 2^-4 |v|, which lo holds to
+// 2^-9 |v|: an FP32 h is off by half of what rounding it to BF16 would cost, and a
+// BF16 v (x) is represented exactly down to 2^-13 of its block's largest value;
+// below that the error is at most 2^-14 (half of lo's smallest step), 2^-21 of the
+// largest value.  A block of x that holds an infinity or NaN, and one of h where an
+// infinity arises, is NaN throughout.
+// W hi and W lo cost what one BF16 product would.
 //
 // Two launches of k_mx4_gemm, each on tiles of 256 weight rows (two accumulators
 // over one token operand): 128 rows of gate and the same 128 of up with the
@@ -54,7 +55,6 @@ constexpr int kMx4MaxActive = 1024;
 constexpr uint32_t kMx4StageOut = 1024;             // 8 token columns x 64 weight rows on their way out
 constexpr uint32_t kMx4TmemCols = 512;
 constexpr uint32_t kMx4SfCol = 448;                 // 4 slots of weight and token scales, 4 columns a tile
-constexpr uint32_t kMx4OneCol = 488;                // gate/up's token scales, constant: x has a row factor
 constexpr int kMx4LoShift = 4;                      // lo pieces are held times 2^4
 constexpr int kMx4SmemLimit = 227 * 1024;
 
@@ -81,91 +81,129 @@ __device__ __forceinline__ void e4m3_split2(float a, float b, uint16_t& hi, uint
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"((b - f.y) * up), "f"((a - f.x) * up));
 }
 
+// Four BF16 values of x, scaled by inv: their E4M3 pieces by way of FP16, which holds
+// a scaled BF16 exactly from 2^-17 up (below 2^-14 it is off by 2^-25 at most, where lo
+// is off by 2^-14).
+__device__ __forceinline__ void e4m3_split4(uint32_t a, uint32_t b, float inv, uint32_t& hi, uint32_t& lo) {
+    uint16_t h[2], l[2];
+    const uint32_t w[2] = {a, b};
+    const __half2 up = __float2half2_rn(1 << kMx4LoShift);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const __half2 v = __floats2half2_rn(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xFFFF0000u) * inv);
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h[i]) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+        uint32_t back;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h[i]));
+        const __half2 rest = __hmul2(__hsub2(v, *reinterpret_cast<const __half2*>(&back)), up);
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l[i]) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+    }
+    hi = h[0] | (static_cast<uint32_t>(h[1]) << 16);
+    lo = l[0] | (static_cast<uint32_t>(l[1]) << 16);
+}
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Where the split puts the scales of x: four bytes (of 128 columns) at `first + kb *
+// step` for a row's hi piece, `lo` bytes further for its lo piece.
+// Narrow token tiles: a 16-byte record per packed row and 128 columns, [kb][rows + 32]:
+// any NT rows in a run are the scales of a token tile as tcgen05 wants them (hi in
+// word 0, lo in word 1 at NT = 32, in a second array at NT = 16).  Wide ones: tiles of
+// 512 bytes, [mx4_x_tile][kb][hi, lo].
+struct Mx4Scales {
+    uint8_t* bytes;
+    int64_t step, lo;
+};
+
+// First scale tile of x of an expert whose packed rows start at seg0: experts of n
+// rows have ceil(n / nt) tiles, which these starts keep apart whatever the list of
+// active experts is; rows / nt + E in all.
+__host__ __device__ constexpr int mx4_x_tile(int seg0, int e, int nt) { return seg0 / nt + e; }
+
 // Token rows in packed order as E4M3 pieces: out [2][rows][Hp] (hi rows, then lo
-// rows, zero past H) and the row's factor 2^(b - 127).  HBM-bound (the pieces
-// are written once, x comes from L2).  A group of WARPS warps takes a row, 16
-// values a lane at a time; the first four (four warps: two) of those stay in
-// registers between finding the row's largest value and splitting, longer rows
-// are read again.  One warp a row for many rows, four for few, where the trip to memory
-// is what a row costs.  The kernel also clears the tickets of the two products
-// that follow.
-constexpr int kMx4SplitWarps = 4;     // warps per CTA
-template <int WARPS>
-__global__ void __launch_bounds__(kMx4SplitWarps * 32, WARPS == 1 ? 7 : 12)
+// rows, zero past H) and a scale byte per 32 values.  A warp takes 512 UNROLL columns of
+// a row, a lane 16 values at a time.  NT > 0: wide token tiles of NT rows, whose scales
+// go by expert.  99,600 rows of 2048 take 110 us, 4.7 TB/s of DRAM traffic (the pieces
+// are written once, x comes from L2 but for a third); 16 us of it are the scale bytes,
+// which lie scattered over their tiles.  CTAs that collect the scales of 8, 16 or 32
+// rows of a tile for whole sectors took 114, 103 and 101 us, and up to 8 us more than
+// this at 1000 rows, where a warp then has several rows one after the other.  The
+// kernel also clears the tickets of the two products that follow.
+constexpr int kMx4SplitThreads = 128;
+template <int UNROLL, int NT>
+__global__ void __launch_bounds__(kMx4SplitThreads, UNROLL == 1 ? 12 : (UNROLL == 2 ? 10 : 7))
     k_mx4_split(const uint16_t* __restrict__ x, const int32_t* __restrict__ tokens, int T, int rows, int H, int Hp,
-                uint8_t* __restrict__ out, float* __restrict__ row_scale, unsigned int* __restrict__ zero_ptr,
-                int zero_words) {
+                uint8_t* __restrict__ out, Mx4Scales scales, const int32_t* __restrict__ offsets, int E,
+                unsigned int* __restrict__ zero_ptr, int zero_words) {
     griddep_wait();
     griddep_launch();
-    constexpr int kMx4SplitHeld = WARPS == 1 ? 4 : 2;
-    __shared__ uint32_t s_top[kMx4SplitWarps];
+    __shared__ int s_off[NT ? kMx4MaxActive + 1 : 1];
     for (int i = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x); i < zero_words;
          i += static_cast<int>(gridDim.x * blockDim.x))
         zero_ptr[i] = 0u;
-    constexpr int kGroups = kMx4SplitWarps / WARPS, kLanes = 32 * WARPS;
-    const int group = static_cast<int>(threadIdx.x) / kLanes, lane = static_cast<int>(threadIdx.x) % kLanes;
-    const int chunks = H / 16, chunks_p = Hp / 16;
-    // WARPS > 1: one group per CTA, so the loop below is uniform over the CTA
-    static_assert(WARPS == 1 || kGroups == 1, "the barriers need whole CTAs");
-    for (int p = static_cast<int>(blockIdx.x) * kGroups + group; p < rows; p += static_cast<int>(gridDim.x) * kGroups) {
+    if (NT) {
+        for (int i = static_cast<int>(threadIdx.x); i <= kMx4MaxActive; i += kMx4SplitThreads)
+            s_off[i] = i <= E ? __ldg(offsets + i) : rows;
+        __syncthreads();
+    }
+    constexpr int kWarps = kMx4SplitThreads / 32;
+    const int lane = static_cast<int>(lane_id()), sub = lane & 7;
+    const int chunks = H / 16, chunks_p = Hp / 16, per_row = (chunks_p + 32 * UNROLL - 1) / (32 * UNROLL);
+    const int units = rows * per_row;
+    const uint32_t odd = sub & 1, minus = odd ? kMx4LoShift : 0;       // even lanes store scales of hi, odd ones of lo
+    for (int u = static_cast<int>(blockIdx.x * kWarps + threadIdx.x / 32); u < units;
+         u += static_cast<int>(gridDim.x) * kWarps) {
+        const int p = per_row == 1 ? u : u / per_row, c0 = (u - p * per_row) * (32 * UNROLL) + lane;
         int t = tokens ? __ldg(tokens + p) : p;
         if (t < 0 || t >= T) {
             raise_error(PDX_DEVERR_BAD_EXPERT);
             t = 0;
         }
-        const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t) * H);
-        struct Sixteen {
-            uint4 a, b;
-        };
-        auto load = [&](int c) {
-            Sixteen v{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-            if (c < chunks) v = Sixteen{__ldg(src + 2 * c), __ldg(src + 2 * c + 1)};
-            return v;
-        };
-        Sixteen held[kMx4SplitHeld];
-        uint32_t top = 0;
-        auto widen = [&](const Sixteen& v) {
-            const uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
+        const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t) * H) + 2 * c0;
+        uint4 v[UNROLL][2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
-        };
-#pragma unroll
-        for (int j = 0; j < kMx4SplitHeld; ++j) held[j] = load(j * kLanes + lane);
-#pragma unroll
-        for (int j = 0; j < kMx4SplitHeld; ++j) widen(held[j]);
-        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks; c += kLanes) widen(load(c));
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (WARPS > 1) {
-            __syncthreads();   // s_top free from the previous row
-            if (lane_id() == 0) s_top[threadIdx.x >> 5] = top;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < WARPS; ++i) top = max(top, s_top[i]);
+        for (int j = 0; j < UNROLL; ++j) {
+            v[j][0] = c0 + 32 * j < chunks ? __ldg(src + 64 * j) : make_uint4(0, 0, 0, 0);
+            v[j][1] = c0 + 32 * j < chunks ? __ldg(src + 64 * j + 1) : make_uint4(0, 0, 0, 0);
         }
-        const uint32_t byte = mx4_group_byte(top);
-        const float inv = mx4_inverse(byte);
-        uint4* hi_row = reinterpret_cast<uint4*>(out + static_cast<int64_t>(p) * Hp);
-        uint4* lo_row = reinterpret_cast<uint4*>(out + (static_cast<int64_t>(rows) + p) * Hp);
-        auto split = [&](const Sixteen& v, int c) {
-            const uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
+        int64_t first = 16 * static_cast<int64_t>(p);
+        bool scaled = true;
+        if (NT) {
+            // the last expert that starts at p or before, in two steps of 32
+            static_assert(kMx4MaxActive == 32 * 32, "two steps");
+            int e = 32 * (__popc(__ballot_sync(0xffffffffu, s_off[32 * lane] <= p)) - 1);
+            e += __popc(__ballot_sync(0xffffffffu, s_off[max(e, 0) + lane] <= p)) - 1;
+            e = min(max(e, 0), E - 1);
+            const int seg0 = s_off[e], r = p - seg0;
+            // a row of no expert is in no tile and has no scales
+            scaled = seg0 >= 0 && r >= 0 && p < s_off[e + 1];
+            first = (mx4_x_tile(seg0, e, NT) + r / NT) * (chunks_p * int64_t(128)) + (r % NT % 32) * 16 + r % NT / 32 * 4;
+        }
+        uint8_t* to = scales.bytes + first + (c0 >> 3) * scales.step + (odd ? scales.lo : 0) + (sub >> 1);
+        uint4* hi_row = reinterpret_cast<uint4*>(out + static_cast<int64_t>(p) * Hp) + c0;
+        uint4* lo_row = reinterpret_cast<uint4*>(out + (static_cast<int64_t>(rows) + p) * Hp) + c0;
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) {
+            const uint32_t w[8] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w,
+                                   v[j][1].x, v[j][1].y, v[j][1].z, v[j][1].w};
+            uint32_t two = w[0] & 0x7FFF7FFFu;                 // the largest magnitudes of the even and of the odd values
+#pragma unroll
+            for (int i = 1; i < 8; ++i) two = max_u16x2(two, w[i] & 0x7FFF7FFFu);
+            two = max_u16x2(two, __shfl_xor_sync(0xffffffffu, two, 1));   // two lanes hold a block of 32
+            const uint32_t byte = mx4_group_byte(max(two << 16, two & 0xFFFF0000u));
+            const float inv = mx4_inverse(byte);
             uint32_t h[4], l[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint16_t h0, h1, l0, l1;
-                e4m3_split2(__uint_as_float(w[2 * i] << 16) * inv, __uint_as_float(w[2 * i] & 0xFFFF0000u) * inv, h0, l0);
-                e4m3_split2(__uint_as_float(w[2 * i + 1] << 16) * inv, __uint_as_float(w[2 * i + 1] & 0xFFFF0000u) * inv,
-                            h1, l1);
-                h[i] = h0 | (static_cast<uint32_t>(h1) << 16);
-                l[i] = l0 | (static_cast<uint32_t>(l1) << 16);
+            for (int i = 0; i < 4; ++i) e4m3_split4(w[2 * i], w[2 * i + 1], inv, h[i], l[i]);
+            if (c0 + 32 * j < chunks_p) {                      // eight lanes, 128 columns, alike
+                __stcs(hi_row + 32 * j, make_uint4(h[0], h[1], h[2], h[3]));   // streaming: x stays in L2
+                __stcs(lo_row + 32 * j, make_uint4(l[0], l[1], l[2], l[3]));
+                if (scaled) to[4 * j * scales.step] = static_cast<uint8_t>(byte - minus);   // kMx4LoShift at least
             }
-            __stcs(hi_row + c, make_uint4(h[0], h[1], h[2], h[3]));   // streaming: x stays in L2
-            __stcs(lo_row + c, make_uint4(l[0], l[1], l[2], l[3]));
-        };
-#pragma unroll
-        for (int j = 0; j < kMx4SplitHeld; ++j)
-            if (j * kLanes + lane < chunks_p) split(held[j], j * kLanes + lane);
-        for (int c = kMx4SplitHeld * kLanes + lane; c < chunks_p; c += kLanes) split(load(c), c);
-        if (lane == 0) row_scale[p] = mx_scale(byte);
+        }
     }
 }
 
@@ -180,7 +218,8 @@ struct Mx4Args {
     int tile0, tile1;               // first weight tile of gate and up, or of down (tile0)
     int K, M;                       // multiples of 128: reduction length, weight rows
     int rows;
-    const float* row_scale;         // [rows] factor of a packed row of x (SWIGLU)
+    const uint8_t* xs;              // x scales of narrow token tiles (Mx4Scales), x_pad records per 128 columns (SWIGLU)
+    int x_pad;
     uint8_t* sf;                    // h scales: [token tile][Ip / 128][kSfTiles] tiles of 512 bytes (out of SWIGLU, else in)
     uint8_t* h;                     // [2][rows][M] pieces (SWIGLU)
     uint16_t* y;                    // [rows, ldy] (down)
@@ -300,12 +339,13 @@ struct Mx4Shape {
     // narrow ones keep the shared memory for the ring.
     static constexpr int kEpi = kPair ? 16 : 8;
     static constexpr int kThreads = 32 * (kEpi + 3);
-    static constexpr uint32_t kFixed = 1024 + 1024 + 512 + kEpi * kMx4StageOut;  // alignment, constants, barriers, staging
+    static constexpr uint32_t kFixed = 1024 + 512 + kEpi * kMx4StageOut;   // alignment, barriers, staging
+    static constexpr uint32_t kEntry = kPair ? 20 : 16;                    // an expert's entry in the tables
     // Ring stages beside tables of `entries` experts, and the shared memory of both.
     static constexpr int stages(int entries) {
-        return static_cast<int>((kMx4SmemLimit - kFixed - 16u * entries) / (kStage + kSf));
+        return static_cast<int>((kMx4SmemLimit - kFixed - kEntry * entries) / (kStage + kSf));
     }
-    static constexpr size_t smem(int entries) { return kFixed + 16u * entries + stages(entries) * (kStage + kSf); }
+    static constexpr size_t smem(int entries) { return kFixed + kEntry * entries + stages(entries) * (kStage + kSf); }
     static constexpr int kMaxStages = stages(1);
     static_assert(NT % 16 == 0 && kBRows % 8 == 0 && stages(kMx4MaxActive) >= 3 && 2 * kMaxStages + 5 <= 56 &&
                       2 * kAcc <= static_cast<int>(kMx4SfCol),
@@ -335,8 +375,8 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     unsigned char* smem = smem_mx4 + ((1024u - (smem_u32(smem_mx4) & 1023u)) & 1023u);
     const int stages = args.stages;
     unsigned char* s_sf = smem + stages * S::kStage;                 // stages x kSf
-    unsigned char* s_one = s_sf + stages * S::kSf;                   // constant token scales, kSfTiles tiles
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_one + 1024);
+    unsigned char* s_bar = s_sf + stages * S::kSf;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_bar);
     uint64_t* empty_bar = full_bar + stages;
     uint64_t* tmem_full = empty_bar + stages;
     uint64_t* tmem_empty = tmem_full + 2;
@@ -344,11 +384,12 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_misc = reinterpret_cast<int*>(tmem_slot + 2);
-    unsigned char* s_out = s_one + 1536;                             // an epilogue warp's staging: kMx4StageOut
+    unsigned char* s_out = s_bar + 512;                              // an epilogue warp's staging: kMx4StageOut
     int* prefix = reinterpret_cast<int*>(s_out + S::kEpi * kMx4StageOut);   // token tiles before an active expert
     int* t_seg0 = prefix + args.table;
     int* t_rows = t_seg0 + args.table;
     int* t_slot = t_rows + args.table;
+    int* t_xs = t_slot + args.table;                                 // PAIR: first scale tile of x
 
     const int warp = static_cast<int>(threadIdx.x >> 5);
     const uint32_t lane = lane_id();
@@ -395,13 +436,6 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
     }
-    if (warp >= 3)
-        for (int i = static_cast<int>(threadIdx.x) - 96; i < 128 * S::kSfTiles; i += S::kThreads - 96) {
-            // word i of a tile: row 32 (i % 4) + i / 4; scale 1 of hi, 2^-kMx4LoShift of lo
-            const bool low = S::kStack ? 32 * (i & 3) + (i >> 2) >= NT : i >= 128;
-            reinterpret_cast<uint32_t*>(s_one)[i] = (127u - (low ? kMx4LoShift : 0)) * 0x01010101u;
-        }
-    fence_proxy_async_smem();
     // The routing tables are older than the launch before this one, which has
     // passed its own wait by the time this one starts; only that launch's
     // output (the token pieces) has to be waited for, by the warps that read it.
@@ -426,6 +460,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
         t_seg0[i] = seg0;
         t_rows[i] = end - seg0;
         t_slot[i] = static_cast<int>(slot);
+        if (PAIR) t_xs[i] = mx4_x_tile(seg0, e, NT);
     }
     tc_fence_before();
     __syncthreads();
@@ -501,7 +536,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                     const int y0 = static_cast<int>(tile0 + b0 + kb) * 128, y1 = static_cast<int>(tile0 + b1 + kb) * 128;
                     if (rank == 0)
                         mbar_arrive_expect_tx(&full_bar[stage],
-                                              kCtas * (S::kATx + S::kB + (SWIGLU ? 2 : 2 + S::kSfTiles) * kMx4SfBytes));
+                                              kCtas * (S::kATx + S::kB + (2 + S::kSfTiles) * kMx4SfBytes));
                     if (PAIR) {
                         const uint32_t fb = full0 + static_cast<uint32_t>(stage) * 8u;
                         tma_load_2d_pair(sa, &tm_w, fb, 0, y0);
@@ -536,22 +571,28 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
             bool ok = true;
             for (Tile t = begin(); ok && next(t);) {
                 const int row = t_seg0[t.a] + t.nb * NT + rank * S::kBRows;
-                const int64_t tt = t.token;
+                const int64_t tt = PAIR && SWIGLU ? t_xs[t.a] + t.nb : t.token;   // scale tiles of x, of h
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     if (!wait(&empty_bar[stage], phase ^ 1u)) { ok = false; break; }
                     if (PAIR) {
                         const uint32_t fb = full0 + static_cast<uint32_t>(stage) * 8u;
                         tma_load_3d_pair(smem + stage * S::kStage + S::kA, &tm_x, fb, kb * kMx4BK, row, 0);
-                        for (int i = 0; !SWIGLU && i < S::kSfTiles; ++i)
+                        for (int i = 0; i < S::kSfTiles; ++i)
                             tma_load_2d_pair(s_sf + stage * S::kSf + (2 + i) * kMx4SfBytes, &tm_xs, fb, 0,
                                              static_cast<int>(tt * nkb + kb) * S::kSfTiles + i);
                         if (++stage == stages) { stage = 0; phase ^= 1u; }
                         continue;
                     }
                     tma_load_3d(smem + stage * S::kStage + S::kA, &tm_x, &full_bar[stage], kb * kMx4BK, row, 0);
-                    if (!SWIGLU)
-                        bulk_load(s_sf + stage * S::kSf + 2 * kMx4SfBytes, args.sf + (tt * nkb + kb) * kMx4SfBytes,
-                                  kMx4SfBytes, &full_bar[stage]);
+                    unsigned char* ss = s_sf + stage * S::kSf + 2 * kMx4SfBytes;
+                    if (SWIGLU) {
+                        const int64_t record = static_cast<int64_t>(kb) * args.x_pad + row;
+                        for (int i = 0; i < 32 / NT; ++i)                        // 32 records; NT = 16: of hi, then of lo
+                            bulk_load(ss + i * (NT * 16), args.xs + (static_cast<int64_t>(i) * nkb * args.x_pad + record) * 16,
+                                      NT * 16, &full_bar[stage]);
+                    } else {
+                        bulk_load(ss, args.sf + (tt * nkb + kb) * kMx4SfBytes, kMx4SfBytes, &full_bar[stage]);
+                    }
                     if (++stage == stages) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -560,7 +601,7 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
     } else if (warp == 1 && rank == 0) {
         // ---------------- MMA issuer (of the pair: rank 0) ----------------
         constexpr uint32_t idesc = mx4_idesc(128 * kCtas, S::kN);
-        constexpr uint32_t kSlot = SWIGLU ? 8 : 8 + 4 * S::kSfTiles;   // scale columns of a K step
+        constexpr uint32_t kSlot = 8 + 4 * S::kSfTiles;   // scale columns of a K step
         auto commit = [&](uint64_t* bar) {   // to this barrier of every CTA of the tile
             if (PAIR) {
                 umma_commit_pair(smem_u32(bar));
@@ -585,13 +626,11 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
                     const uint32_t sa = smem_u32(smem + stage * S::kStage);
                     const uint32_t ss = smem_u32(s_sf + stage * S::kSf);
                     const uint32_t sf = tmem_base + kMx4SfCol + static_cast<uint32_t>(step & 3) * kSlot;
-                    for (int i = 0; SWIGLU && step == 0 && i < S::kSfTiles; ++i)
-                        tmem_cp_sf<PAIR>(tmem_base + kMx4OneCol + 4 * i, mx4_sf_desc(smem_u32(s_one) + i * kMx4SfBytes));
                     tmem_cp_sf<PAIR>(sf, mx4_sf_desc(ss));
                     tmem_cp_sf<PAIR>(sf + 4, mx4_sf_desc(ss + kMx4SfBytes));
-                    for (int i = 0; !SWIGLU && i < S::kSfTiles; ++i)
+                    for (int i = 0; i < S::kSfTiles; ++i)
                         tmem_cp_sf<PAIR>(sf + 8 + 4 * i, mx4_sf_desc(ss + (2 + i) * kMx4SfBytes));
-                    const uint32_t sfb = SWIGLU ? tmem_base + kMx4OneCol : sf + 8, sfb_lo = sfb + 4;
+                    const uint32_t sfb = sf + 8, sfb_lo = sfb + 4;
                     const uint64_t a0 = sw128_desc(sa), a1 = sw128_desc(sa + kMx4ABytes);
                     const uint64_t hi = sw128_desc(sa + S::kA), lo = sw128_desc(sa + S::kA + S::kBRows * kMx4BK);
 #pragma unroll
@@ -622,24 +661,17 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
         // 16-byte halves change places, so eight lanes read eight different bank groups.
         const uint32_t turn = lane >> 2 & 1u;
         uint32_t* out = reinterpret_cast<uint32_t*>(s_out + (warp - 2) * kMx4StageOut);
-        float rs[(NT + 31) / 32];                                // factor of the tile's row 32 i + lane (SWIGLU)
         // Token columns [c0, c0 + n), n <= 8, of a tile: the sums g of the first, u of the second 128 weight rows.
         auto finish = [&](const Tile& t, int c0, int n, float (&g)[kMx4Chunk], float (&u)[kMx4Chunk]) {
             const int64_t p0 = static_cast<int64_t>(t_seg0[t.a]) + t.nb * NT + c0;
             const int part = t.mt * kCtas + rank;                // of the tiles of 256 weight rows
             if (SWIGLU) {
                 if (part >= m_blocks) return;
-                float factor = 0.f;                              // of row 32 (c0 / 32) + lane
-#pragma unroll
-                for (int i = 0; i < (NT + 31) / 32; ++i)
-                    if (c0 / 32 == i) factor = rs[i];
                 uint32_t byte = 0;                               // lane j: scale byte of column j
                 uint32_t top[kMx4Chunk];
 #pragma unroll
                 for (int j = 0; j < kMx4Chunk; ++j) {
-                    const float s = __shfl_sync(0xffffffffu, factor, c0 % 32 + j);
-                    const float gs = g[j] * s;
-                    g[j] = __fdividef(gs, 1.0f + __expf(-gs)) * (u[j] * s);
+                    g[j] = __fdividef(g[j], 1.0f + __expf(-g[j])) * u[j];
                     // the 32 lanes are one scale block of h
                     top[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(g[j]) & 0x7FFFFFFFu);
                 }
@@ -725,12 +757,6 @@ __global__ void __launch_bounds__(Mx4Shape<NT>::kThreads, 1)
             const int b = lt & 1;
             const uint32_t acc_phase = static_cast<uint32_t>(lt >> 1) & 1u;
             const int ne = min(NT, t_rows[t.a] - t.nb * NT);     // rows of the tile
-            if (SWIGLU) {
-                const float* row_scale = args.row_scale + t_seg0[t.a] + t.nb * NT;
-#pragma unroll
-                for (int i = 0; i < (NT + 31) / 32; ++i)
-                    rs[i] = 32 * i + static_cast<int>(lane) < ne ? __ldcg(row_scale + 32 * i + lane) : 0.f;
-            }
             if (!wait(&tmem_full[b], acc_phase)) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(b * S::kAcc);

@@ -949,6 +949,8 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
                     static_cast<long long>(I));
     if (H > 65536 || I > 65536 || rows > (int64_t(1) << 26) || T >= (int64_t(1) << 31))
         return fail(PDX_ERR_UNSUPPORTED, "FFN batch too large");
+    if (rows * ((H + 127) / 128) >= (int64_t(1) << 30))   // the split counts its blocks in 32 bits
+        return fail(PDX_ERR_UNSUPPORTED, "FFN batch too large");
     if (E > kMaxExperts) return fail(PDX_ERR_UNSUPPORTED, "E=%lld > %d experts", static_cast<long long>(E), kMaxExperts);
     if (!gathered && T < rows) return fail(PDX_ERR_INVALID, "x has fewer rows than the packed order");
     if (!w || !w->codes || !w->scales) return fail(PDX_ERR_INVALID, "expert weights missing");
@@ -978,8 +980,16 @@ int mx4_tile(int64_t rows, int64_t E) {
     return avg <= 8 ? 16 : (avg <= 56 ? 32 : 112);
 }
 
-// Rows up to which the split takes four warps a row (all rows in flight at once).
-constexpr int64_t kMx4SplitFew = 4 * kPlanSMs;
+// Blocks of 512 columns a warp of the split has in flight.  One while that makes no
+// more warps than are resident (48 an SM), then as many as a row has, to 4.  Measured
+// with one / two / four (us, all launches): 1332 rows of 1056 27.2 / 27.3 / 27.9; 2048 of
+// 4096 246.9 / 246.0 / 245.6; 8192 of 1024 51.3 (one, four: half of it idle) / 49.4 (two);
+// 99,600 of 2048 841 (two) / 831 (four).
+int64_t mx4_split_unroll(int64_t rows, int64_t nkb) {
+    const int64_t blocks = (nkb + 3) / 4;
+    if (rows * blocks <= 48 * kPlanSMs) return 1;
+    return blocks <= 2 ? 2 : 4;
+}
 
 // Tickets of a product: tiles have parts only while they are fewer than the CTAs.
 constexpr int kMx4Tickets = kPlanSMs * kMx4MaxEpi;
@@ -988,7 +998,8 @@ struct Mx4Bufs {
     int nt;
     int64_t tiles;          // token tiles at most, over all experts
     uint8_t* x;             // [2][rows][Hp] pieces of the gathered rows
-    float* row_scale;       // [rows]
+    uint8_t* xs;            // scales of x (Mx4Scales)
+    int64_t x_tiles;        // their tiles (wide token tiles)
     uint8_t* h;             // [2][rows][Ip] pieces
     uint8_t* sf;            // [tiles][Ip / 128][sf_tiles] scale tiles of h
     int sf_tiles;
@@ -1002,7 +1013,9 @@ Mx4Bufs carve_mx4(Carver& c, int64_t rows, int64_t E, int64_t H, int64_t I) {
     b.nt = mx4_tile(rows, E);
     b.tiles = rows / b.nt + std::min(E, rows);
     b.x = static_cast<uint8_t*>(c.take(2 * rows * Hp));
-    b.row_scale = static_cast<float*>(c.take(rows * 4));
+    b.x_tiles = rows / b.nt + E;
+    b.xs = static_cast<uint8_t*>(c.take(b.nt > 32 ? b.x_tiles * (Hp / 128) * 2 * kMx4SfBytes
+                                                   : (32 / b.nt) * (Hp / 128) * (rows + 32) * 16));
     b.h = static_cast<uint8_t*>(c.take(2 * rows * Ip));
     b.sf_tiles = b.nt > 32 ? 2 : 1;
     b.sf = static_cast<uint8_t*>(c.take(b.tiles * (Ip / 128) * b.sf_tiles * kMx4SfBytes));
@@ -1065,7 +1078,7 @@ int encode_mx4_tokens(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 
 struct Mx4Maps {
     CUtensorMap w, ws;      // weight codes and scales
-    CUtensorMap x, h, hs;   // token pieces of both products, scales of h
+    CUtensorMap x, xs, h, hs;   // token pieces of both products and their scales
 };
 
 // The two products on tiles of NT tokens.
@@ -1078,7 +1091,7 @@ int launch_mx4_products(const Mx4Maps& m, Mx4Args gu, Mx4Args down, int64_t tile
     // no more CTAs than K steps
     const int64_t work1 = tiles * ((gu.M / 128 + ctas - 1) / ctas) * (gu.K / kMx4BK);
     const int64_t work2 = tiles * ((down.M / 128 + 2 * ctas - 1) / (2 * ctas)) * (down.K / kMx4BK);
-    auto launch = [&](auto kernel, int64_t work, const CUtensorMap& tokens, const Mx4Args& a) {
+    auto launch = [&](auto kernel, int64_t work, const CUtensorMap& tokens, const CUtensorMap& scales, const Mx4Args& a) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(ctas * std::min(most, work)));
         cfg.blockDim = dim3(S::kThreads);
@@ -1092,10 +1105,10 @@ int launch_mx4_products(const Mx4Maps& m, Mx4Args gu, Mx4Args down, int64_t tile
         attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = S::kPair ? 2 : 1;
-        return cudaLaunchKernelEx(&cfg, kernel, m.w, tokens, m.ws, m.hs, a);
+        return cudaLaunchKernelEx(&cfg, kernel, m.w, tokens, m.ws, scales, a);
     };
-    PDX_PDL_TRY(launch(k_mx4_gemm<NT, true>, work1, m.x, gu));
-    PDX_PDL_TRY(launch(k_mx4_gemm<NT, false>, work2, m.h, down));
+    PDX_PDL_TRY(launch(k_mx4_gemm<NT, true>, work1, m.x, m.xs, gu));
+    PDX_PDL_TRY(launch(k_mx4_gemm<NT, false>, work2, m.h, m.hs, down));
     return PDX_OK;
 }
 
@@ -1119,15 +1132,21 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     if ((st = encode_mx4_tokens(&m.h, b.h, rows, Ip, box))) return st;
     if (pair) {
         if ((st = encode_mx4_scales(&m.ws, w->scales, (slots - 1) * (ss / kMx4SfBytes) + 3 * per))) return st;
+        if ((st = encode_mx4_scales(&m.xs, b.xs, b.x_tiles * (Hp / 128) * 2))) return st;
         if ((st = encode_mx4_scales(&m.hs, b.sf, b.tiles * (Ip / 128) * b.sf_tiles))) return st;
     }
-    const bool few = rows <= kMx4SplitFew;
-    const int64_t split_ctas = few ? rows : (rows + kMx4SplitWarps - 1) / kMx4SplitWarps;
-    PDX_PDL_TRY(launch_pdl(few ? k_mx4_split<kMx4SplitWarps> : k_mx4_split<1>,
-                           dim3(static_cast<unsigned>(std::min<int64_t>(split_ctas, 16 * kPlanSMs))),
-                           dim3(kMx4SplitWarps * 32), 0, stream, static_cast<const uint16_t*>(x), tokens,
-                           static_cast<int>(T), n, static_cast<int>(H), Hp, b.x, b.row_scale, b.tickets,
-                           2 * kMx4Tickets));
+    const int64_t x_pad = rows + 32, nkb = Hp / 128, unroll = mx4_split_unroll(rows, nkb);
+    const Mx4Scales scales{b.xs, pair ? 2 * kMx4SfBytes : 16 * x_pad,
+                           pair ? kMx4SfBytes : (b.nt == 32 ? 4 : 16 * x_pad * nkb)};
+    const int64_t split_warps = rows * ((nkb + 4 * unroll - 1) / (4 * unroll));
+    const int64_t split_ctas = (split_warps + kMx4SplitThreads / 32 - 1) / (kMx4SplitThreads / 32);
+    const auto split = unroll == 1   ? (pair ? k_mx4_split<1, 112> : k_mx4_split<1, 0>)
+                       : unroll == 2 ? (pair ? k_mx4_split<2, 112> : k_mx4_split<2, 0>)
+                                     : (pair ? k_mx4_split<4, 112> : k_mx4_split<4, 0>);
+    PDX_PDL_TRY(launch_pdl(split, dim3(static_cast<unsigned>(std::min<int64_t>(split_ctas, 16 * kPlanSMs))),
+                           dim3(kMx4SplitThreads), 0, stream, static_cast<const uint16_t*>(x), tokens,
+                           static_cast<int>(T), n, static_cast<int>(H), Hp, b.x, scales, offsets, static_cast<int>(E),
+                           b.tickets, 2 * kMx4Tickets));
     Mx4Args gu{};
     gu.offsets = offsets;
     gu.active = active;
@@ -1139,7 +1158,8 @@ int launch_mx4_ffn(const void* x, int64_t T, const int32_t* tokens, const int32_
     gu.rows = n;
     gu.table = static_cast<int>(E);
     gu.max_tiles = static_cast<int>(b.tiles);
-    gu.row_scale = b.row_scale;
+    gu.xs = b.xs;
+    gu.x_pad = static_cast<int>(x_pad);
     gu.sf = b.sf;
     gu.h = b.h;
     gu.y = static_cast<uint16_t*>(y);

@@ -467,3 +467,68 @@ def test_many_long_rows(pdx, tokens, hidden, inter, experts, top_k):
     packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), experts)
     got = pdx.moe_ffn_mxfp4(x, packed, slab)
     _check_rows(got, x, packed, qs, experts)
+
+
+@pytest.mark.parametrize("tokens", (3, 40, 300))      # the three token tiles
+def test_far_outlier_the_weights_ignore(pdx, tokens):
+    """A channel 2^15 times the rest whose weights are zero takes bits only from
+    the 31 values that share its block."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    ws = [torch.randn(2, r, c, device="cuda", generator=gen) * 0.02 for r, c in ((128, 2048), (128, 2048), (2048, 128))]
+    ws[0][:, :, 77], ws[1][:, :, 77] = 0, 0
+    qs = [pdx.quantize_mxfp4(w) for w in ws]
+    slab = pdx.Mxfp4ExpertSlab.from_quantized(*qs)
+    x = torch.randn(tokens, 2048, device="cuda", generator=gen)
+    x[:, 77] = 2.0 ** 15
+    x = x.to(torch.bfloat16)
+    sel = _selected(tokens, 2, 1, seed=1)
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 2)
+    got = pdx.moe_ffn_mxfp4(x, packed, slab).double().cpu().numpy()
+    offsets, order, x64 = packed.offsets.tolist(), packed.tokens.cpu().numpy(), x.double().cpu().numpy()
+    y = np.concatenate([ref.ffn_rows(x64[order[offsets[e]:offsets[e + 1]]], *_weights64(qs, e))[0] for e in range(2)])
+    # 31 of 2048 values off by 2^-21 2^15 = 2^-6 at most: 2^-6 sqrt(31/2048) = 1.9e-3 of gate and of up, 3.8e-3 of h;
+    # the roundings of h and y 2^-8 each: in quadrature 6.7e-3 < 2^-7
+    assert np.linalg.norm(got - y) <= 2.0 ** -7 * np.linalg.norm(y)
+
+
+@pytest.mark.parametrize("tokens,hidden", ((1, 96), (3, 1024), (40, 1056), (300, 2080)))
+def test_blocks_of_far_apart_sizes(pdx, tokens, hidden):
+    """Blocks of 32 channels from 2^-30 to 2^30 times the first, weights the other
+    way round: every block counts alike, and a power of two changes no bit of a product."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    ws = [torch.randn(3, r, c, device="cuda", generator=gen) * 0.05 for r, c in ((160, hidden), (160, hidden), (hidden, 160))]
+    x = torch.randn(tokens, hidden, device="cuda", generator=gen).to(torch.bfloat16)
+    sel = _selected(tokens, 3, 1, seed=1)
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), 3)
+    power = torch.exp2(((torch.arange(hidden, device="cuda") // 32 * 17) % 61 - 30).float())
+    qs = [pdx.quantize_mxfp4(ws[0] / power), pdx.quantize_mxfp4(ws[1] / power), pdx.quantize_mxfp4(ws[2])]
+    slab = pdx.Mxfp4ExpertSlab.from_quantized(*qs)
+    got = pdx.moe_ffn_mxfp4((x.float() * power).to(torch.bfloat16), packed, slab)
+    offsets, order = packed.offsets.tolist(), packed.tokens.cpu().numpy()
+    x64, wide = x.double().cpu().numpy(), power.double().cpu().numpy()
+    for e in range(3):
+        rows = slice(offsets[e], offsets[e + 1])
+        if rows.start == rows.stop:
+            continue
+        g, u, d = _weights64(qs, e)
+        y, bound = ref.ffn_rows(x64[order[rows]], g * wide, u * wide, d)     # as if every block were of the first's size
+        assert (np.abs(got[rows].double().cpu().numpy() - y) <= bound).all()
+
+
+# the split of x with one, two and four blocks of 512 columns in flight, narrow and wide token tiles
+SPLITS = ((900, 128, 64, 120, 8), (900, 1024, 64, 60, 8), (4000, 640, 64, 9, 2), (3600, 1056, 64, 120, 2),
+          (1000, 4096, 32, 130, 7), (1300, 2080, 32, 5, 3))
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", SPLITS)
+def test_split_forms(pdx, tokens, hidden, inter, experts, top_k):
+    slab, qs = _slab(pdx, experts, hidden, inter, seed=hidden + tokens)
+    gen = torch.Generator().manual_seed(tokens)
+    x = torch.randn(tokens, hidden, generator=gen) * torch.exp2(torch.randint(-8, 8, (tokens, 1), generator=gen).float())
+    x[:, ::97] *= 300
+    x = x.to(torch.bfloat16).cuda()
+    sel = _selected(tokens, experts, top_k, seed=tokens + 1)
+    packed = pdx.pack(sel, torch.ones(sel.shape, dtype=torch.bfloat16, device="cuda"), experts)
+    got = pdx.moe_ffn_mxfp4(x, packed, slab)
+    _check_rows(got, x, packed, qs, experts)
+    assert torch.equal(got, pdx.moe_ffn_mxfp4(x, packed, slab))
