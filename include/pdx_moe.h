@@ -346,7 +346,12 @@ typedef struct pdx_mxfp4_weights {
 
 /* pdx_moe_ffn_grouped on MXFP4 experts:
  *   y[p] = bf16( Wd (silu(Wg x) * (Wu x)) ),  x = x[tokens[p]] (BF16)
- * with exactly dequantised weights, FP32 sums and one rounding at the end.
+ * with exactly dequantised weights and FP32 sums.  Rounded are the result, once to
+ * BF16; h = silu(Wg x) * (Wu x) before the second product, to within 2^-9 of each
+ * value or 2^-21 of the largest of its 32 (along I, from a multiple of 32), whichever
+ * is more; and values of x that are below 2^-13 of the largest of their 32, by 2^-21 of that
+ * one at most (others enter exactly).  Where x holds an infinity or NaN, or a value
+ * of h overflows, the row of y is NaN throughout.
  * H, I multiples of 32; rows of no active expert are left as they are.
  * active may list experts without rows, in any order.  A list of more than E
  * entries, ids outside [0, E), offsets that fall or leave [0, rows], and experts

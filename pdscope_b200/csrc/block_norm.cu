@@ -12,7 +12,8 @@
 // registers between the reductions, so nothing is read twice.  12,450 rows of
 // H = 2048 combined from k = 8, FP32 stream: 114 us (5.8 TB/s); of H = 4096 with a
 // full sigmoid gate, layer and rms norm: 103 us (5.0 TB/s, issue slots); 64
-// combined rows of 2048: 4.3 us; 3 rows of 5003: 5.0 us.
+// combined rows of 2048: 4.3 us; 3 rows of 5003: 5.0 us.  Many combined rows with an
+// FP32 stream spill 48 bytes a thread, from L1, and other forms 8 or 16.
 #include "pdx_common.cuh"
 
 namespace pdx {

@@ -29,9 +29,11 @@
 // order by the warp that takes its last ticket (FP32, deterministic, nothing waits).
 // Bound by HBM while an expert has few rows, by the power cap at prefill.  Device
 // time of the three launches at H = 2048, I = 768, 128 experts, top-8, with the
-// least the measured copy and BF16 rates allow: one token 16.3 us (3.1), 64 tokens
-// 68-71 (48.5; 6.0-6.6 TB/s between the launches' starts and tails), 12,450 tokens
-// 810-850 (578; 1.11-1.16 PFLOP/s, the BF16 experts take 1042).
+// least the measured copy and BF16 rates allow: one token 16.2 us (3.1), 64 tokens
+// 68-72 (48.5; 6.0-6.6 TB/s between the launches' starts and tails), 12,450 tokens
+// 824-841 (578; 1.12-1.14 PFLOP/s).  The BF16 experts on the same packing, in turn
+// with these: 23.2, 179 and 851 us; back to back for seconds, on the power cap, 12,450
+// tokens take both 966 us (at 1455 MHz, these at 1327).
 // Roles: warp 0 streams weights and scales, the last warp the token pieces, warp
 // 1 issues the MMAs, the others are the epilogue (32 weight rows, = one scale
 // block of h, and every second or fourth 8 token columns each).  Neither launch

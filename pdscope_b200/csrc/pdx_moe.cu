@@ -969,11 +969,16 @@ int check_mx4_ffn(int64_t T, int64_t rows, int64_t E, int64_t H, int64_t I, bool
 
 // Token tile of the MXFP4 path, from the average rows of an expert.  A tile's MMAs
 // cost its full width and its weights are read once, so the tile should hold an
-// expert's rows.  Measured at H = 2048, I = 768, 128 experts (us, uniform routing):
-// 8 rows 68.5 (16) 70.3 (32); 16 rows 84.1 (16) 73.1 (32); 48 rows 121 (32) 122
-// (112), with a skewed router 121 (32) 137 (112); 64 rows 144 (32) 128 (112), skewed
-// 148 and 149; 128 rows 246 (32) 215 (112).  112 is the widest of which two
-// accumulators of gate and up (2 x 112 columns each) and the scales fit TMEM.
+// expert's rows.  Measured (us, uniform routing) at H = 2048, I = 768, 128 experts:
+// 8 rows 68.2 (16) 69.6 (32); 16 rows 86.0 (16) 72.8 (32); 56 rows 125 (32) 123 (112),
+// with a skewed router 48 rows 121 (32) 137 (112); 80 rows 171 (32) 131 (112).  At
+// 4096, 1536, 32 experts: 8 rows 66.2, 68.0; 16 rows 82.1, 70.6; 56 rows 122, 116; 80
+// rows 161, 119.  At 1024, 512, 64: 22.1, 22.6; 26.1, 23.7; 35.4, 38.0; 45.4, 41.0.  At 640, 1280, 16,
+// where no tile fills the SMs: 16.5, 17.0; 19.0, 19.0; 22.1, 27.3; 25.4, 29.8.  The host
+// does not know the counts, so the average is over every expert that could have a row:
+// a router that uses few of them gets narrower tiles than their rows want, and reads
+// their weights once a tile.  112 is the widest of which two accumulators of gate and up
+// (2 x 112 columns each) and the scales fit TMEM.
 int mx4_tile(int64_t rows, int64_t E) {
     const int64_t est = std::max<int64_t>(1, std::min(E, rows));
     const int64_t avg = (rows + est - 1) / est;

@@ -196,8 +196,11 @@ class Mxfp4ExpertSlab:
 def moe_ffn_mxfp4(x, packed, slab, out=None):
     """Unweighted expert rows [T*k, H] of a packed batch on MXFP4 experts:
     ``out[p] = down(silu(gate(x[t])) * up(x[t]))`` for packed row p of token t,
-    with FP32 sums and one rounding to BF16.  ``packed`` is ``pack``'s result
-    for the batch ``x`` [T, H]."""
+    with exact weights and FP32 sums.  Rounded are the result, once to BF16; the
+    input of ``down``, to within 2**-9 of each value or 2**-21 of the largest of its
+    32; and values of x below 2**-13 of the largest of their 32, by 2**-21 of that
+    one at most.  A row of x with an infinity or NaN gives rows of NaN.  ``packed``
+    is ``pack``'s result for the batch ``x`` [T, H]."""
     _require_cuda_bf16("x", x, 2)
     t_count, hidden = x.shape
     if not isinstance(slab, Mxfp4ExpertSlab) or not isinstance(packed, Packed):
