@@ -562,12 +562,14 @@ def check_slab(slab, experts, hidden, device):
     channels on ``device`` cannot run."""
     if slab.hidden != hidden:
         raise ValueError("activation and expert hidden sizes differ")
-    slots, mx = slab.slot_of_expert, is_mxfp4(slab)
+    # a BF16 slab may be any object with the struct and the sizes
+    slots, mx = getattr(slab, "slot_of_expert", None), is_mxfp4(slab)
+    memory = [t for t in (slab.codes if mx else getattr(slab, "storage", None), slots) if t is not None]
     # the device reads slot_of_expert[e] unchecked; without it a BF16 slab may hold the first experts only,
     # and an expert behind them sets the error word
     if (slots is not None and slots.shape[0] < experts) or (mx and slots is None and slab.num_slots < experts):
         raise ValueError("the slab holds fewer experts than the routing names")
-    if (slab.codes if mx else slab.storage).device != device or (slots is not None and slots.device != device):
+    if any(t.device != device for t in memory):
         raise ValueError("the activations, the router and the slab must be on one device")
 
 

@@ -191,8 +191,11 @@ def test_stack_refuses_slabs_that_do_not_fit():
             ResidentMoEStack([gate, gate], [slab, bad])
     with pytest.raises(ValueError, match="alike"):
         ResidentMoEStack([gate, torch.zeros(5, 64, dtype=torch.bfloat16)], [slab, slab])
-    # fewer slots than experts is an error of the routing, not of a BF16 slab
+    # fewer slots than experts is an error of the routing, not of a BF16 slab, which may be any object of the sizes
     ResidentMoEStack([gate], [_bf16_slab(3, 64, 64)])
+    bare = _bf16_slab(4, 64, 64)
+    del bare.storage, bare.slot_of_expert
+    ResidentMoEStack([gate], [bare])
 
 
 @pytest.mark.parametrize("dtype,at", ((0, 257), (1, 257), (2, 258), (2, 257)))
